@@ -217,7 +217,7 @@ def _plain_gate_norm(st):
 
 
 def _plain_quantize(x):
-    scale = x.float().abs().amax(1) / 127.0
+    scale = (x.double().abs().amax(1) / 127.0).float()  # the nearest fp32 value: torch divides fp32 by a number as a product with its reciprocal
     q = torch.round(x.double() / torch.where(scale > 0, scale, 1.0).double()[:, None])  # 64 bits: a value next to a border falls on its own side
     return q.float(), scale
 
@@ -340,7 +340,7 @@ def _exact_gate_norm(st):
 def _exact_product(st, x, epi):
     """The rows x, values of the storage type, in steps of the 32-bit scale."""
     largest = x.abs().max(1, keepdim=True).values
-    step = (largest.float() / 127.0).double()
+    step = (largest / 127.0).float().double()
     whole = torch.where(step > 0, x / step.clamp_min(1e-300), torch.zeros_like(x)).round()
     o = (whole * step) @ (_wide(st["w"]) * _wide(st["w_scale"])[:, None]).T + _wide(st["bias"])
     if epi == "gelu":
