@@ -28,7 +28,7 @@ def _engine(dtype):
     """The handle that a program keeps: the smallest engine of that type."""
     from ecad_amd.engine import EcadEngine
 
-    return EcadEngine(num_layers=1, num_heads=2, caption_channels=64, max_batch=1, max_tokens=64, max_text_tokens=8, dtype=TYPES[dtype])
+    return EcadEngine(num_layers=1, num_heads=16, caption_channels=64, max_batch=1, max_tokens=64, max_text_tokens=8, dtype=TYPES[dtype])
 
 
 # ---- cases ----------------------------------------------------------------------------------------------------------------------------------------------
