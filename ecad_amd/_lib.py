@@ -10,7 +10,7 @@ import os
 from pathlib import Path
 
 LIB_NAME = "libecad_hip.so"
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 ECAD_DTYPE_F16, ECAD_DTYPE_BF16, ECAD_DTYPE_F32 = 0, 1, 2
 ECAD_E_INVALID, ECAD_E_HIP, ECAD_E_NOT_READY, ECAD_E_UNSUPPORTED = -1, -2, -3, -4
@@ -113,6 +113,27 @@ class EcadFluxStats(C.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
+class EcadGateNorm(C.Structure):
+    _fields_ = [
+        ("h", C.c_void_p), ("ldh", C.c_int64),
+        ("y", C.c_void_p), ("ldy", C.c_int64),
+        ("h_out", C.c_void_p), ("ldho", C.c_int64),
+        ("n_out", C.c_void_p), ("ldn", C.c_int64),
+        ("q", C.c_void_p), ("ldq", C.c_int64),
+        ("q_scale", C.c_void_p),
+        ("post_weight", C.c_void_p),
+        ("pre_weight", C.c_void_p),
+        ("gate_table", C.c_void_p),
+        ("gate_mod", C.c_void_p), ("gate_mod_stride", C.c_int64),
+        ("table_shift", C.c_void_p),
+        ("table_scale", C.c_void_p),
+        ("mod_shift", C.c_void_p),
+        ("mod_scale", C.c_void_p), ("mod_stride", C.c_int64),
+        ("M", C.c_int32), ("D", C.c_int32), ("rows_per_batch", C.c_int32), ("post", C.c_int32), ("pre", C.c_int32),
+        ("resid_scale", C.c_float), ("eps", C.c_float),
+    ]
+
+
 _P = C.c_void_p
 _I = C.c_int
 _I64 = C.c_int64
@@ -154,6 +175,11 @@ SIGNATURES = {
     "ecad_op_ln_modulate": (_I, [_P, _P, _P, _I, _I, _P, _P, _P, _P, _I64, _I, _P]),
     "ecad_op_cache_accumulate": (_I, [_P, _P, _I, _I, _I, C.POINTER(_P), C.POINTER(_P), C.POINTER(_P), _I64, _I, _P]),
     "ecad_op_attention": (_I, [_P, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I, _I, _I, _I, _I, _P, _P]),
+    "ecad_op_quantize_int8": (_I, [_P, _P, _I64, _P, _I64, _P, _I, _I, _P]),
+    "ecad_op_gemm_int8": (_I, [_P, _I, _I, _P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I, _I, _I, _I, _P]),
+    "ecad_op_gate_norm": (_I, [_P, C.POINTER(EcadGateNorm), _P]),
+    "ecad_op_rope_table": (_I, [_P, _P, _I, C.POINTER(C.c_int32), _I, _I, _I, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, _P, _P]),
+    "ecad_op_rope": (_I, [_P, _P, C.POINTER(_I64), _P, C.POINTER(_I64), _I, _P, C.POINTER(_I64), _P, C.POINTER(_I64), _I, _P, _I, _P, _I64, _I, _I, _I, _I, _I, _I, _P]),
     "ecad_vae_create": (_I, [_I, _I, C.POINTER(_P)]),
     "ecad_vae_destroy": (None, [_P]),
     "ecad_vae_last_error": (C.c_char_p, [_P]),

@@ -1,0 +1,324 @@
+// gemm_int8.h -- 8-bit integer products with a scale per row (token) and per column (output channel):
+//
+//   o[m][n] = act(sa[m] sw[n] sum_k A[m][k] W[n][k] + bias[n]),   epilogue 3: resid'[m][n] = resid[m][n] + (gt[n] + gm[sample][n]) T(o[m][n])
+//
+// The sums are whole numbers in 32 bits (K < 2^17: 127^2 K < 2^31), so no order of K changes them and every kernel here gives the same bits.  The product of the
+// two scales, the bias, the activation and the gate are fp32; o is rounded once to the storage type, and the residual takes the rounded o (it is what a cache of
+// the sub-layer holds and replays).  A row whose scale is NaN comes out NaN.
+//
+// Operands: rows of 8-bit integers on 16 bytes, any M, N, K.  The last 16-byte piece of a row may reach past column K: it stays inside the aligned 16 bytes that
+// hold a value of the row, and the bytes behind K are masked on the W side (zero times anything is zero).
+#pragma once
+#include "row_ops.h"
+
+namespace ecad {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+enum Int8Epi { I8_BIAS = 0, I8_GELU = 1, I8_SILU = 2, I8_RESID = 3 };
+
+struct Int8GemmArgs {
+  const int8_t* A;
+  const int8_t* W;
+  const float* sa;
+  const float* sw;
+  const float* bias;
+  void* out;
+  const void* resid;
+  void* resid_out;
+  const float* gate_table;
+  const void* gate_mod;
+  int64_t lda, ldw, ldo, ldr, ldro, gate_stride;
+  int M, N, K, epi, rows_per_batch;
+};
+
+ECAD_DEV i32x4 mfma_i8(const Pack8& a, const Pack8& b, i32x4 c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a.u), __builtin_bit_cast(i32x4, b.u), c, 0, 0, 0);
+}
+
+// 16 bytes per lane from base + off (32-bit lane offsets, uniform base) to LDS at lds_off + 16 lane.  In asm, as glds16_raw: the kernel owns the waits.
+ECAD_DEV void lds_dma16(const void* base, unsigned off, unsigned lds_off) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0" : "=&s"(keep) : "v"(off), "s"(base), "s"(lds_off) : "memory");
+}
+
+// keeps the first n bytes of a 16-byte piece
+ECAD_DEV void keep_bytes(Pack8& p, int n) {
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    const int left = n - 4 * d;
+    p.u[d] = left >= 4 ? p.u[d] : (left <= 0 ? 0u : p.u[d] & ((1u << (8 * left)) - 1u));
+  }
+}
+
+// The fp32 value before its rounding to the storage type, in every kernel the same: without the pin the compiler may fuse the last fma with the conversion
+// (v_fma_mixlo_f16, one rounding instead of two) in one kernel and not in another.
+ECAD_DEV float pinned(float v) {
+  asm("" : "+v"(v));
+  return v;
+}
+ECAD_DEV float int8_act(float v, int epi) {
+  v = pinned(v);
+  if (epi == I8_GELU) v = pinned(gelu_tanh(v));
+  if (epi == I8_SILU) v = pinned(silu(v));
+  return v;
+}
+
+// XCD-aware order: workgroups b, b + 8, ... share an XCD and get a run of neighbouring tiles, walked in strips of four tile rows, so that the tiles in flight on one
+// L2 share their A and W rows
+ECAD_DEV void int8_tile_of(int bid, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int total = tiles_m * tiles_n;
+  const int q = total >> 3, r = total & 7, xcd = bid & 7, idx = bid >> 3;
+  bid = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+  const int strip = bid / (4 * tiles_n), in = bid - strip * 4 * tiles_n;
+  const int rows = tiles_m - 4 * strip < 4 ? tiles_m - 4 * strip : 4;
+  tn = in / rows;
+  tm = 4 * strip + in - tn * rows;
+}
+
+// Epilogue of a wave's block from its accumulators: lane (l15, g) holds row m = 16 i + l15, columns 16 j + 4 g .. + 3 of fragment (i, j).  Two neighbouring fragments
+// swap halves between lane rows, so a lane ends with eight consecutive columns: one 16-byte access per pair of fragments, 64 contiguous bytes of each of 16 rows.
+template <typename T, int FM, int FN, typename AccFn>
+ECAD_DEV void int8_epilogue(const Int8GemmArgs& p, int m_base, int n_base, AccFn&& acc) {
+  const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+  float sa[FM];
+  const T* gate[FM];
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int m = m_base + 16 * i + l15 < p.M ? m_base + 16 * i + l15 : p.M - 1;
+    sa[i] = p.sa[m];
+    gate[i] = reinterpret_cast<const T*>(p.gate_mod) + (p.epi == I8_RESID ? (int64_t)(m / p.rows_per_batch) * p.gate_stride : 0);
+  }
+  auto columns = [&](const float* v, int n, f32x4& f) {
+    f = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if (!v) return;
+    if (n + 3 < p.N) {
+      f = reinterpret_cast<const Floats4*>(v + n)->f;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 3; ++r)
+        if (n + r < p.N) f[r] = v[n + r];
+    }
+  };
+  static_for<(FN + 1) / 2>([&](auto jh) {
+    constexpr int j = 2 * decltype(jh)::value;
+    constexpr bool pair = j + 1 < FN;
+    f32x4 sw[2], bias[2];
+#pragma unroll
+    for (int h = 0; h < (pair ? 2 : 1); ++h) {
+      columns(p.sw, n_base + 16 * (j + h) + 4 * g, sw[h]);
+      columns(p.bias, n_base + 16 * (j + h) + 4 * g, bias[h]);
+    }
+    // where this lane's columns lie after the swap
+    const int n = pair ? n_base + 16 * (j + (g & 1)) + 8 * (g >> 1) : n_base + 16 * j + 4 * g;
+    const int left = p.N - n < (pair ? 8 : 4) ? p.N - n : (pair ? 8 : 4);
+    float table[8];
+    if (p.epi == I8_RESID) {
+      if (p.gate_table) load_floats(p.gate_table + n, left, table);
+      else
+#pragma unroll
+        for (int e = 0; e < 8; ++e) table[e] = p.gate_mod ? 0.f : 1.f;
+    }
+    static_for<FM>([&](auto ic) {
+      constexpr int i = decltype(ic)::value;
+      const int m = m_base + 16 * i + l15;
+      Pack8 v;
+      v.u = (u32x4){0, 0, 0, 0};
+#pragma unroll
+      for (int h = 0; h < (pair ? 2 : 1); ++h) {
+        const i32x4 a = h ? acc(ic, std::integral_constant<int, pair ? j + 1 : j>{}) : acc(ic, std::integral_constant<int, j>{});
+        float o[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = int8_act(__builtin_fmaf((float)a[r], sa[i] * sw[h][r], bias[h][r]), p.epi);
+        v.u[2 * h] = pack2<T>(o[0], o[1]);
+        v.u[2 * h + 1] = pack2<T>(o[2], o[3]);
+      }
+      if constexpr (pair) {
+        unsigned a0 = v.u[0], a1 = v.u[1], b0 = v.u[2], b1 = v.u[3];
+        swap_rows16(a0, b0);
+        swap_rows16(a1, b1);
+        v.u = (u32x4){a0, a1, b0, b1};
+      }
+      if (m < p.M) {
+        if (p.out) {
+          T* o = reinterpret_cast<T*>(p.out) + (int64_t)m * p.ldo + n;
+          if (!pair && left == 4) reinterpret_cast<Bytes8*>(o)->u = (u32x2){v.u[0], v.u[1]};
+          else store_piece<T>(o, v, left);
+        }
+        if (p.epi == I8_RESID) {
+          float o[8], h[8], gm[8];
+          unpack8<T>(v, o);
+          unpack8<T>(load_piece<T>(reinterpret_cast<const T*>(p.resid) + (int64_t)m * p.ldr + n, left), h);
+          if (p.gate_mod) unpack8<T>(load_piece<T>(gate[i] + n, left), gm);
+          else
+#pragma unroll
+            for (int e = 0; e < 8; ++e) gm[e] = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) h[e] = pinned(__builtin_fmaf(table[e] + gm[e], o[e], h[e]));
+          store_piece<T>(reinterpret_cast<T*>(p.resid_out) + (int64_t)m * p.ldro + n, pack8<T>(h), left);
+        }
+      }
+    });
+  });
+}
+
+// BM x BN tile on WM x WN waves.  A K-step is 128 bytes of every row of the tile: pieces of eight rows (1 KiB) travel straight to LDS, 16-byte chunks
+// XOR-swizzled by (row >> 1) & 7 on the source side, so that the fragment reads (16 rows x 16 bytes) meet every bank once.  One barrier per step, STAGES steps in a ring.
+template <typename T, int BM, int BN, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(WM * WN * 64) void gemm_int8_kernel(const Int8GemmArgs p) {
+  constexpr int NW = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
+  constexpr int A_BYTES = BM * 128, STAGE_BYTES = (BM + BN) * 128;
+  constexpr int PIECES = (BM + BN) / 8, PPW = (PIECES + NW - 1) / NW;  // not a multiple of the waves: the last ones fetch the first pieces again (same bytes, same place)
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % WM, wn = wave / WM;
+  const int l15 = lane & 15, g = lane >> 4;
+  int tm, tn;
+  int8_tile_of(blockIdx.x, (p.M + BM - 1) / BM, (p.N + BN - 1) / BN, tm, tn);
+  const int m0 = tm * BM, n0 = tn * BN;
+  const char* a_tile = reinterpret_cast<const char*>(p.A) + (int64_t)m0 * p.lda;
+  const char* w_tile = reinterpret_cast<const char*>(p.W) + (int64_t)n0 * p.ldw;
+  const unsigned lds = __builtin_amdgcn_readfirstlane(lds_offset(smem));
+
+  unsigned row_off[PPW], chunk[PPW], dst[PPW];  // lane offset of the row, of the 16-byte chunk in the step; LDS place of the piece
+  const char* base[PPW];
+#pragma unroll
+  for (int i = 0; i < PPW; ++i) {
+    int piece = wave + NW * i;
+    if (piece >= PIECES) piece -= PIECES;
+    const bool of_a = piece < BM / 8;
+    const int r = (of_a ? piece : piece - BM / 8) * 8 + (lane >> 3);
+    const int rows = of_a ? p.M - m0 : p.N - n0;
+    row_off[i] = (unsigned)(r < rows ? r : rows - 1) * (unsigned)(of_a ? p.lda : p.ldw);
+    chunk[i] = (unsigned)(((lane & 7) ^ ((r >> 1) & 7)) * 16);
+    dst[i] = __builtin_amdgcn_readfirstlane(piece * 1024);
+    base[i] = of_a ? a_tile : w_tile;
+  }
+  const int nk = (p.K + 127) >> 7;
+  auto issue = [&](int kt, int slot) {
+    const int k0 = kt * 128;
+    if (k0 + 128 <= p.K) {
+#pragma unroll
+      for (int i = 0; i < PPW; ++i) lds_dma16(base[i] + k0, row_off[i] + chunk[i], lds + slot * STAGE_BYTES + dst[i]);
+    } else {  // the step that holds the end of K: chunks behind it read the start of their row instead (masked below)
+#pragma unroll
+      for (int i = 0; i < PPW; ++i) {
+        const unsigned k = (unsigned)k0 + chunk[i];
+        lds_dma16(base[i], row_off[i] + (k < (unsigned)p.K ? k : 0u), lds + slot * STAGE_BYTES + dst[i]);
+      }
+    }
+  };
+
+  i32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) acc[i][j] = (i32x4){0, 0, 0, 0};
+  const int swz = (l15 >> 1) & 7;
+  const int a_row = (wm * (BM / WM) + l15) * 128, w_row = A_BYTES + (wn * (BN / WN) + l15) * 128;
+  auto step = [&](int slot, int left, auto last) {
+    const char* st = smem + slot * STAGE_BYTES;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      Pack8 af[FM], wf[FN];
+      const int at = ((4 * s + g) ^ swz) * 16;
+#pragma unroll
+      for (int i = 0; i < FM; ++i) af[i] = lds_read16(st + a_row + i * 2048 + at);
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        wf[j] = lds_read16(st + w_row + j * 2048 + at);
+        if constexpr (decltype(last)::value) keep_bytes(wf[j], left - (4 * s + g) * 16);
+      }
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int i = 0; i < FM; ++i) acc[i][j] = mfma_i8(wf[j], af[i], acc[i][j]);
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (s < nk) issue(s, s);
+  int slot = 0;
+  for (int kt = 0; kt < nk; ++kt) {
+    // this wave's pieces of step kt have landed (later ones may be in flight), its reads of the slot that is filled next are done; the barrier says so for all waves
+    if (STAGES > 2 && kt + STAGES - 2 < nk) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(PPW * (STAGES - 2)) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (kt + STAGES - 1 < nk) issue(kt + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
+    const int left = p.K - kt * 128;
+    if (left >= 128) step(slot, left, std::false_type{});
+    else step(slot, left, std::true_type{});
+    slot = slot + 1 == STAGES ? 0 : slot + 1;
+  }
+  int8_epilogue<T, FM, FN>(p, m0 + wm * (BM / WM), n0 + wn * (BN / WN), [&](auto ic, auto jc) -> i32x4 { return acc[decltype(ic)::value][decltype(jc)::value]; });
+}
+
+// Few rows (M <= 16 FM): the time is the reading of W.  A workgroup owns 16 columns; its waves take turns along K in steps of 64 bytes per row, operands go
+// straight to registers in the matrix instruction's layout (each W byte is used by one wave only: nothing to share through LDS), several steps in flight; the waves'
+// sums meet in LDS.
+template <typename T, int FM, int NW>
+__global__ __launch_bounds__(NW * 64) void gemm_int8_rows_kernel(const Int8GemmArgs p) {
+  __shared__ int part[NW][FM * 256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16;
+  const int8_t* wp = p.W + (int64_t)(n0 + l15 < p.N ? n0 + l15 : p.N - 1) * p.ldw;
+  const int8_t* ap[FM];
+#pragma unroll
+  for (int i = 0; i < FM; ++i) ap[i] = p.A + (int64_t)(16 * i + l15 < p.M ? 16 * i + l15 : p.M - 1) * p.lda;
+  i32x4 acc[FM];
+#pragma unroll
+  for (int i = 0; i < FM; ++i) acc[i] = (i32x4){0, 0, 0, 0};
+  constexpr int U = 4;
+  int k = wave * 64 + 16 * g;  // this lane's first byte; the wave's steps lie NW * 64 apart
+  for (; k - 16 * g + (U - 1) * NW * 64 + 64 <= p.K; k += U * NW * 64) {
+    Pack8 w[U], a[U][FM];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      w[u] = gload16(wp + k + u * NW * 64);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) a[u][i] = gload16(ap[i] + k + u * NW * 64);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < FM; ++i) acc[i] = mfma_i8(w[u], a[u][i], acc[i]);
+  }
+  for (; k - 16 * g < p.K; k += NW * 64) {
+    Pack8 w, a[FM];
+    w.u = (u32x4){0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < FM; ++i) a[i].u = (u32x4){0, 0, 0, 0};
+    if (k < p.K) {
+      w = gload16(wp + k);
+      keep_bytes(w, p.K - k);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) a[i] = gload16(ap[i] + k);
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) acc[i] = mfma_i8(w, a[i], acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) part[wave][i * 256 + l15 * 16 + 4 * g + r] = acc[i][r];
+  __syncthreads();
+  for (int it = threadIdx.x; it < FM * 256; it += NW * 64) {
+    const int m = it >> 4, n = n0 + (it & 15);
+    if (m >= p.M || n >= p.N) continue;
+    int sum = part[0][it];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) sum += part[w][it];
+    const float o = int8_act(__builtin_fmaf((float)sum, p.sa[m] * p.sw[n], p.bias ? p.bias[n] : 0.f), p.epi);
+    const float rounded = round_elem<T>(o);
+    if (p.out) reinterpret_cast<T*>(p.out)[(int64_t)m * p.ldo + n] = (T)o;
+    if (p.epi == I8_RESID) {
+      float gate = p.gate_table ? p.gate_table[n] : (p.gate_mod ? 0.f : 1.f);
+      if (p.gate_mod) gate += (float)reinterpret_cast<const T*>(p.gate_mod)[(int64_t)(m / p.rows_per_batch) * p.gate_stride + n];
+      reinterpret_cast<T*>(p.resid_out)[(int64_t)m * p.ldro + n] = (T)pinned(__builtin_fmaf(gate, rounded, (float)reinterpret_cast<const T*>(p.resid)[(int64_t)m * p.ldr + n]));
+    }
+  }
+}
+
+}  // namespace ecad

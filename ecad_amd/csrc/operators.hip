@@ -1,0 +1,268 @@
+// operators.hip -- the single-op entry points of an 8-bit transformer block (operators.h): argument checks and launches of row_ops.h, gate_norm.h, rope.h and
+// gemm_int8.h.  A unit of its own, compiled without -ffast-math: the 8-bit rounding needs the divisions and remainders it writes down.
+#include "operators.h"
+
+#include <math.h>
+#include <stdarg.h>
+#include <stdio.h>
+
+#include <atomic>
+
+#include "../../include/ecad_hip.h"
+#include "gate_norm.h"
+#include "gemm_int8.h"
+#include "rope.h"
+
+namespace ecad {
+namespace {
+
+int refuse(OpStatus& st, int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(st.msg, sizeof st.msg, fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+int launched(OpStatus& st, const char* what) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? ECAD_OK : refuse(st, ECAD_E_HIP, "%s: launch failed: %s", what, hipGetErrorString(e));
+}
+
+bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+// more than 64 KiB of LDS has to be asked for once per kernel and device
+int allow_lds(std::atomic<uint64_t>& done, const void* kernel, int bytes, OpStatus& st) {
+  int dev = 0;
+  if (bytes <= 65536) return ECAD_OK;
+  if (hipGetDevice(&dev) == hipSuccess && dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1)) return ECAD_OK;
+  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return refuse(st, ECAD_E_HIP, "LDS of %d bytes refused: %s", bytes, hipGetErrorString(e));
+  if (dev < 64) done.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
+  return ECAD_OK;
+}
+
+constexpr int MAX_ROW = 32768;       // widest row that the norms hold in registers (1024 lanes x 4 pieces)
+constexpr int MAX_INT8_K = 131071;   // 128^2 K stays below 2^31
+
+constexpr int row_slots(int waves) { return waves >= 4 ? 1 : 4 / waves; }  // rows a workgroup works on at a time
+
+// ---- 8-bit rows ----------------------------------------------------------------------------------------------------------------------------------------------
+
+template <typename T> int quantize_t(const OpCtx& ctx, const QuantizeArgs& a, OpStatus& st) {
+  const int pieces = (a.K + 7) / 8;
+  auto grid = [&](int rows) { return dim3((unsigned)(((int64_t)a.M + rows - 1) / rows)); };
+#define ECAD_QUANT(WAVES, CH) hipLaunchKernelGGL((quantize_rows_kernel<T, WAVES, CH>), grid(row_slots(WAVES)), dim3(WAVES > 4 ? WAVES * 64 : 256), 0, ctx.stream, a)
+  if (pieces <= 64) ECAD_QUANT(1, 1);
+  else if (pieces <= 128) ECAD_QUANT(1, 2);
+  else if (pieces <= 192) ECAD_QUANT(1, 3);
+  else if (pieces <= 256) ECAD_QUANT(4, 1);
+  else if (pieces <= 512) ECAD_QUANT(4, 2);
+  else if (pieces <= 768) ECAD_QUANT(4, 3);
+  else if (pieces <= 1024) ECAD_QUANT(4, 4);
+  else if (pieces <= 2048) ECAD_QUANT(4, 8);
+  else if (pieces <= 4096) ECAD_QUANT(16, 4);
+  else ECAD_QUANT(16, 16);
+#undef ECAD_QUANT
+  return launched(st, "quantize_int8");
+}
+
+// ---- norms ---------------------------------------------------------------------------------------------------------------------------------------------------
+
+template <typename T> int gate_norm_t(const OpCtx& ctx, GateNormArgs& a, OpStatus& st) {
+  const int pieces = (a.D + 7) / 8;
+  // rows a wave (or a workgroup of a wide row) takes: enough to reuse the channel vectors, few enough to leave work for the whole chip
+  auto group = [&](int slots) {
+    int r = 1;
+    while (r < 16 && (int64_t)a.M >= (int64_t)2 * r * slots * 8 * ctx.num_cus) r *= 2;
+    a.rows_per_group = r;
+    return dim3((unsigned)((a.M + (int64_t)slots * r - 1) / ((int64_t)slots * r)));
+  };
+#define ECAD_NORM(WAVES, CH) hipLaunchKernelGGL((gate_norm_kernel<T, WAVES, CH>), group(row_slots(WAVES)), dim3(WAVES > 4 ? WAVES * 64 : 256), 0, ctx.stream, a)
+  if (pieces <= 64) ECAD_NORM(1, 1);
+  else if (pieces <= 128) ECAD_NORM(1, 2);
+  else if (pieces <= 192) ECAD_NORM(1, 3);
+  else if (pieces <= 256) ECAD_NORM(4, 1);
+  else if (pieces <= 512) ECAD_NORM(4, 2);
+  else if (pieces <= 1024) ECAD_NORM(4, 4);
+  else if (pieces <= 2048) ECAD_NORM(16, 2);
+  else ECAD_NORM(16, 4);
+#undef ECAD_NORM
+  return launched(st, "gate_norm");
+}
+
+// ---- products ------------------------------------------------------------------------------------------------------------------------------------------------
+
+template <typename T, int BM, int BN, int WM, int WN, int STAGES> int launch_tile(const OpCtx& ctx, const Int8GemmArgs& a, OpStatus& st) {
+  static std::atomic<uint64_t> done{0};
+  constexpr int bytes = STAGES * (BM + BN) * 128;
+  const int rc = allow_lds(done, (const void*)gemm_int8_kernel<T, BM, BN, WM, WN, STAGES>, bytes, st);
+  if (rc) return rc;
+  const int64_t tiles = ((int64_t)a.M + BM - 1) / BM * (((int64_t)a.N + BN - 1) / BN);
+  if (tiles > 0x7fffffff) return refuse(st, ECAD_E_UNSUPPORTED, "gemm_int8: %lld tiles are more than one launch takes", (long long)tiles);
+  hipLaunchKernelGGL((gemm_int8_kernel<T, BM, BN, WM, WN, STAGES>), dim3((unsigned)tiles), dim3(WM * WN * 64), bytes, ctx.stream, a);
+  return launched(st, "gemm_int8");
+}
+
+template <typename T> int gemm_int8_t(const OpCtx& ctx, const Int8GemmArgs& a, int kernel, OpStatus& st) {
+  if (kernel == ECAD_I8_K_ROWS && a.M > 64) return refuse(st, ECAD_E_UNSUPPORTED, "gemm_int8: the few-rows kernel takes up to 64 rows, got %d", a.M);
+  if (kernel == ECAD_I8_K_AUTO) {
+    auto tiles = [&](int bm, int bn) { return ((int64_t)a.M + bm - 1) / bm * (((int64_t)a.N + bn - 1) / bn); };
+    if (a.M <= 64) kernel = ECAD_I8_K_ROWS;
+    else if (tiles(256, 256) >= ctx.num_cus) kernel = ECAD_I8_K_TILE256;
+    else if (tiles(128, 128) >= ctx.num_cus) kernel = ECAD_I8_K_TILE128;
+    else kernel = ECAD_I8_K_TILE64;
+  }
+  switch (kernel) {
+    case ECAD_I8_K_ROWS: {
+      const dim3 grid((unsigned)((a.N + 15) / 16));
+      if (a.M <= 16) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 1, 8>), grid, dim3(512), 0, ctx.stream, a);
+      else if (a.M <= 32) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 2, 8>), grid, dim3(512), 0, ctx.stream, a);
+      else hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 4, 8>), grid, dim3(512), 0, ctx.stream, a);
+      return launched(st, "gemm_int8");
+    }
+    case ECAD_I8_K_TILE64: return launch_tile<T, 64, 64, 2, 2, 4>(ctx, a, st);
+    case ECAD_I8_K_TILE128: return launch_tile<T, 128, 128, 2, 2, 2>(ctx, a, st);
+    case ECAD_I8_K_TILE144: return launch_tile<T, 256, 144, 8, 1, 3>(ctx, a, st);
+    case ECAD_I8_K_TILE256: return launch_tile<T, 256, 256, 4, 2, 2>(ctx, a, st);
+    case ECAD_I8_K_TILE288: return launch_tile<T, 256, 288, 4, 2, 2>(ctx, a, st);
+    default: return refuse(st, ECAD_E_INVALID, "gemm_int8: kernel %d unknown", kernel);
+  }
+}
+
+}  // namespace
+
+int op_num_cus(int device) noexcept {
+  static std::atomic<int> known[64];
+  if (device >= 0 && device < 64 && known[device].load(std::memory_order_relaxed)) return known[device].load(std::memory_order_relaxed);
+  int n = 0;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || n < 1) n = 256;
+  if (device >= 0 && device < 64) known[device].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+int op_quantize_int8(const OpCtx& ctx, const QuantizeCall& c, OpStatus& st) noexcept {
+  if (c.M < 0 || c.K < 1 || c.K > MAX_INT8_K) return refuse(st, ECAD_E_INVALID, "quantize_int8: %d rows of %d values (1 to %d values a row)", c.M, c.K, MAX_INT8_K);
+  if (c.M == 0) return ECAD_OK;
+  if (!c.x || !c.q || !c.scale) return refuse(st, ECAD_E_INVALID, "quantize_int8: NULL pointer");
+  if (c.ldx < (c.M > 1 ? c.K : 0) || c.ldq < c.K || c.ldq % 16 || !aligned(c.q, 16) || !aligned(c.x, 2) || !aligned(c.scale, 4))
+    return refuse(st, ECAD_E_INVALID, "quantize_int8: x rows need a stride of at least %d, 8-bit rows start on 16 bytes with a stride of a multiple of 16 (got %lld and %lld)", c.K, (long long)c.ldx,
+                  (long long)c.ldq);
+  const QuantizeArgs a{c.x, c.q, c.scale, c.ldx, c.ldq, c.M, c.K};
+  return ctx.dtype == ECAD_DTYPE_F16 ? quantize_t<f16_t>(ctx, a, st) : quantize_t<bf16_t>(ctx, a, st);
+}
+
+int op_gemm_int8(const OpCtx& ctx, const Int8GemmCall& c, OpStatus& st) noexcept {
+  if (c.M < 0 || c.N < 0 || c.K < 1 || c.K > MAX_INT8_K) return refuse(st, ECAD_E_INVALID, "gemm_int8: M=%d N=%d K=%d (K from 1 to %d)", c.M, c.N, c.K, MAX_INT8_K);
+  if (c.epi < 0 || c.epi > 3) return refuse(st, ECAD_E_INVALID, "gemm_int8: epilogue %d unknown", c.epi);
+  if (c.M == 0 || c.N == 0) return ECAD_OK;
+  if (!c.A || !c.W || !c.sa || !c.sw || (c.epi != I8_RESID && !c.out)) return refuse(st, ECAD_E_INVALID, "gemm_int8: NULL pointer");
+  if (c.epi == I8_RESID && (!c.resid || !c.resid_out)) return refuse(st, ECAD_E_INVALID, "gemm_int8: epilogue 3 needs resid");
+  if (!aligned(c.A, 16) || !aligned(c.W, 16) || c.lda % 16 || c.ldw % 16 || c.lda < c.K || c.ldw < c.K || c.lda > (1 << 23) || c.ldw > (1 << 23))
+    return refuse(st, ECAD_E_INVALID, "gemm_int8: 8-bit rows start on 16 bytes with a stride of a multiple of 16, at least %d (got %lld and %lld)", c.K, (long long)c.lda, (long long)c.ldw);
+  if (!aligned(c.sa, 4) || !aligned(c.sw, 4) || !aligned(c.bias, 4) || !aligned(c.gate_table, 4) || !aligned(c.out, 2) || !aligned(c.resid, 2) || !aligned(c.resid_out, 2) || !aligned(c.gate_mod, 2))
+    return refuse(st, ECAD_E_INVALID, "gemm_int8: pointers are not aligned to their type");
+  if ((c.out && c.M > 1 && c.ldo < c.N) || (c.epi == I8_RESID && c.M > 1 && (c.ldr < c.N || c.ldro < c.N))) return refuse(st, ECAD_E_INVALID, "gemm_int8: row strides of the outputs are shorter than %d", c.N);
+  if (c.epi == I8_RESID && c.rows_per_batch < 1) return refuse(st, ECAD_E_INVALID, "gemm_int8: rows_per_batch must be at least 1");
+  Int8GemmArgs a{};
+  a.A = c.A; a.W = c.W; a.sa = c.sa; a.sw = c.sw; a.bias = c.bias; a.out = c.out; a.resid = c.resid; a.resid_out = c.resid_out; a.gate_table = c.gate_table; a.gate_mod = c.gate_mod;
+  a.lda = c.lda; a.ldw = c.ldw; a.ldo = c.ldo; a.ldr = c.ldr; a.ldro = c.ldro; a.gate_stride = c.gate_stride;
+  a.M = c.M; a.N = c.N; a.K = c.K; a.epi = c.epi; a.rows_per_batch = c.rows_per_batch > 0 ? c.rows_per_batch : 1;
+  return ctx.dtype == ECAD_DTYPE_F16 ? gemm_int8_t<f16_t>(ctx, a, c.kernel, st) : gemm_int8_t<bf16_t>(ctx, a, c.kernel, st);
+}
+
+int op_gate_norm(const OpCtx& ctx, const GateNormCall& c, OpStatus& st) noexcept {
+  if (c.M < 0 || c.D < 1) return refuse(st, ECAD_E_INVALID, "gate_norm: %d rows of %d values", c.M, c.D);
+  if (c.D > MAX_ROW) return refuse(st, ECAD_E_UNSUPPORTED, "gate_norm: rows of up to %d values, got %d", MAX_ROW, c.D);
+  if (c.post < NORM_NONE || c.post > NORM_LAYER || c.pre < NORM_NONE || c.pre > NORM_LAYER) return refuse(st, ECAD_E_INVALID, "gate_norm: norm kinds are 0 (none), 1 (rms), 2 (layer)");
+  if (!(c.eps >= 0.f) || !(fabsf(c.resid_scale) < INFINITY)) return refuse(st, ECAD_E_INVALID, "gate_norm: eps %g, residual scale %g", (double)c.eps, (double)c.resid_scale);
+  if (c.rows_per_batch < 1) return refuse(st, ECAD_E_INVALID, "gate_norm: rows_per_batch must be at least 1");
+  if (!c.y && (c.post != NORM_NONE || c.post_weight || c.gate_table || c.gate_mod || c.resid_scale != 1.f || c.pre == NORM_NONE))
+    return refuse(st, ECAD_E_INVALID, "gate_norm: without y there is no gate, post-norm or residual scale, and the pre-norm is what is left to do");
+  if (c.pre == NORM_NONE && (c.pre_weight || c.table_shift || c.table_scale || c.mod_shift || c.mod_scale || c.n_out || c.q))
+    return refuse(st, ECAD_E_INVALID, "gate_norm: weight, modulation and output of a pre-norm that is 'none'");
+  if (c.post == NORM_NONE && c.post_weight) return refuse(st, ECAD_E_INVALID, "gate_norm: weight of a post-norm that is 'none'");
+  if (c.M == 0) return ECAD_OK;
+  if (!c.h || (c.y && !c.h_out) || (c.pre != NORM_NONE && !c.n_out == !c.q) || (c.q && !c.q_scale)) return refuse(st, ECAD_E_INVALID, "gate_norm: NULL pointer, or both n and its 8-bit rows asked for");
+  const int64_t least = c.M > 1 ? c.D : 0;
+  if (c.ldh < least || (c.y && (c.ldy < least || c.ldho < least)) || (c.n_out && c.ldn < least)) return refuse(st, ECAD_E_INVALID, "gate_norm: a row stride is shorter than %d", c.D);
+  if (c.q && (c.ldq < c.D || c.ldq % 16 || !aligned(c.q, 16) || !aligned(c.q_scale, 4))) return refuse(st, ECAD_E_INVALID, "gate_norm: 8-bit rows start on 16 bytes with a stride of a multiple of 16");
+  if (!aligned(c.h, 2) || !aligned(c.y, 2) || !aligned(c.h_out, 2) || !aligned(c.n_out, 2) || !aligned(c.gate_mod, 2) || !aligned(c.mod_shift, 2) || !aligned(c.mod_scale, 2) || !aligned(c.post_weight, 4) ||
+      !aligned(c.pre_weight, 4) || !aligned(c.gate_table, 4) || !aligned(c.table_shift, 4) || !aligned(c.table_scale, 4))
+    return refuse(st, ECAD_E_INVALID, "gate_norm: pointers are not aligned to their type");
+  GateNormArgs a{};
+  a.h = c.h; a.y = c.y; a.h_out = c.h_out; a.n_out = c.n_out; a.q = c.q; a.q_scale = c.q_scale; a.post_weight = c.post_weight; a.pre_weight = c.pre_weight;
+  a.gate_table = c.gate_table; a.table_shift = c.table_shift; a.table_scale = c.table_scale; a.gate_mod = c.gate_mod; a.mod_shift = c.mod_shift; a.mod_scale = c.mod_scale;
+  a.ldh = c.ldh; a.ldy = c.ldy; a.ldho = c.ldho; a.ldn = c.ldn; a.ldq = c.ldq; a.gate_stride = c.gate_stride; a.mod_stride = c.mod_stride;
+  a.M = c.M; a.D = c.D; a.rows_per_batch = c.rows_per_batch; a.post = c.post; a.pre = c.pre; a.resid_scale = c.resid_scale; a.eps = c.eps;
+  return ctx.dtype == ECAD_DTYPE_F16 ? gate_norm_t<f16_t>(ctx, a, st) : gate_norm_t<bf16_t>(ctx, a, st);
+}
+
+int op_rope_table(const OpCtx& ctx, const RopeTableCall& c, OpStatus& st) noexcept {
+  if (c.axes < 1 || c.axes > ROPE_MAX_AXES || !c.axes_dims || c.S < 0) return refuse(st, ECAD_E_INVALID, "rope_table: %d positions on %d axes (1 to %d)", c.S, c.axes, ROPE_MAX_AXES);
+  RopeTableArgs a{};
+  const double two_pi = 6.283185307179586476925;
+  if (!(c.theta > 0) || c.theta == INFINITY || !(c.factor > 0) || c.factor == INFINITY) return refuse(st, ECAD_E_INVALID, "rope_table: theta %g and factor %g must be positive", c.theta, c.factor);
+  if (c.scaling < ECAD_ROPE_NONE || c.scaling > ECAD_ROPE_YARN) return refuse(st, ECAD_E_INVALID, "rope_table: scaling %d unknown", c.scaling);
+  if (c.scaling == ECAD_ROPE_YARN && (!(c.original_length > 0) || !(c.beta_fast > c.beta_slow) || !(c.factor >= 1)))
+    return refuse(st, ECAD_E_INVALID, "rope_table: yarn needs an original length, beta_fast > beta_slow and a factor of at least 1");
+  for (int x = 0; x < c.axes; ++x) {
+    const int d = c.axes_dims[x];
+    if (d < 2 || d % 2 || a.pairs + d / 2 > ROPE_MAX_PAIRS) return refuse(st, ECAD_E_INVALID, "rope_table: axis %d has %d elements (even, at least 2, at most %d over all axes)", x, d, 2 * ROPE_MAX_PAIRS);
+    const double theta = c.scaling == ECAD_ROPE_NTK && d > 2 ? c.theta * pow(c.factor, (double)d / (d - 2)) : c.theta;
+    for (int j = 0; j < d / 2; ++j) {
+      double f = pow(theta, -2.0 * j / d);
+      if (c.scaling == ECAD_ROPE_LINEAR) f /= c.factor;
+      if (c.scaling == ECAD_ROPE_YARN) {
+        double keep = (c.original_length * f / two_pi - c.beta_slow) / (c.beta_fast - c.beta_slow);
+        keep = keep < 0 ? 0 : (keep > 1 ? 1 : keep);
+        f = f * keep + f / c.factor * (1 - keep);
+      }
+      a.turns[a.pairs] = f / two_pi;
+      a.axis[a.pairs++] = (unsigned char)x;
+    }
+  }
+  if (c.S == 0) return ECAD_OK;
+  if (!c.positions || !c.table || !aligned(c.positions, 4) || !aligned(c.table, 8)) return refuse(st, ECAD_E_INVALID, "rope_table: NULL or unaligned pointer");
+  a.positions = c.positions; a.table = c.table; a.positions_float = c.positions_float; a.axes = c.axes; a.S = c.S;
+  a.size = c.scaling == ECAD_ROPE_YARN ? (float)(0.1 * log(c.factor) + 1.0) : 1.0f;
+  const int64_t blocks = ((int64_t)c.S * a.pairs + 255) / 256, most = (int64_t)ctx.num_cus * 32;
+  hipLaunchKernelGGL(rope_table_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, ctx.stream, a);
+  return launched(st, "rope_table");
+}
+
+int op_rope(const OpCtx& ctx, const RopeCall& c, OpStatus& st) noexcept {
+  if (c.B < 0 || c.S < 0 || c.q.H < 1 || c.k.H < 0 || c.D < 2 || c.rot < 2 || c.rot % 2 || c.rot > c.D || c.table_rows < 0)
+    return refuse(st, ECAD_E_INVALID, "rope: %d samples of %d tokens, %d + %d heads of %d elements, %d of them turned (even, 2 to the head's size)", c.B, c.S, c.q.H, c.k.H, c.D, c.rot);
+  if (c.B == 0 || c.S == 0) return ECAD_OK;
+  if (!c.q.x || !c.q.out || (c.k.H && (!c.k.x || !c.k.out)) || !c.table) return refuse(st, ECAD_E_INVALID, "rope: NULL pointer");
+  if (!aligned(c.q.x, 2) || !aligned(c.q.out, 2) || !aligned(c.k.x, 2) || !aligned(c.k.out, 2) || !aligned(c.table, 4) || !aligned(c.index, 4)) return refuse(st, ECAD_E_INVALID, "rope: pointers are not aligned to their type");
+  if (!c.index && c.table_rows < c.S) return refuse(st, ECAD_E_INVALID, "rope: the table has %d rows for %d tokens", c.table_rows, c.S);
+  const bool q_in = c.q.x == c.q.out, k_in = c.k.H == 0 || c.k.x == c.k.out;
+  if (c.k.H && q_in != k_in) return refuse(st, ECAD_E_INVALID, "rope: queries and keys are both turned in place or both not");
+  auto same = [](const RopeHeads& x) { return x.sb == x.ob && x.ss == x.os && x.sh == x.oh; };
+  if (q_in && (!same(c.q) || (c.k.H && !same(c.k)))) return refuse(st, ECAD_E_INVALID, "rope: in place needs the same strides on both sides");
+  RopeArgs a{};
+  a.q = c.q; a.k = c.k; a.table = c.table; a.index = c.index; a.index_stride = c.index_stride; a.S = c.S; a.D = c.D; a.rot = c.rot; a.table_rows = c.table_rows; a.copy = !q_in;
+  a.sign = c.inverse ? -1.f : 1.f;
+  a.tokens = (int64_t)c.B * c.S;
+  a.turning = c.half ? (c.rot / 2 + 7) / 8 : (c.rot + 7) / 8;
+  a.units = c.half ? a.turning + (a.copy ? (c.D - c.rot + 7) / 8 : 0) : (a.copy ? (c.D + 7) / 8 : a.turning);
+  a.groups = (c.q.H + c.k.H + ROPE_HEADS - 1) / ROPE_HEADS;
+  const int64_t per_token = (int64_t)a.units * a.groups;
+  if (per_token > (1 << 24)) return refuse(st, ECAD_E_UNSUPPORTED, "rope: %lld pieces a token", (long long)per_token);
+  a.tokens_per_block = per_token >= 256 ? 1 : (int)(256 / per_token);
+  const int64_t blocks = (a.tokens + a.tokens_per_block - 1) / a.tokens_per_block;
+  if (blocks > 0x7fffffff) return refuse(st, ECAD_E_UNSUPPORTED, "rope: %lld tokens are more than one launch takes", (long long)a.tokens);
+  const dim3 grid((unsigned)blocks), block(256);
+  if (ctx.dtype == ECAD_DTYPE_F16) {
+    if (c.half) hipLaunchKernelGGL((rope_kernel<f16_t, true>), grid, block, 0, ctx.stream, a);
+    else hipLaunchKernelGGL((rope_kernel<f16_t, false>), grid, block, 0, ctx.stream, a);
+  } else {
+    if (c.half) hipLaunchKernelGGL((rope_kernel<bf16_t, true>), grid, block, 0, ctx.stream, a);
+    else hipLaunchKernelGGL((rope_kernel<bf16_t, false>), grid, block, 0, ctx.stream, a);
+  }
+  return launched(st, "rope");
+}
+
+}  // namespace ecad

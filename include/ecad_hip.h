@@ -20,7 +20,7 @@
 extern "C" {
 #endif
 
-#define ECAD_ABI_VERSION 7
+#define ECAD_ABI_VERSION 8
 
 enum {
   ECAD_OK = 0,
@@ -277,6 +277,69 @@ int ecad_op_attention_ex(EcadEngine* e, int kernel, const void* q, int64_t ldq, 
  * also a multiple of 128 keys), else ECAD_E_UNSUPPORTED -- the engine then runs the projection and ecad_op_attention as separate launches, and so can the caller. */
 int ecad_op_qproj_attention(EcadEngine* e, int call_site, const void* x, const void* wq, const float* bq, const void* k, const void* v, int64_t ld_kv,
                             const float* key_bias, void* out, int Bt, int n_tokens, int n_keys, void* stream);
+
+/* ---- the launches of an 8-bit transformer block (ABI 8): quantised rows and products, gated norms, rotary positions -------------------------------------------
+ * Companions of the single-op entry points above for a Linear in 8-bit integers (a scale per token, a scale per output channel), for blocks with norms on both sides of
+ * a sub-layer, and for rotary positions of any head layout.  All of them only launch on `stream` (no allocation, no synchronisation, nothing kept between calls): they
+ * may be captured into a graph, and called from several streams.  They run on the engine's device whatever the current device is, and leave that as it was.
+ * 16-bit tensors have the engine's dtype; rows may have any width and any stride (in elements) at the alignment of an element; 8-bit rows start on 16 bytes with a
+ * stride of a multiple of 16 (so the last 16-byte piece of a row may be read whole; what lies behind the row's values does not matter).
+ * Zero rows: nothing is done. */
+
+/* q[i][k] = x[i][k] / scale[i] rounded to the nearest integer (exactly, ties to even), scale[i] = max_k |x[i][k]| / 127 as fp32.  A row of zeros: scale 0, zeros.
+ * A row with an infinity or a NaN: scale NaN, zeros -- its products are NaN.  1 <= K < 131072.  Weights [N, K] are quantised by the same call, once. */
+int ecad_op_quantize_int8(EcadEngine* e, const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int M, int K, void* stream);
+
+/* o[M,N] = act(a_scale[m] w_scale[n] (A[M,K] @ W[N,K]^T) + bias[n]), the sum in 32-bit integers; epi as ecad_op_gemm: 0 none, 1 GELU(tanh), 2 SiLU, 3 cache write and
+ * gated residual: out = o rounded (may be NULL), resid_out = resid + (gate_table[n] + gate_mod[m / rows_per_batch][n]) * out (either or both NULL: gate 1 where
+ * neither is given; resid_out may be resid).  kernel: ECAD_I8_K_AUTO, or one by name (the same bits; ECAD_E_UNSUPPORTED if it cannot take the shape). */
+enum { ECAD_I8_K_AUTO = 0, ECAD_I8_K_ROWS = 1 /* up to 64 rows: operands straight to registers, K over the waves */, ECAD_I8_K_TILE64 = 2, ECAD_I8_K_TILE128 = 3, ECAD_I8_K_TILE144 = 4 /* 256 x 144 */,
+       ECAD_I8_K_TILE256 = 5, ECAD_I8_K_TILE288 = 6 /* 256 x 288 */ };
+int ecad_op_gemm_int8(EcadEngine* e, int kernel, int epi, const int8_t* A, int64_t lda, const float* a_scale, const int8_t* W, int64_t ldw, const float* w_scale, const float* bias, void* out,
+                      int64_t ldo, const void* resid, int64_t ldr, void* resid_out, int64_t ldro, const float* gate_table, const void* gate_mod, int64_t gate_mod_stride, int rows_per_batch, int M,
+                      int N, int K, void* stream);
+
+/* h' = resid_scale * h + g * post(y);  n = pre(h') * (1 + s) + t.   post / pre: ECAD_NORM_*, x / sqrt(mean x^2 + eps) or (x - mean) / sqrt(var + eps), times weight[D]
+ * where not NULL.  g = gate_table[D] + gate_mod[row / rows_per_batch][D] (1 where both are NULL), s and t in the same way from table_scale / mod_scale and
+ * table_shift / mod_shift (0 where both are NULL); tables fp32, modulations engine dtype with a stride between samples.
+ * y NULL: h' = h and h_out is not written (no gate, post-norm or residual scale then).  pre ECAD_NORM_NONE: only h_out.  n goes to n_out, or, rounded to the engine
+ * dtype first, to 8-bit rows q / q_scale (ecad_op_quantize_int8 of n, bit for bit): exactly one of the two.  h_out may be h, n_out may be y.  1 <= D <= 32768. */
+enum { ECAD_NORM_NONE = 0, ECAD_NORM_RMS = 1, ECAD_NORM_LAYER = 2 };
+typedef struct EcadGateNorm {
+  const void* h; int64_t ldh;
+  const void* y; int64_t ldy;
+  void* h_out; int64_t ldho;
+  void* n_out; int64_t ldn;
+  int8_t* q; int64_t ldq;
+  float* q_scale;
+  const float* post_weight;
+  const float* pre_weight;
+  const float* gate_table;
+  const void* gate_mod; int64_t gate_mod_stride;
+  const float* table_shift;
+  const float* table_scale;
+  const void* mod_shift;
+  const void* mod_scale; int64_t mod_stride;
+  int32_t M, D, rows_per_batch, post, pre;
+  float resid_scale, eps;
+} EcadGateNorm;
+int ecad_op_gate_norm(EcadEngine* e, const EcadGateNorm* args, void* stream);
+
+/* table[S][pairs][2] = m (cos, sin)(p[s][axis(j)] f_j), angles in 64 bits.  positions [S][axes] int32 (positions_float 0) or fp32 (1); the pairs of the axes follow each
+ * other, axes_dims[a] / 2 (host array) on axis a, f = theta^(-2 j / axes_dims[a]).  Scalings for positions beyond the trained ones, by `factor`:
+ *   LINEAR  f / factor
+ *   NTK     theta * factor^(d / (d - 2)) in place of theta (axes of two elements: theta)
+ *   YARN    f w + (f / factor)(1 - w), w = clamp((original_length f / 2 pi - beta_slow) / (beta_fast - beta_slow), 0, 1), and m = 0.1 ln(factor) + 1 (else m = 1) */
+enum { ECAD_ROPE_NONE = 0, ECAD_ROPE_LINEAR = 1, ECAD_ROPE_NTK = 2, ECAD_ROPE_YARN = 3 };
+int ecad_op_rope_table(EcadEngine* e, const void* positions, int positions_float, const int32_t* axes_dims, int axes, int S, int scaling, double theta, double factor, double original_length,
+                       double beta_fast, double beta_slow, float* table, void* stream);
+
+/* Turns the first `rot` elements of every head by table[row][rot / 2][2], the others stay: pair j = elements (2j, 2j + 1), or (j, j + rot / 2) with `half`; `inverse`
+ * turns back (which is also the gradient's rotation).  Queries q [B, S, Hq, D] and keys k [B, S, Hk, D] (Hk 0: queries only) at any strides {sample, token, head};
+ * the elements of a head are contiguous.  q_out == q (and k_out == k, same strides): in place.  row = index[b * index_stride + s] (index_stride 0: one list for all samples), or s
+ * where index is NULL; a token whose index lies outside the table is not turned. */
+int ecad_op_rope(EcadEngine* e, const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int Hq, const void* k, const int64_t* k_strides, void* k_out,
+                 const int64_t* k_out_strides, int Hk, const float* table, int table_rows, const int32_t* index, int64_t index_stride, int B, int S, int D, int rot, int half, int inverse, void* stream);
 
 /* ---- decode tail: AutoencoderKL decoder + postprocess ------------------------------------------------
  * Replaces `self.vae.decode(latents / scaling_factor)` and `image_processor.postprocess(..., "pil")` inside the reference's
