@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 LIB_NAME = "libecad_hip.so"
@@ -113,26 +114,12 @@ class EcadFluxStats(C.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
-class EcadGateNorm(C.Structure):
-    _fields_ = [
-        ("h", C.c_void_p), ("ldh", C.c_int64),
-        ("y", C.c_void_p), ("ldy", C.c_int64),
-        ("h_out", C.c_void_p), ("ldho", C.c_int64),
-        ("n_out", C.c_void_p), ("ldn", C.c_int64),
-        ("q", C.c_void_p), ("ldq", C.c_int64),
-        ("q_scale", C.c_void_p),
-        ("post_weight", C.c_void_p),
-        ("pre_weight", C.c_void_p),
-        ("gate_table", C.c_void_p),
-        ("gate_mod", C.c_void_p), ("gate_mod_stride", C.c_int64),
-        ("table_shift", C.c_void_p),
-        ("table_scale", C.c_void_p),
-        ("mod_shift", C.c_void_p),
-        ("mod_scale", C.c_void_p), ("mod_stride", C.c_int64),
-        ("M", C.c_int32), ("D", C.c_int32), ("rows_per_batch", C.c_int32), ("post", C.c_int32), ("pre", C.c_int32),
-        ("resid_scale", C.c_float), ("eps", C.c_float),
-    ]
-
+# Arguments of the operators of an 8-bit transformer block (EcadInt8Gemm, EcadGateNorm, EcadRope), packed by struct: members in the header's order, which has no
+# padding (tests/test_cpu_operators.py holds the layouts to the C compiler's).  P pointer, q int64, i int32, f float.
+_HEADS = "PP" + "qqq" + "qqq" + "q"
+INT8_GEMM = struct.Struct("PqPPqPPPqPqPqPPq" + "iiiiii")
+GATE_NORM = struct.Struct("PqPqPqPqPqPPPPPqPPPPq" + "iiiiii" + "ff")
+ROPE = struct.Struct(_HEADS + _HEADS + "PPq" + "iiiiiiii")
 
 _P = C.c_void_p
 _I = C.c_int
@@ -176,10 +163,10 @@ SIGNATURES = {
     "ecad_op_cache_accumulate": (_I, [_P, _P, _I, _I, _I, C.POINTER(_P), C.POINTER(_P), C.POINTER(_P), _I64, _I, _P]),
     "ecad_op_attention": (_I, [_P, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _I, _I, _I, _I, _I, _P, _P]),
     "ecad_op_quantize_int8": (_I, [_P, _P, _I64, _P, _I64, _P, _I, _I, _P]),
-    "ecad_op_gemm_int8": (_I, [_P, _I, _I, _P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I, _I, _I, _I, _P]),
-    "ecad_op_gate_norm": (_I, [_P, C.POINTER(EcadGateNorm), _P]),
+    "ecad_op_gemm_int8": (_I, [_P, _P, _P]),
+    "ecad_op_gate_norm": (_I, [_P, _P, _P]),
     "ecad_op_rope_table": (_I, [_P, _P, _I, C.POINTER(C.c_int32), _I, _I, _I, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, _P, _P]),
-    "ecad_op_rope": (_I, [_P, _P, C.POINTER(_I64), _P, C.POINTER(_I64), _I, _P, C.POINTER(_I64), _P, C.POINTER(_I64), _I, _P, _I, _P, _I64, _I, _I, _I, _I, _I, _I, _P]),
+    "ecad_op_rope": (_I, [_P, _P, _P]),
     "ecad_vae_create": (_I, [_I, _I, C.POINTER(_P)]),
     "ecad_vae_destroy": (None, [_P]),
     "ecad_vae_last_error": (C.c_char_p, [_P]),

@@ -2343,19 +2343,15 @@ int ecad_op_quantize_int8(EcadEngine* e, const void* x, int64_t ldx, int8_t* q, 
   ENG(e);
   return run_operator(E, stream, [&](const OpCtx& c, OpStatus& st) { return op_quantize_int8(c, QuantizeCall{x, ldx, q, ldq, scale, M, K}, st); });
 }
-int ecad_op_gemm_int8(EcadEngine* e, int kernel, int epi, const int8_t* A, int64_t lda, const float* a_scale, const int8_t* W, int64_t ldw, const float* w_scale, const float* bias, void* out,
-                      int64_t ldo, const void* resid, int64_t ldr, void* resid_out, int64_t ldro, const float* gate_table, const void* gate_mod, int64_t gate_mod_stride, int rows_per_batch, int M,
-                      int N, int K, void* stream) {
+int ecad_op_gemm_int8(EcadEngine* e, const EcadInt8Gemm* a, void* stream) {
   ENG(e);
-  const Int8GemmCall g{A, lda, a_scale, W, ldw, w_scale, bias, out, ldo, resid, ldr, resid_out, ldro, gate_table, gate_mod, gate_mod_stride, M, N, K, epi, rows_per_batch, kernel};
-  return run_operator(E, stream, [&](const OpCtx& c, OpStatus& st) { return op_gemm_int8(c, g, st); });
+  if (!a) return E->fail(ECAD_E_INVALID, "NULL argument");
+  return run_operator(E, stream, [&](const OpCtx& c, OpStatus& st) { return op_gemm_int8(c, *a, st); });
 }
 int ecad_op_gate_norm(EcadEngine* e, const EcadGateNorm* a, void* stream) {
   ENG(e);
   if (!a) return E->fail(ECAD_E_INVALID, "NULL argument");
-  const GateNormCall g{a->h, a->ldh, a->y, a->ldy, a->h_out, a->ldho, a->n_out, a->ldn, a->q, a->ldq, a->q_scale, a->post_weight, a->pre_weight, a->gate_table, a->gate_mod, a->gate_mod_stride,
-                       a->table_shift, a->table_scale, a->mod_shift, a->mod_scale, a->mod_stride, a->M, a->D, a->rows_per_batch, a->post, a->pre, a->resid_scale, a->eps};
-  return run_operator(E, stream, [&](const OpCtx& c, OpStatus& st) { return op_gate_norm(c, g, st); });
+  return run_operator(E, stream, [&](const OpCtx& c, OpStatus& st) { return op_gate_norm(c, *a, st); });
 }
 int ecad_op_rope_table(EcadEngine* e, const void* positions, int positions_float, const int32_t* axes_dims, int axes, int S, int scaling, double theta, double factor, double original_length,
                        double beta_fast, double beta_slow, float* table, void* stream) {
@@ -2363,16 +2359,10 @@ int ecad_op_rope_table(EcadEngine* e, const void* positions, int positions_float
   const RopeTableCall g{positions, positions_float, axes_dims, axes, S, scaling, table, theta, factor, original_length, beta_fast, beta_slow};
   return run_operator(E, stream, [&](const OpCtx& c, OpStatus& st) { return op_rope_table(c, g, st); });
 }
-int ecad_op_rope(EcadEngine* e, const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int Hq, const void* k, const int64_t* k_strides, void* k_out,
-                 const int64_t* k_out_strides, int Hk, const float* table, int table_rows, const int32_t* index, int64_t index_stride, int B, int S, int D, int rot, int half, int inverse, void* stream) {
+int ecad_op_rope(EcadEngine* e, const EcadRope* a, void* stream) {
   ENG(e);
-  if (!q_strides || !q_out_strides || (Hk > 0 && (!k_strides || !k_out_strides))) return E->fail(ECAD_E_INVALID, "NULL strides");
-  RopeCall g{};
-  g.q = RopeHeads{q, q_out, q_strides[0], q_strides[1], q_strides[2], q_out_strides[0], q_out_strides[1], q_out_strides[2], Hq};
-  if (Hk > 0) g.k = RopeHeads{k, k_out, k_strides[0], k_strides[1], k_strides[2], k_out_strides[0], k_out_strides[1], k_out_strides[2], Hk};
-  else g.k.H = Hk;
-  g.table = table; g.index = index; g.index_stride = index_stride; g.B = B; g.S = S; g.D = D; g.rot = rot; g.table_rows = table_rows; g.half = half; g.inverse = inverse;
-  return run_operator(E, stream, [&](const OpCtx& c, OpStatus& st) { return op_rope(c, g, st); });
+  if (!a) return E->fail(ECAD_E_INVALID, "NULL argument");
+  return run_operator(E, stream, [&](const OpCtx& c, OpStatus& st) { return op_rope(c, *a, st); });
 }
 
 }  // extern "C"

@@ -8,7 +8,6 @@
 
 #include <atomic>
 
-#include "../../include/ecad_hip.h"
 #include "gate_norm.h"
 #include "gemm_int8.h"
 #include "rope.h"
@@ -40,6 +39,70 @@ int allow_lds(std::atomic<uint64_t>& done, const void* kernel, int bytes, OpStat
   if (e != hipSuccess) return refuse(st, ECAD_E_HIP, "LDS of %d bytes refused: %s", bytes, hipGetErrorString(e));
   if (dev < 64) done.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
   return ECAD_OK;
+}
+
+// ---- memory that an argument covers: sizes and strides (bytes), outermost first, the elements of the last dimension dense ----------------------------------------
+
+struct Region {
+  const char* p;
+  int64_t n[4], step[4];
+  int64_t bytes;  // of the dense innermost part
+  bool empty() const {
+    if (!p || bytes <= 0) return true;
+    for (int64_t x : n)
+      if (x == 0) return true;
+    return false;
+  }
+  int64_t reach() const {
+    int64_t r = bytes;
+    for (int i = 0; i < 4; ++i) r += (n[i] - 1) * step[i];
+    return r;
+  }
+};
+Region matrix(const void* p, int64_t rows, int64_t width, int64_t stride, int64_t size) { return {(const char*)p, {1, 1, 1, rows}, {0, 0, 0, stride * size}, width * size}; }
+Region vector(const void* p, int64_t n, int64_t size) { return matrix(p, 1, n, 0, size); }
+
+// every element of an output has memory of its own
+bool distinct(const Region& r) {
+  int64_t n[4], step[4];
+  int d = 0;
+  for (int i = 0; i < 4; ++i)
+    if (r.n[i] > 1) {  // insertion by stride
+      int j = d++;
+      for (; j > 0 && step[j - 1] > r.step[i]; --j) n[j] = n[j - 1], step[j] = step[j - 1];
+      n[j] = r.n[i], step[j] = r.step[i];
+    }
+  int64_t need = r.bytes;
+  for (int i = 0; i < d; ++i) {
+    if (step[i] < need) return false;
+    need += step[i] * (n[i] - 1);
+  }
+  return true;
+}
+
+// Whether two regions may share memory.  Where all the strides of both that are not inside a row are multiples of that row's length (columns of one buffer), the
+// bytes that each takes of the row decide.
+bool meet(const Region& a, const Region& b) {
+  if (a.empty() || b.empty() || a.p + a.reach() <= b.p || b.p + b.reach() <= a.p) return false;
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = a.step[i];
+    if (a.n[i] < 2 || row <= 0) continue;
+    auto inner = [&](const Region& r) {
+      int64_t x = r.bytes;
+      for (int j = 0; j < 4; ++j)
+        if (r.n[j] > 1 && r.step[j] % row) x += (r.n[j] - 1) * r.step[j];
+      return x;
+    };
+    const int64_t gap = ((b.p - a.p) % row + row) % row;
+    if (gap >= inner(a) && gap + inner(b) <= row) return false;
+  }
+  return true;
+}
+
+template <size_t N> bool meets_any(const Region& out, const Region (&others)[N]) {
+  for (const Region& r : others)
+    if (meet(out, r)) return true;
+  return false;
 }
 
 constexpr int MAX_ROW = 32768;       // widest row that the norms hold in registers (1024 lanes x 4 pieces)
@@ -148,30 +211,40 @@ int op_quantize_int8(const OpCtx& ctx, const QuantizeCall& c, OpStatus& st) noex
   if (c.ldx < (c.M > 1 ? c.K : 0) || c.ldq < c.K || c.ldq % 16 || !aligned(c.q, 16) || !aligned(c.x, 2) || !aligned(c.scale, 4))
     return refuse(st, ECAD_E_INVALID, "quantize_int8: x rows need a stride of at least %d, 8-bit rows start on 16 bytes with a stride of a multiple of 16 (got %lld and %lld)", c.K, (long long)c.ldx,
                   (long long)c.ldq);
+  const Region x = matrix(c.x, c.M, c.K, c.ldx, 2), q = matrix(c.q, c.M, c.K, c.ldq, 1), scale = vector(c.scale, c.M, 4);
+  if (meet(q, x) || meet(q, scale) || meet(scale, x)) return refuse(st, ECAD_E_INVALID, "quantize_int8: an output overlaps another argument");
   const QuantizeArgs a{c.x, c.q, c.scale, c.ldx, c.ldq, c.M, c.K};
   return ctx.dtype == ECAD_DTYPE_F16 ? quantize_t<f16_t>(ctx, a, st) : quantize_t<bf16_t>(ctx, a, st);
 }
 
-int op_gemm_int8(const OpCtx& ctx, const Int8GemmCall& c, OpStatus& st) noexcept {
+int op_gemm_int8(const OpCtx& ctx, const EcadInt8Gemm& c, OpStatus& st) noexcept {
   if (c.M < 0 || c.N < 0 || c.K < 1 || c.K > MAX_INT8_K) return refuse(st, ECAD_E_INVALID, "gemm_int8: M=%d N=%d K=%d (K from 1 to %d)", c.M, c.N, c.K, MAX_INT8_K);
   if (c.epi < 0 || c.epi > 3) return refuse(st, ECAD_E_INVALID, "gemm_int8: epilogue %d unknown", c.epi);
   if (c.M == 0 || c.N == 0) return ECAD_OK;
-  if (!c.A || !c.W || !c.sa || !c.sw || (c.epi != I8_RESID && !c.out)) return refuse(st, ECAD_E_INVALID, "gemm_int8: NULL pointer");
+  if (!c.A || !c.W || !c.a_scale || !c.w_scale || (c.epi != I8_RESID && !c.out)) return refuse(st, ECAD_E_INVALID, "gemm_int8: NULL pointer");
   if (c.epi == I8_RESID && (!c.resid || !c.resid_out)) return refuse(st, ECAD_E_INVALID, "gemm_int8: epilogue 3 needs resid");
   if (!aligned(c.A, 16) || !aligned(c.W, 16) || c.lda % 16 || c.ldw % 16 || c.lda < c.K || c.ldw < c.K || c.lda > (1 << 23) || c.ldw > (1 << 23))
     return refuse(st, ECAD_E_INVALID, "gemm_int8: 8-bit rows start on 16 bytes with a stride of a multiple of 16, at least %d (got %lld and %lld)", c.K, (long long)c.lda, (long long)c.ldw);
-  if (!aligned(c.sa, 4) || !aligned(c.sw, 4) || !aligned(c.bias, 4) || !aligned(c.gate_table, 4) || !aligned(c.out, 2) || !aligned(c.resid, 2) || !aligned(c.resid_out, 2) || !aligned(c.gate_mod, 2))
+  if (!aligned(c.a_scale, 4) || !aligned(c.w_scale, 4) || !aligned(c.bias, 4) || !aligned(c.gate_table, 4) || !aligned(c.out, 2) || !aligned(c.resid, 2) || !aligned(c.resid_out, 2) || !aligned(c.gate_mod, 2))
     return refuse(st, ECAD_E_INVALID, "gemm_int8: pointers are not aligned to their type");
   if ((c.out && c.M > 1 && c.ldo < c.N) || (c.epi == I8_RESID && c.M > 1 && (c.ldr < c.N || c.ldro < c.N))) return refuse(st, ECAD_E_INVALID, "gemm_int8: row strides of the outputs are shorter than %d", c.N);
   if (c.epi == I8_RESID && c.rows_per_batch < 1) return refuse(st, ECAD_E_INVALID, "gemm_int8: rows_per_batch must be at least 1");
+  const bool gated = c.epi == I8_RESID;
+  const int64_t samples = gated ? ((int64_t)c.M - 1) / c.rows_per_batch + 1 : 0;
+  const Region out = matrix(c.out, c.M, c.N, c.ldo, 2), resid_out = matrix(gated ? c.resid_out : nullptr, c.M, c.N, c.ldro, 2), resid = matrix(gated ? c.resid : nullptr, c.M, c.N, c.ldr, 2);
+  const Region in[] = {matrix(c.A, c.M, c.K, c.lda, 1), matrix(c.W, c.N, c.K, c.ldw, 1), vector(c.a_scale, c.M, 4), vector(c.w_scale, c.N, 4), vector(c.bias, c.N, 4),
+                       vector(gated ? c.gate_table : nullptr, c.N, 4), matrix(gated ? c.gate_mod : nullptr, samples, c.N, c.gate_mod_stride, 2)};
+  const bool in_place = gated && c.resid_out == c.resid && (c.ldr == c.ldro || c.M == 1);
+  if (meets_any(out, in) || meets_any(resid_out, in) || meet(out, resid) || meet(out, resid_out) || (!in_place && meet(resid_out, resid)))
+    return refuse(st, ECAD_E_INVALID, "gemm_int8: an output overlaps another argument");
   Int8GemmArgs a{};
-  a.A = c.A; a.W = c.W; a.sa = c.sa; a.sw = c.sw; a.bias = c.bias; a.out = c.out; a.resid = c.resid; a.resid_out = c.resid_out; a.gate_table = c.gate_table; a.gate_mod = c.gate_mod;
-  a.lda = c.lda; a.ldw = c.ldw; a.ldo = c.ldo; a.ldr = c.ldr; a.ldro = c.ldro; a.gate_stride = c.gate_stride;
+  a.A = c.A; a.W = c.W; a.sa = c.a_scale; a.sw = c.w_scale; a.bias = c.bias; a.out = c.out; a.resid = c.resid; a.resid_out = c.resid_out; a.gate_table = c.gate_table; a.gate_mod = c.gate_mod;
+  a.lda = c.lda; a.ldw = c.ldw; a.ldo = c.ldo; a.ldr = c.ldr; a.ldro = c.ldro; a.gate_stride = c.gate_mod_stride;
   a.M = c.M; a.N = c.N; a.K = c.K; a.epi = c.epi; a.rows_per_batch = c.rows_per_batch > 0 ? c.rows_per_batch : 1;
   return ctx.dtype == ECAD_DTYPE_F16 ? gemm_int8_t<f16_t>(ctx, a, c.kernel, st) : gemm_int8_t<bf16_t>(ctx, a, c.kernel, st);
 }
 
-int op_gate_norm(const OpCtx& ctx, const GateNormCall& c, OpStatus& st) noexcept {
+int op_gate_norm(const OpCtx& ctx, const EcadGateNorm& c, OpStatus& st) noexcept {
   if (c.M < 0 || c.D < 1) return refuse(st, ECAD_E_INVALID, "gate_norm: %d rows of %d values", c.M, c.D);
   if (c.D > MAX_ROW) return refuse(st, ECAD_E_UNSUPPORTED, "gate_norm: rows of up to %d values, got %d", MAX_ROW, c.D);
   if (c.post < NORM_NONE || c.post > NORM_LAYER || c.pre < NORM_NONE || c.pre > NORM_LAYER) return refuse(st, ECAD_E_INVALID, "gate_norm: norm kinds are 0 (none), 1 (rms), 2 (layer)");
@@ -190,10 +263,21 @@ int op_gate_norm(const OpCtx& ctx, const GateNormCall& c, OpStatus& st) noexcept
   if (!aligned(c.h, 2) || !aligned(c.y, 2) || !aligned(c.h_out, 2) || !aligned(c.n_out, 2) || !aligned(c.gate_mod, 2) || !aligned(c.mod_shift, 2) || !aligned(c.mod_scale, 2) || !aligned(c.post_weight, 4) ||
       !aligned(c.pre_weight, 4) || !aligned(c.gate_table, 4) || !aligned(c.table_shift, 4) || !aligned(c.table_scale, 4))
     return refuse(st, ECAD_E_INVALID, "gate_norm: pointers are not aligned to their type");
+  const int64_t samples = ((int64_t)c.M - 1) / c.rows_per_batch + 1;
+  const Region h = matrix(c.h, c.M, c.D, c.ldh, 2), y = matrix(c.y, c.M, c.D, c.ldy, 2), ho = matrix(c.y ? c.h_out : nullptr, c.M, c.D, c.ldho, 2), no = matrix(c.n_out, c.M, c.D, c.ldn, 2),
+               q = matrix(c.q, c.M, c.D, c.ldq, 1), qs = vector(c.q ? c.q_scale : nullptr, c.M, 4);
+  const Region in[] = {vector(c.post_weight, c.D, 4), vector(c.pre_weight, c.D, 4), vector(c.gate_table, c.D, 4), vector(c.table_shift, c.D, 4), vector(c.table_scale, c.D, 4),
+                       matrix(c.gate_mod, samples, c.D, c.gate_mod_stride, 2), matrix(c.mod_shift, samples, c.D, c.mod_stride, 2), matrix(c.mod_scale, samples, c.D, c.mod_stride, 2)};
+  const bool h_same = c.h_out == c.h && (c.ldho == c.ldh || c.M == 1), y_same = c.y && c.n_out == c.y && (c.ldn == c.ldy || c.M == 1);
+  const Region outs[] = {ho, no, q, qs};
+  bool clash = (!h_same && meet(ho, h)) || meet(ho, y) || meet(no, h) || (!y_same && meet(no, y)) || meet(q, h) || meet(q, y) || meet(qs, h) || meet(qs, y) || meet(ho, no) || meet(ho, q) || meet(ho, qs) ||
+               meet(q, qs);
+  for (const Region& o : outs) clash = clash || meets_any(o, in);
+  if (clash) return refuse(st, ECAD_E_INVALID, "gate_norm: an output overlaps another argument");
   GateNormArgs a{};
   a.h = c.h; a.y = c.y; a.h_out = c.h_out; a.n_out = c.n_out; a.q = c.q; a.q_scale = c.q_scale; a.post_weight = c.post_weight; a.pre_weight = c.pre_weight;
   a.gate_table = c.gate_table; a.table_shift = c.table_shift; a.table_scale = c.table_scale; a.gate_mod = c.gate_mod; a.mod_shift = c.mod_shift; a.mod_scale = c.mod_scale;
-  a.ldh = c.ldh; a.ldy = c.ldy; a.ldho = c.ldho; a.ldn = c.ldn; a.ldq = c.ldq; a.gate_stride = c.gate_stride; a.mod_stride = c.mod_stride;
+  a.ldh = c.ldh; a.ldy = c.ldy; a.ldho = c.ldho; a.ldn = c.ldn; a.ldq = c.ldq; a.gate_stride = c.gate_mod_stride; a.mod_stride = c.mod_stride;
   a.M = c.M; a.D = c.D; a.rows_per_batch = c.rows_per_batch; a.post = c.post; a.pre = c.pre; a.resid_scale = c.resid_scale; a.eps = c.eps;
   return ctx.dtype == ECAD_DTYPE_F16 ? gate_norm_t<f16_t>(ctx, a, st) : gate_norm_t<bf16_t>(ctx, a, st);
 }
@@ -224,6 +308,7 @@ int op_rope_table(const OpCtx& ctx, const RopeTableCall& c, OpStatus& st) noexce
   }
   if (c.S == 0) return ECAD_OK;
   if (!c.positions || !c.table || !aligned(c.positions, 4) || !aligned(c.table, 8)) return refuse(st, ECAD_E_INVALID, "rope_table: NULL or unaligned pointer");
+  if (meet(vector(c.table, (int64_t)c.S * a.pairs * 2, 4), vector(c.positions, (int64_t)c.S * c.axes, 4))) return refuse(st, ECAD_E_INVALID, "rope_table: the table overlaps the positions");
   a.positions = c.positions; a.table = c.table; a.positions_float = c.positions_float; a.axes = c.axes; a.S = c.S;
   a.size = c.scaling == ECAD_ROPE_YARN ? (float)(0.1 * log(c.factor) + 1.0) : 1.0f;
   const int64_t blocks = ((int64_t)c.S * a.pairs + 255) / 256, most = (int64_t)ctx.num_cus * 32;
@@ -231,24 +316,31 @@ int op_rope_table(const OpCtx& ctx, const RopeTableCall& c, OpStatus& st) noexce
   return launched(st, "rope_table");
 }
 
-int op_rope(const OpCtx& ctx, const RopeCall& c, OpStatus& st) noexcept {
-  if (c.B < 0 || c.S < 0 || c.q.H < 1 || c.k.H < 0 || c.D < 2 || c.rot < 2 || c.rot % 2 || c.rot > c.D || c.table_rows < 0)
-    return refuse(st, ECAD_E_INVALID, "rope: %d samples of %d tokens, %d + %d heads of %d elements, %d of them turned (even, 2 to the head's size)", c.B, c.S, c.q.H, c.k.H, c.D, c.rot);
+int op_rope(const OpCtx& ctx, const EcadRope& c, OpStatus& st) noexcept {
+  if (c.B < 0 || c.S < 0 || c.q.H < 1 || c.k.H < 0 || c.q.H > (1 << 20) || c.k.H > (1 << 20) || c.D < 2 || c.rot < 2 || c.rot % 2 || c.rot > c.D || c.table_rows < 0)
+    return refuse(st, ECAD_E_INVALID, "rope: %d samples of %d tokens, %lld + %lld heads of %d elements, %d of them turned (even, 2 to the head's size)", c.B, c.S,
+                  (long long)c.q.H, (long long)c.k.H, c.D, c.rot);
   if (c.B == 0 || c.S == 0) return ECAD_OK;
   if (!c.q.x || !c.q.out || (c.k.H && (!c.k.x || !c.k.out)) || !c.table) return refuse(st, ECAD_E_INVALID, "rope: NULL pointer");
   if (!aligned(c.q.x, 2) || !aligned(c.q.out, 2) || !aligned(c.k.x, 2) || !aligned(c.k.out, 2) || !aligned(c.table, 4) || !aligned(c.index, 4)) return refuse(st, ECAD_E_INVALID, "rope: pointers are not aligned to their type");
   if (!c.index && c.table_rows < c.S) return refuse(st, ECAD_E_INVALID, "rope: the table has %d rows for %d tokens", c.table_rows, c.S);
   const bool q_in = c.q.x == c.q.out, k_in = c.k.H == 0 || c.k.x == c.k.out;
   if (c.k.H && q_in != k_in) return refuse(st, ECAD_E_INVALID, "rope: queries and keys are both turned in place or both not");
-  auto same = [](const RopeHeads& x) { return x.sb == x.ob && x.ss == x.os && x.sh == x.oh; };
+  auto same = [](const EcadRopeHeads& x) { return x.sample == x.out_sample && x.token == x.out_token && x.head == x.out_head; };
   if (q_in && (!same(c.q) || (c.k.H && !same(c.k)))) return refuse(st, ECAD_E_INVALID, "rope: in place needs the same strides on both sides");
+  auto in_of = [&](const EcadRopeHeads& x) { return Region{x.H ? (const char*)x.x : nullptr, {1, c.B, c.S, x.H}, {0, 2 * x.sample, 2 * x.token, 2 * x.head}, (int64_t)2 * c.D}; };
+  auto out_of = [&](const EcadRopeHeads& x) { return Region{x.H ? (const char*)x.out : nullptr, {1, c.B, c.S, x.H}, {0, 2 * x.out_sample, 2 * x.out_token, 2 * x.out_head}, (int64_t)2 * c.D}; };
+  const Region q = in_of(c.q), k = in_of(c.k), qo = out_of(c.q), ko = out_of(c.k);
+  const Region in[] = {vector(c.table, (int64_t)c.table_rows * c.rot, 4), matrix(c.index, c.index_stride ? c.B : 1, c.S, c.index_stride, 4)};
+  if (!distinct(qo) || (c.k.H && !distinct(ko))) return refuse(st, ECAD_E_INVALID, "rope: an output overlaps itself");
+  if (meet(qo, ko) || meets_any(qo, in) || meets_any(ko, in) || meet(qo, k) || meet(ko, q) || (!q_in && (meet(qo, q) || meet(ko, k)))) return refuse(st, ECAD_E_INVALID, "rope: an output overlaps another argument");
   RopeArgs a{};
   a.q = c.q; a.k = c.k; a.table = c.table; a.index = c.index; a.index_stride = c.index_stride; a.S = c.S; a.D = c.D; a.rot = c.rot; a.table_rows = c.table_rows; a.copy = !q_in;
   a.sign = c.inverse ? -1.f : 1.f;
   a.tokens = (int64_t)c.B * c.S;
   a.turning = c.half ? (c.rot / 2 + 7) / 8 : (c.rot + 7) / 8;
   a.units = c.half ? a.turning + (a.copy ? (c.D - c.rot + 7) / 8 : 0) : (a.copy ? (c.D + 7) / 8 : a.turning);
-  a.groups = (c.q.H + c.k.H + ROPE_HEADS - 1) / ROPE_HEADS;
+  a.groups = (int)((c.q.H + c.k.H + ROPE_HEADS - 1) / ROPE_HEADS);
   const int64_t per_token = (int64_t)a.units * a.groups;
   if (per_token > (1 << 24)) return refuse(st, ECAD_E_UNSUPPORTED, "rope: %lld pieces a token", (long long)per_token);
   a.tokens_per_block = per_token >= 256 ? 1 : (int)(256 / per_token);

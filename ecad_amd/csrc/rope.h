@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256) void rope_table_kernel(const RopeTableArgs p) 
 }
 
 struct RopeArgs {
-  RopeHeads q, k;
+  EcadRopeHeads q, k;
   const float* table;
   const int32_t* index;
   int64_t index_stride;
@@ -90,17 +90,17 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs p) {
       for (int e = 0; e < (HALF ? 8 : 4); ++e)
         if (e < left) c[e] = f[2 * e], sn[e] = p.sign * f[2 * e + 1];
     }
-    const int heads = p.q.H + p.k.H, head0 = (int)grp * ROPE_HEADS;
+    const int heads = (int)(p.q.H + p.k.H), head0 = (int)grp * ROPE_HEADS;
     Pack8 lo[ROPE_HEADS], hi[ROPE_HEADS];
     T* dst[ROPE_HEADS];
 #pragma unroll
     for (int i = 0; i < ROPE_HEADS; ++i) {
       const int h = head0 + i < heads ? head0 + i : heads - 1;
       const bool key = h >= p.q.H;
-      const RopeHeads& x = key ? p.k : p.q;
-      const int hh = key ? h - p.q.H : h;
-      const T* src = reinterpret_cast<const T*>(x.x) + b * x.sb + s * x.ss + hh * x.sh + at;
-      dst[i] = reinterpret_cast<T*>(x.out) + b * x.ob + s * x.os + hh * x.oh + at;
+      const EcadRopeHeads& x = key ? p.k : p.q;
+      const int hh = key ? h - (int)p.q.H : h;
+      const T* src = reinterpret_cast<const T*>(x.x) + b * x.sample + s * x.token + hh * x.head + at;
+      dst[i] = reinterpret_cast<T*>(x.out) + b * x.out_sample + s * x.out_token + hh * x.out_head + at;
       lo[i] = load_piece<T>(src, n);
       if constexpr (HALF)
         if (turns) hi[i] = load_piece<T>(src + half, n);

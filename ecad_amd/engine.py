@@ -29,36 +29,6 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    """Elements between the rows of a matrix (a single row: its width, whatever the tensor says)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
-
-
-def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
-    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
-
-
-def _span(t: torch.Tensor) -> tuple[int, int]:
-    """First byte of a tensor and the first behind its last element."""
-    at, size = t.data_ptr(), t.element_size()
-    return at, at + (size if t.numel() else 0) + sum((n - 1) * st for n, st in zip(t.shape, t.stride()) if n > 1) * size
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two tensors can share memory.  Columns of one buffer side by side do not: where the outer strides of both are multiples of a row's length, the bytes that
-    the rest takes of a row decide."""
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    if a1 <= b0 or b1 <= a0 or not a.numel() or not b.numel():
-        return False
-    dims = lambda t: [((n - 1) * st * t.element_size(), st * t.element_size()) for n, st in zip(t.shape, t.stride()) if n > 1]  # noqa: E731
-    for _, row in dims(a):
-        inner = [t.element_size() + sum(reach for reach, step in dims(t) if step % row) for t in (a, b)] if row else [1, 1]
-        gap = (b0 - a0) % row if row else 0
-        if row and gap >= inner[0] and gap + inner[1] <= row:
-            return False
-    return True
-
-
 class EcadEngine:
     def __init__(
         self,
@@ -432,62 +402,58 @@ class EcadEngine:
 
     # -- the launches of an 8-bit transformer block ---------------------------------------------
     # Inference only, like every op here: tensors that require a gradient are refused while gradients are recorded.  Work goes to the current stream of the engine's
-    # device; nothing is allocated but the results.
-    def _check(self, name: str, t: torch.Tensor | None, dtype: torch.dtype, shape: tuple | None = None, rows: bool = False) -> None:
-        """``t`` (None passes) on this engine's device, of ``dtype`` and ``shape``; last dimension dense (``rows``: the others at any stride), else contiguous."""
-        if t is None:
-            return
+    # device; nothing is allocated but the results.  The library refuses outputs that overlap themselves or another argument.
+    def _refuse(self, name: str, t, dtype: torch.dtype, shape: tuple, dense: str) -> None:
+        """Says what is wrong with an argument that failed its check."""
         if not isinstance(t, torch.Tensor):
             raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
         if t.device != self.device:
             raise ValueError(f"{name} is on {t.device}, this engine on {self.device}")
-        if t.dtype != dtype:
+        if t.dtype is not dtype:
             raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-        if shape is not None and t.shape != shape:
+        if t.shape != shape:
             raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-        if not (t.shape[-1] <= 1 or t.stride(-1) == 1 if rows else t.is_contiguous()):
-            raise ValueError(f"{name} must {'have a dense last dimension' if rows else 'be contiguous'}, got strides {t.stride()}")
         if t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{name} requires a gradient: this op has none (detach it, or call under torch.no_grad())")
+        raise ValueError(f"{name} must {dense}, got strides {t.stride()}")
+
+    def _rows(self, name: str, t, dtype: torch.dtype, M: int, N: int) -> int:
+        """Row stride of an [M, N] matrix with dense rows."""
+        if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == (M, N) and t.device == self.device and not (t.requires_grad and torch.is_grad_enabled()):
+            row, one = t.stride()
+            if one == 1 or N <= 1:
+                return row if M > 1 else N
+        self._refuse(name, t, dtype, (M, N), "have a dense last dimension")
+
+    def _vector(self, name: str, t, n: int) -> int:
+        """Address of a contiguous fp32 [n]; 0 for None."""
+        if t is None:
+            return 0
+        if isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.shape == (n,) and t.device == self.device and t.is_contiguous() and not (t.requires_grad and torch.is_grad_enabled()):
+            return t.data_ptr()
+        self._refuse(name, t, torch.float32, (n,), "be contiguous")
+
+    def _mod(self, name: str, t, M: int, N: int, rows_per_batch: int) -> tuple[int, int]:
+        """(address, stride between samples) of modulations [samples, N] that cover M rows; (0, 0) for None, stride 0 for one sample."""
+        if t is None:
+            return 0, 0
+        if not isinstance(t, torch.Tensor) or t.dim() != 2:
+            raise ValueError(f"{name} must have shape (samples, {N})")
+        samples = t.shape[0]
+        stride = self._rows(name, t, self.dtype, samples, N)
+        if rows_per_batch < 1:
+            raise ValueError(f"rows_per_batch must be at least 1, got {rows_per_batch}")
+        if M > samples * rows_per_batch:
+            raise ValueError(f"{name} has {samples} samples of {rows_per_batch} rows, {M} rows are given")
+        return t.data_ptr(), stride if samples > 1 else 0
+
+    def _new_int8_rows(self, M: int, N: int) -> torch.Tensor:
+        """[M, N] int8 whose rows start on 16 bytes."""
+        rows = torch.empty((M, (N + 15) & ~15), device=self.device, dtype=torch.int8)
+        return rows if N % 16 == 0 else rows[:, :N]
 
     def _stream(self) -> int:
-        return int(torch.cuda.current_stream(self.device).cuda_stream)
-
-    def _check_mods(self, M: int, D: int, rows_per_batch: int, **mods: torch.Tensor | None) -> int:
-        """Modulations [samples, D] at one common stride between samples; ``rows_per_batch`` rows each cover all M rows.  Returns that stride."""
-        stride = None
-        if int(rows_per_batch) < 1:
-            raise ValueError(f"rows_per_batch must be at least 1, got {rows_per_batch}")
-        for name, t in mods.items():
-            if t is None:
-                continue
-            if not isinstance(t, torch.Tensor) or t.dim() != 2:
-                raise ValueError(f"{name} must have shape (samples, {D})")
-            self._check(name, t, self.dtype, (t.shape[0], D), rows=True)
-            if M > t.shape[0] * rows_per_batch:
-                raise ValueError(f"{name} has {t.shape[0]} samples of {rows_per_batch} rows, {M} rows are given")
-            step = t.stride(0) if t.shape[0] > 1 else None
-            if step is not None:
-                if stride not in (None, step):
-                    raise ValueError(f"{name}: shift and scale must have the same stride between samples, got {stride} and {step}")
-                stride = step
-        return stride or 0
-
-    @staticmethod
-    def _distinct(name: str, out: torch.Tensor) -> None:
-        """An output whose elements are all different memory."""
-        need = 1
-        for step, size in sorted((st, n) for st, n in zip(out.stride(), out.shape) if n > 1):
-            if step < need:
-                raise ValueError(f"{name} overlaps itself: strides {out.stride()} for shape {tuple(out.shape)}")
-            need = step * (size - 1) + need
-
-    @staticmethod
-    def _apart(name: str, out: torch.Tensor, /, **others: torch.Tensor | None) -> None:
-        """``out`` shares no memory with the other tensors (columns of one buffer side by side are apart)."""
-        for other, t in others.items():
-            if t is not None and _overlap(out, t):
-                raise ValueError(f"{name} overlaps {other}")
+        return torch.cuda.current_stream(self.device).cuda_stream
 
     def op_quantize_int8(self, x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Rows to 8-bit integers with one scale each (``ecad_op_quantize_int8``): x [M, K] of the engine's dtype at any row stride -> (q [M, K] int8 whose rows start on
@@ -496,19 +462,19 @@ class EcadEngine:
         ``out``: (q, scale) to write to; q's rows on 16 bytes."""
         if not isinstance(x, torch.Tensor) or x.dim() != 2:
             raise ValueError("x must have shape (rows, values)")
-        self._check("x", x, self.dtype, rows=True)
         M, K = x.shape
+        ldx = self._rows("x", x, self.dtype, M, K)
         if out is None:
-            q = torch.empty((M, (K + 15) // 16 * 16), device=self.device, dtype=torch.int8)[:, :K]
-            scale = torch.empty((M,), device=self.device, dtype=torch.float32)
+            q, scale = self._new_int8_rows(M, K), torch.empty((M,), device=self.device, dtype=torch.float32)
+            ldq = (K + 15) & ~15
         else:
             q, scale = out
-            self._check("q", q, torch.int8, (M, K), rows=True)
-            self._check("scale", scale, torch.float32, (M,))
-            self._distinct("q", q)
-            self._apart("q", q, x=x, scale=scale)
-            self._apart("scale", scale, x=x)
-        self._chk(self.lib.ecad_op_quantize_int8(self._h, x.data_ptr(), _row_stride(x), q.data_ptr(), _row_stride(q), scale.data_ptr(), M, K, self._stream()))
+            ldq = self._rows("q", q, torch.int8, M, K)
+            ldq = q.stride(0) if M == 1 else ldq
+            if scale is None:
+                raise ValueError("out must be (q, scale)")
+            self._vector("scale", scale, M)
+        self._chk(self.lib.ecad_op_quantize_int8(self._h, x.data_ptr(), ldx, q.data_ptr(), ldq, scale.data_ptr(), M, K, self._stream()))
         return q, scale
 
     INT8_KERNELS = {"auto": 0, "rows": 1, "tile64": 2, "tile128": 3, "tile144": 4, "tile256": 5, "tile288": 6}
@@ -517,44 +483,33 @@ class EcadEngine:
         """A Linear in 8-bit integers (``ecad_op_gemm_int8``): o = act(a_scale[m] w_scale[n] (a @ w.T)[m, n] + bias[n]); a [M, K], w [N, K] int8 with rows on 16 bytes
         (``op_quantize_int8`` makes such), scales and bias fp32.  epi as ``op_gemm``: 0 none, 1 GELU(tanh), 2 SiLU -> o [M, N]; 3: ``out`` (None: not written) takes o, and
         ``resid_out`` (None: ``resid`` itself) takes resid + (gate_table[n] + gate_mod[m // rows_per_batch, n]) * o -> out.  ``kernel``: one by name, the same bits."""
-        for name, t in (("a", a), ("w", w)):
-            if not isinstance(t, torch.Tensor) or t.dim() != 2:
-                raise ValueError(f"{name} must have two dimensions")
+        if not isinstance(a, torch.Tensor) or not isinstance(w, torch.Tensor) or a.dim() != 2 or w.dim() != 2:
+            raise ValueError("a and w must have two dimensions")
         (M, K), N = a.shape, w.shape[0]
-        self._check("a", a, torch.int8, rows=True)
-        self._check("w", w, torch.int8, (N, K), rows=True)
-        self._check("a_scale", a_scale, torch.float32, (M,))
-        self._check("w_scale", w_scale, torch.float32, (N,))
-        self._check("bias", bias, torch.float32, (N,))
+        self._rows("a", a, torch.int8, M, K)
+        self._rows("w", w, torch.int8, N, K)
         if a_scale is None or w_scale is None:
             raise ValueError("a_scale and w_scale are needed")
+        sa, sw, b = self._vector("a_scale", a_scale, M), self._vector("w_scale", w_scale, N), self._vector("bias", bias, N)
         if kernel not in self.INT8_KERNELS:
             raise ValueError(f"kernel {kernel!r} unknown: one of {', '.join(self.INT8_KERNELS)}")
-        mod_stride = 0
+        r = ro = gt = gm = ldr = ldro = gs = po = ldo = 0
         if epi == 3:
             if resid is None:
                 raise ValueError("epilogue 3 needs resid")
-            self._check("resid", resid, self.dtype, (M, N), rows=True)
-            self._check("gate_table", gate_table, torch.float32, (N,))
-            mod_stride = self._check_mods(M, N, rows_per_batch, gate_mod=gate_mod)
+            ldr, gt, (gm, gs) = self._rows("resid", resid, self.dtype, M, N), self._vector("gate_table", gate_table, N), self._mod("gate_mod", gate_mod, M, N, rows_per_batch)
             resid_out = resid if resid_out is None else resid_out
-            self._check("resid_out", resid_out, self.dtype, (M, N), rows=True)
-            self._distinct("resid_out", resid_out)
-            same = resid_out.data_ptr() == resid.data_ptr() and resid_out.stride() == resid.stride()
-            self._apart("resid_out", resid_out, a=a, a_scale=a_scale, w=w, w_scale=w_scale, bias=bias, gate_table=gate_table, gate_mod=gate_mod, resid=None if same else resid, out=out)
-        else:
-            if resid is not None or gate_table is not None or gate_mod is not None or resid_out is not None:
-                raise ValueError("resid and gates belong to epilogue 3")
-        if out is None and epi != 3:
+            ldro = self._rows("resid_out", resid_out, self.dtype, M, N)
+            r, ro = resid.data_ptr(), resid_out.data_ptr()
+        elif resid is not None or gate_table is not None or gate_mod is not None or resid_out is not None:
+            raise ValueError("resid and gates belong to epilogue 3")
+        elif out is None:
             out = torch.empty((M, N), device=self.device, dtype=self.dtype)
-        elif out is not None:
-            self._check("out", out, self.dtype, (M, N), rows=True)
-            self._distinct("out", out)
-            self._apart("out", out, a=a, a_scale=a_scale, w=w, w_scale=w_scale, bias=bias, gate_table=gate_table, gate_mod=gate_mod, resid=resid)
-        self._chk(self.lib.ecad_op_gemm_int8(
-            self._h, self.INT8_KERNELS[kernel], int(epi), a.data_ptr(), _row_stride(a), a_scale.data_ptr(), w.data_ptr(), _row_stride(w), w_scale.data_ptr(), _ptr(bias), _ptr(out),
-            0 if out is None else _row_stride(out), _ptr(resid), 0 if resid is None else _row_stride(resid), _ptr(resid_out), 0 if resid_out is None else _row_stride(resid_out), _ptr(gate_table),
-            _ptr(gate_mod), mod_stride, int(rows_per_batch), M, N, K, self._stream()))
+        if out is not None:
+            ldo, po = self._rows("out", out, self.dtype, M, N), out.data_ptr()
+        args = L.INT8_GEMM.pack(a.data_ptr(), a.stride(0), sa, w.data_ptr(), w.stride(0), sw, b, po, ldo, r, ldr, ro, ldro, gt, gm, gs, M, N, K, int(epi), int(rows_per_batch),
+                                self.INT8_KERNELS[kernel])
+        self._chk(self.lib.ecad_op_gemm_int8(self._h, args, self._stream()))
         return out
 
     NORMS = {"none": 0, "rms": 1, "layer": 2}
@@ -574,53 +529,41 @@ class EcadEngine:
         M, D = h.shape
         if pre not in self.NORMS or post not in self.NORMS:
             raise ValueError(f"pre and post are one of {', '.join(self.NORMS)}, got {pre!r} and {post!r}")
-        if quantize and pre == "none":
-            raise ValueError("nothing to quantise without a pre-norm")
-        self._check("h", h, self.dtype, rows=True)
-        self._check("y", y, self.dtype, (M, D), rows=True)
-        for name, t in (("pre_weight", pre_weight), ("post_weight", post_weight), ("gate_table", gate_table), ("table_shift", table_shift), ("table_scale", table_scale)):
-            self._check(name, t, torch.float32, (D,))
-        gate_stride = self._check_mods(M, D, rows_per_batch, gate_mod=gate_mod)
-        mod_stride = self._check_mods(M, D, rows_per_batch, mod_shift=mod_shift, mod_scale=mod_scale)
-        inputs = dict(pre_weight=pre_weight, post_weight=post_weight, gate_table=gate_table, table_shift=table_shift, table_scale=table_scale, gate_mod=gate_mod, mod_shift=mod_shift,
-                      mod_scale=mod_scale)
+        dt, ldh = self.dtype, self._rows("h", h, self.dtype, M, D)
         new_h, n, q, q_scale = h, None, None, None
+        py = ldy = ph = ldho = pn = ldn = pq = ldq = ps = 0
         if y is not None:
-            if out_h is None:
-                new_h = torch.empty((M, D), device=self.device, dtype=self.dtype)
-            else:
-                new_h = out_h
-                self._check("out_h", out_h, self.dtype, (M, D), rows=True)
-                self._distinct("out_h", out_h)
-                self._apart("out_h", out_h, h=None if _same(out_h, h) else h, y=y, **inputs)
+            ldy, py = self._rows("y", y, dt, M, D), y.data_ptr()
+            new_h = torch.empty((M, D), device=self.device, dtype=dt) if out_h is None else out_h
+            ldho, ph = self._rows("out_h", new_h, dt, M, D), new_h.data_ptr()
         elif out_h is not None:
             raise ValueError("out_h without y: h' is h")
         if pre == "none":
-            if out_n is not None:
-                raise ValueError("out_n without a pre-norm")
+            if out_n is not None or quantize:
+                raise ValueError("out_n or quantize without a pre-norm")
         elif quantize:
             if out_n is None:
-                q = torch.empty((M, (D + 15) // 16 * 16), device=self.device, dtype=torch.int8)[:, :D]
-                q_scale = torch.empty((M,), device=self.device, dtype=torch.float32)
+                q, q_scale = self._new_int8_rows(M, D), torch.empty((M,), device=self.device, dtype=torch.float32)
+                ldq = (D + 15) & ~15
             else:
                 q, q_scale = out_n
-                self._check("q", q, torch.int8, (M, D), rows=True)
-                self._check("scale", q_scale, torch.float32, (M,))
-                self._distinct("q", q)
-                self._apart("q", q, h=h, y=y, out_h=new_h, scale=q_scale, **inputs)
-                self._apart("scale", q_scale, h=h, y=y, out_h=new_h, **inputs)
-        elif out_n is None:
-            n = torch.empty((M, D), device=self.device, dtype=self.dtype)
+                ldq = self._rows("q", q, torch.int8, M, D)
+                ldq = q.stride(0) if M == 1 else ldq
+                if q_scale is None:
+                    raise ValueError("out_n must be (q, scale)")
+            pq, ps = q.data_ptr(), self._vector("scale", q_scale, M)
         else:
-            n = out_n
-            self._check("out_n", n, self.dtype, (M, D), rows=True)
-            self._distinct("out_n", n)
-            self._apart("out_n", n, h=h, y=None if y is not None and _same(n, y) else y, out_h=new_h, **inputs)
-        args = L.EcadGateNorm(
-            h.data_ptr(), _row_stride(h), _ptr(y), 0 if y is None else _row_stride(y), None if y is None else new_h.data_ptr(), _row_stride(new_h), _ptr(n), 0 if n is None else _row_stride(n),
-            _ptr(q), 0 if q is None else _row_stride(q), _ptr(q_scale), _ptr(post_weight), _ptr(pre_weight), _ptr(gate_table), _ptr(gate_mod), gate_stride, _ptr(table_shift), _ptr(table_scale),
-            _ptr(mod_shift), _ptr(mod_scale), mod_stride, M, D, int(rows_per_batch), self.NORMS[post], self.NORMS[pre], float(resid_scale), self.cfg.norm_eps if eps is None else float(eps))
-        self._chk(self.lib.ecad_op_gate_norm(self._h, C.byref(args), self._stream()))
+            n = torch.empty((M, D), device=self.device, dtype=dt) if out_n is None else out_n
+            ldn, pn = self._rows("out_n", n, dt, M, D), n.data_ptr()
+        gm, gs = self._mod("gate_mod", gate_mod, M, D, rows_per_batch)
+        ms, ss = self._mod("mod_shift", mod_shift, M, D, rows_per_batch)
+        mc, cs = self._mod("mod_scale", mod_scale, M, D, rows_per_batch)
+        if ss and cs and ss != cs:
+            raise ValueError(f"mod_shift and mod_scale must have the same stride between samples, got {ss} and {cs}")
+        args = L.GATE_NORM.pack(h.data_ptr(), ldh, py, ldy, ph, ldho, pn, ldn, pq, ldq, ps, self._vector("post_weight", post_weight, D), self._vector("pre_weight", pre_weight, D),
+                                self._vector("gate_table", gate_table, D), gm, gs, self._vector("table_shift", table_shift, D), self._vector("table_scale", table_scale, D), ms, mc, ss or cs, M, D,
+                                int(rows_per_batch), self.NORMS[post], self.NORMS[pre], 0, float(resid_scale), self.cfg.norm_eps if eps is None else float(eps))
+        self._chk(self.lib.ecad_op_gate_norm(self._h, args, self._stream()))
         return new_h, (q, q_scale) if quantize else n
 
     ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
@@ -629,24 +572,32 @@ class EcadEngine:
         """Cosines and sines of rotary positions (``ecad_op_rope_table``): positions [S] or [S, axes] int32 or fp32 -> [S, sum(axes_dims) / 2, 2] fp32, angles in 64 bits.
         axes_dims: elements that turn with each axis (even; an int for one axis), e.g. (16, 56, 56) for FLUX's (index, row, column).  scaling "linear" (f / factor), "ntk" (theta
         factor^(d / (d - 2))) or "yarn" (pairs that turn often within ``original_length`` stay, the others are stretched; cosine and sine times 0.1 ln(factor) + 1)."""
-        dims = (int(axes_dims),) if isinstance(axes_dims, int) else tuple(int(d) for d in axes_dims)
+        dims = (axes_dims,) if isinstance(axes_dims, int) else tuple(axes_dims)
         if not isinstance(positions, torch.Tensor) or positions.dim() not in (1, 2) or positions.dtype not in (torch.int32, torch.float32):
             raise ValueError("positions must be an int32 or float32 tensor of shape (S,) or (S, axes)")
+        S = positions.shape[0]
         if (positions.shape[1] if positions.dim() == 2 else 1) != len(dims):
             raise ValueError(f"positions of shape {tuple(positions.shape)} for {len(dims)} axes")
         if scaling not in self.ROPE_SCALINGS:
             raise ValueError(f"scaling {scaling!r} unknown: one of {', '.join(self.ROPE_SCALINGS)}")
-        self._check("positions", positions, positions.dtype)
-        S = positions.shape[0]
+        if positions.device != self.device or not positions.is_contiguous() or (positions.requires_grad and torch.is_grad_enabled()):
+            self._refuse("positions", positions, positions.dtype, positions.shape, "be contiguous")
         shape = (S, max(0, sum(dims)) // 2, 2)
         if out is None:
             out = torch.empty(shape, device=self.device, dtype=torch.float32)
-        else:
-            self._check("out", out, torch.float32, shape)
-            self._apart("out", out, positions=positions)
-        self._chk(self.lib.ecad_op_rope_table(self._h, positions.data_ptr(), int(positions.dtype == torch.float32), (C.c_int32 * len(dims))(*dims), len(dims), S, self.ROPE_SCALINGS[scaling],
-                                              float(theta), float(factor), float(original_length), float(beta_fast), float(beta_slow), out.data_ptr(), self._stream()))
+        elif not isinstance(out, torch.Tensor) or out.shape != shape or out.dtype is not torch.float32 or out.device != self.device or not out.is_contiguous():
+            self._refuse("out", out, torch.float32, shape, "be contiguous")
+        self._chk(self.lib.ecad_op_rope_table(self._h, positions.data_ptr(), int(positions.dtype is torch.float32), (C.c_int32 * len(dims))(*dims), len(dims), S, self.ROPE_SCALINGS[scaling],
+                                              theta, factor, original_length, beta_fast, beta_slow, out.data_ptr(), self._stream()))
         return out
+
+    def _heads(self, name: str, t, shape: tuple) -> tuple:
+        """Strides (sample, token, head) of [B, S, H, D] with dense heads."""
+        if isinstance(t, torch.Tensor) and t.dtype is self.dtype and t.shape == shape and t.device == self.device and not (t.requires_grad and torch.is_grad_enabled()):
+            sample, token, head, one = t.stride()
+            if one == 1 or shape[3] <= 1:
+                return sample, token, head
+        self._refuse(name, t, self.dtype, shape, "have dense heads")
 
     def op_rope(self, q, k, table, layout="interleaved", index=None, inverse=False, out=None):
         """Rotary positions applied to heads (``ecad_op_rope``): q [B, S, Hq, D], k [B, S, Hk, D] (or None) at any strides with dense heads, e.g. column slices of a fused
@@ -655,42 +606,41 @@ class EcadEngine:
         ``inverse`` turns back.  Returns (q', k'): new tensors, or ``out`` = (q_out, k_out), which may be (q, k) themselves."""
         if layout not in ("interleaved", "half"):
             raise ValueError(f"layout {layout!r} unknown: interleaved or half")
-        for name, t in (("q", q), ("k", k)):
-            if (t is None and name == "q") or (t is not None and (not isinstance(t, torch.Tensor) or t.dim() != 4)):
-                raise ValueError(f"{name} must have shape (samples, tokens, heads, elements)")
-            self._check(name, t, self.dtype, rows=True)
-        B, S, Hq, D = q.shape
-        Hk = 0
-        if k is not None:
-            Hk = k.shape[2]
-            if k.shape != (B, S, Hk, D) or Hk < 1:
-                raise ValueError(f"k of shape {tuple(k.shape)} for q of shape {tuple(q.shape)}")
+        if not isinstance(q, torch.Tensor) or q.dim() != 4:
+            raise ValueError("q must have shape (samples, tokens, heads, elements)")
+        shape = B, S, Hq, D = q.shape
+        strides = self._heads("q", q, shape)
         if not isinstance(table, torch.Tensor) or table.dim() != 3 or table.shape[2] != 2:
             raise ValueError("table must have shape (rows, pairs, 2)")
-        self._check("table", table, torch.float32)
-        index_stride = 0
+        rows, pairs, _ = table.shape
+        if table.dtype is not torch.float32 or table.device != self.device or not table.is_contiguous() or (table.requires_grad and torch.is_grad_enabled()):
+            self._refuse("table", table, torch.float32, table.shape, "be contiguous")
+        at = index_stride = 0
         if index is not None:
             if not isinstance(index, torch.Tensor) or index.shape not in ((S,), (B, S)):
                 raise ValueError(f"index must have shape ({S},) or ({B}, {S})")
-            self._check("index", index, torch.int32, rows=True)
-            index_stride = index.stride(0) if index.dim() == 2 and B > 1 else 0
+            if index.dtype is not torch.int32 or index.device != self.device or (S > 1 and index.stride(-1) != 1):
+                self._refuse("index", index, torch.int32, index.shape, "have a dense last dimension")
+            at, index_stride = index.data_ptr(), index.stride(0) if index.dim() == 2 and B > 1 else 0
         if out is None:
-            q_out, k_out = torch.empty((B, S, Hq, D), device=self.device, dtype=self.dtype), None if k is None else torch.empty((B, S, Hk, D), device=self.device, dtype=self.dtype)
+            q_out, k_out = torch.empty(shape, device=self.device, dtype=self.dtype), None
         else:
             q_out, k_out = out
-            if (k is None) != (k_out is None) or q_out is None:
+            if (k is None) != (k_out is None):
                 raise ValueError("out must be (q_out, k_out), k_out None where k is None")
-            for name, t, x, other in (("q_out", q_out, q, k), ("k_out", k_out, k, q)):
-                if t is None:
-                    continue
-                self._check(name, t, self.dtype, x.shape, rows=True)
-                self._distinct(name, t)
-                self._apart(name, t, x=None if _same(t, x) else x, other=other, table=table, index=index, other_out=k_out if t is q_out else None)
-        three = C.c_int64 * 3
-        self._chk(self.lib.ecad_op_rope(
-            self._h, q.data_ptr(), three(*q.stride()[:3]), q_out.data_ptr(), three(*q_out.stride()[:3]), Hq, _ptr(k), None if k is None else three(*k.stride()[:3]), _ptr(k_out),
-            None if k is None else three(*k_out.stride()[:3]), Hk, table.data_ptr(), table.shape[0], _ptr(index), index_stride, B, S, D, 2 * table.shape[1], int(layout == "half"), int(bool(inverse)),
-            self._stream()))
+        out_strides = self._heads("q_out", q_out, shape)
+        heads = (q.data_ptr(), q_out.data_ptr(), *strides, *out_strides, Hq)
+        keys = (0,) * 9
+        if k is not None:
+            if not isinstance(k, torch.Tensor) or k.dim() != 4 or k.shape[2] < 1 or k.shape != (B, S, k.shape[2], D):
+                raise ValueError(f"k of shape {tuple(k.shape) if isinstance(k, torch.Tensor) else k} for q of shape {tuple(shape)}")
+            k_strides = self._heads("k", k, k.shape)
+            if out is None:
+                k_out = torch.empty(k.shape, device=self.device, dtype=self.dtype)
+            out_strides = self._heads("k_out", k_out, k.shape)
+            keys = (k.data_ptr(), k_out.data_ptr(), *k_strides, *out_strides, k.shape[2])
+        args = L.ROPE.pack(*heads, *keys, table.data_ptr(), at, index_stride, B, S, D, 2 * pairs, rows, layout == "half", bool(inverse), 0)
+        self._chk(self.lib.ecad_op_rope(self._h, args, self._stream()))
         return q_out, k_out
 
 

@@ -284,7 +284,8 @@ int ecad_op_qproj_attention(EcadEngine* e, int call_site, const void* x, const v
  * may be captured into a graph, and called from several streams.  They run on the engine's device whatever the current device is, and leave that as it was.
  * 16-bit tensors have the engine's dtype; rows may have any width and any stride (in elements) at the alignment of an element; 8-bit rows start on 16 bytes with a
  * stride of a multiple of 16 (so the last 16-byte piece of a row may be read whole; what lies behind the row's values does not matter).
- * Zero rows: nothing is done. */
+ * Zero rows: nothing is done.  Outputs that overlap themselves, each other or an input are refused (columns of one buffer side by side do not overlap), but for the
+ * in-place forms that each entry names. */
 
 /* q[i][k] = x[i][k] / scale[i] rounded to the nearest integer (exactly, ties to even), scale[i] = max_k |x[i][k]| / 127 as fp32.  A row of zeros: scale 0, zeros.
  * A row with an infinity or a NaN: scale NaN, zeros -- its products are NaN.  1 <= K < 131072.  Weights [N, K] are quantised by the same call, once. */
@@ -295,9 +296,20 @@ int ecad_op_quantize_int8(EcadEngine* e, const void* x, int64_t ldx, int8_t* q, 
  * neither is given; resid_out may be resid).  kernel: ECAD_I8_K_AUTO, or one by name (the same bits; ECAD_E_UNSUPPORTED if it cannot take the shape). */
 enum { ECAD_I8_K_AUTO = 0, ECAD_I8_K_ROWS = 1 /* up to 64 rows: operands straight to registers, K over the waves */, ECAD_I8_K_TILE64 = 2, ECAD_I8_K_TILE128 = 3, ECAD_I8_K_TILE144 = 4 /* 256 x 144 */,
        ECAD_I8_K_TILE256 = 5, ECAD_I8_K_TILE288 = 6 /* 256 x 288 */ };
-int ecad_op_gemm_int8(EcadEngine* e, int kernel, int epi, const int8_t* A, int64_t lda, const float* a_scale, const int8_t* W, int64_t ldw, const float* w_scale, const float* bias, void* out,
-                      int64_t ldo, const void* resid, int64_t ldr, void* resid_out, int64_t ldro, const float* gate_table, const void* gate_mod, int64_t gate_mod_stride, int rows_per_batch, int M,
-                      int N, int K, void* stream);
+typedef struct EcadInt8Gemm {
+  const int8_t* A; int64_t lda;
+  const float* a_scale;
+  const int8_t* W; int64_t ldw;
+  const float* w_scale;
+  const float* bias;
+  void* out; int64_t ldo;
+  const void* resid; int64_t ldr;
+  void* resid_out; int64_t ldro;
+  const float* gate_table;
+  const void* gate_mod; int64_t gate_mod_stride;
+  int32_t M, N, K, epi, rows_per_batch, kernel;
+} EcadInt8Gemm;
+int ecad_op_gemm_int8(EcadEngine* e, const EcadInt8Gemm* args, void* stream);
 
 /* h' = resid_scale * h + g * post(y);  n = pre(h') * (1 + s) + t.   post / pre: ECAD_NORM_*, x / sqrt(mean x^2 + eps) or (x - mean) / sqrt(var + eps), times weight[D]
  * where not NULL.  g = gate_table[D] + gate_mod[row / rows_per_batch][D] (1 where both are NULL), s and t in the same way from table_scale / mod_scale and
@@ -320,7 +332,7 @@ typedef struct EcadGateNorm {
   const float* table_scale;
   const void* mod_shift;
   const void* mod_scale; int64_t mod_stride;
-  int32_t M, D, rows_per_batch, post, pre;
+  int32_t M, D, rows_per_batch, post, pre, reserved;
   float resid_scale, eps;
 } EcadGateNorm;
 int ecad_op_gate_norm(EcadEngine* e, const EcadGateNorm* args, void* stream);
@@ -335,11 +347,23 @@ int ecad_op_rope_table(EcadEngine* e, const void* positions, int positions_float
                        double beta_fast, double beta_slow, float* table, void* stream);
 
 /* Turns the first `rot` elements of every head by table[row][rot / 2][2], the others stay: pair j = elements (2j, 2j + 1), or (j, j + rot / 2) with `half`; `inverse`
- * turns back (which is also the gradient's rotation).  Queries q [B, S, Hq, D] and keys k [B, S, Hk, D] (Hk 0: queries only) at any strides {sample, token, head};
- * the elements of a head are contiguous.  q_out == q (and k_out == k, same strides): in place.  row = index[b * index_stride + s] (index_stride 0: one list for all samples), or s
+ * turns back (which is also the gradient's rotation).  Queries [B, S, Hq, D] and keys [B, S, Hk, D] (Hk 0: queries only) at any strides; the elements of a
+ * head are contiguous.  out == x (for both, at the same strides): in place.  row = index[b * index_stride + s] (index_stride 0: one list for all samples), or s
  * where index is NULL; a token whose index lies outside the table is not turned. */
-int ecad_op_rope(EcadEngine* e, const void* q, const int64_t* q_strides, void* q_out, const int64_t* q_out_strides, int Hq, const void* k, const int64_t* k_strides, void* k_out,
-                 const int64_t* k_out_strides, int Hk, const float* table, int table_rows, const int32_t* index, int64_t index_stride, int B, int S, int D, int rot, int half, int inverse, void* stream);
+typedef struct EcadRopeHeads {
+  const void* x;  /* NULL with H 0 */
+  void* out;
+  int64_t sample, token, head;             /* strides of x, in elements */
+  int64_t out_sample, out_token, out_head;
+  int64_t H;
+} EcadRopeHeads;
+typedef struct EcadRope {
+  EcadRopeHeads q, k;
+  const float* table;
+  const int32_t* index; int64_t index_stride;
+  int32_t B, S, D, rot, table_rows, half, inverse, reserved;
+} EcadRope;
+int ecad_op_rope(EcadEngine* e, const EcadRope* args, void* stream);
 
 /* ---- decode tail: AutoencoderKL decoder + postprocess ------------------------------------------------
  * Replaces `self.vae.decode(latents / scaling_factor)` and `image_processor.postprocess(..., "pil")` inside the reference's
