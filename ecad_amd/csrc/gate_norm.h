@@ -29,8 +29,9 @@ struct GateNormArgs {
   float resid_scale, eps;
 };
 
-// mean (layer) and 1 / sqrt(. + eps) of the values of a row that is spread over WAVES waves, CH pieces per lane; lanes and pieces beyond the row hold zeros
-template <int WAVES, int CH>
+// mean (layer) and 1 / sqrt(. + eps) of the values of a row that is spread over WAVES waves, CH pieces per lane; lanes and pieces beyond the row hold zeros.
+// RAGGED: the row's last piece is not whole.
+template <int WAVES, int CH, bool RAGGED>
 ECAD_DEV void row_statistics(const float (&x)[CH][8], int kind, int first, int D, float eps, unsigned (*scratch)[WAVES], int& turn, float& mean, float& rstd) {
   const float inv_d = 1.0f / (float)D;
   mean = 0.f;
@@ -46,147 +47,157 @@ ECAD_DEV void row_statistics(const float (&x)[CH][8], int kind, int first, int D
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int left = D - (first + i * WAVES * 512);
+    float part = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float d = e < left ? x[i][e] - mean : 0.f;
-      sq += d * d;
+      const float d = RAGGED && e >= left ? 0.f : x[i][e] - mean;
+      part += d * d;
     }
+    sq += left > 0 ? part : 0.f;
   }
   rstd = 1.0f / sqrtf(row_all<WAVES>(sq, AddOp{}, scratch, turn) * inv_d + eps);
 }
 
-// A row on WAVES waves, CH pieces of eight elements per lane; a workgroup of 256 threads (or WAVES waves) takes rows_per_group consecutive rows.  The channel
-// vectors g, 1 + s, t of a sample stay in registers from row to row: read anew for every row they are up to 26 bytes per element out of L2 against the 8 that
-// the rows themselves move.
-template <typename T, int WAVES, int CH>
+template <typename T, bool RAGGED> ECAD_DEV Pack8 row_piece(const T* p, int left) {
+  if constexpr (RAGGED) return load_piece<T>(p, left);
+  Pack8 v;
+  v.u = (u32x4){0, 0, 0, 0};
+  if (left > 0) v.u = reinterpret_cast<const Bytes16*>(p)->u;
+  return v;
+}
+template <typename T, bool RAGGED> ECAD_DEV void row_store(T* p, const Pack8& v, int left) {
+  if constexpr (RAGGED) store_piece<T>(p, v, left);
+  else if (left > 0) reinterpret_cast<Bytes16*>(p)->u = v.u;
+}
+
+// A row on WAVES waves, CH pieces of eight elements per lane; every wave (or workgroup of a wider row) takes rows_per_group consecutive rows, the next one's
+// loads in flight while one is worked on.  The channel vectors g, 1 + s, t of a sample stay in registers from row to row: read anew for every row they are up to
+// 26 bytes per element out of L2 against the 8 that the rows themselves move.  They are zero beyond the row, and with them everything that is computed there.
+// HOLD false (rows of more than 8192 values on 16 waves, whose lanes have 128 registers): read anew all the same.
+template <typename T, int WAVES, int CH, bool RAGGED, bool HOLD>
 __global__ __launch_bounds__(WAVES > 4 ? WAVES * 64 : 256) void gate_norm_kernel(const GateNormArgs p) {
   constexpr int SLOTS = WAVES >= 4 ? 1 : 4 / WAVES;  // rows a workgroup works on at a time
   __shared__ unsigned scratch_all[SLOTS][2][WAVES];
-  const int slot = WAVES >= 4 ? 0 : (threadIdx.x >> 6) / WAVES;
+  const int slot = WAVES >= 4 ? 0 : __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) / WAVES);
   unsigned(*scratch)[WAVES] = scratch_all[slot];
   const int lane = WAVES >= 4 ? threadIdx.x : (threadIdx.x & (64 * WAVES - 1));
   const int first = lane * 8;
   int turn = 0;
-  float G[CH][8], A[CH][8], B[CH][8];
+  float G[HOLD ? CH : 1][8], A[HOLD ? CH : 1][8], B[HOLD ? CH : 1][8];
   int have = -1;  // the sample that G, A, B belong to
   const int64_t row0 = ((int64_t)blockIdx.x * SLOTS + slot) * p.rows_per_group;
-  // every wave of a workgroup makes the same number of turns: barriers inside (WAVES > 1) are met by all, and a wave without a row repeats the last one unwritten
-  for (int r = 0; r < p.rows_per_group; ++r) {
-    const int64_t row_ = row0 + r;
-    if (WAVES == 1 && row_ >= p.M) break;
-    const bool live = row_ < p.M;
-    const int64_t row = live ? row_ : p.M - 1;
+  // rows_per_group and M are the same for all waves of a row: they leave the loop together (the barriers inside are a row's own where WAVES > 1)
+  const int64_t end = row0 + p.rows_per_group < p.M ? row0 + p.rows_per_group : p.M;
+  Pack8 hv[CH], yv[CH];
+  auto fetch = [&](int64_t row) {
     const T* hrow = reinterpret_cast<const T*>(p.h) + row * p.ldh;
     const T* yrow = reinterpret_cast<const T*>(p.y) + row * p.ldy;
-    Pack8 hv[CH], yv[CH];
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int c = first + i * WAVES * 512;
-      hv[i] = load_piece<T>(hrow + c, p.D - c);
-      if (p.y) yv[i] = load_piece<T>(yrow + c, p.D - c);
+      hv[i] = row_piece<T, RAGGED>(hrow + c, p.D - c);
+      if (p.y) yv[i] = row_piece<T, RAGGED>(yrow + c, p.D - c);
     }
-    const int b = (int)(row / p.rows_per_batch);
-    if (b != have) {
-      have = b;
-      const T* gm = reinterpret_cast<const T*>(p.gate_mod) + (int64_t)b * p.gate_stride;
-      const T* sm = reinterpret_cast<const T*>(p.mod_scale) + (int64_t)b * p.mod_stride;
-      const T* tm = reinterpret_cast<const T*>(p.mod_shift) + (int64_t)b * p.mod_stride;
+  };
+  if (row0 < end) fetch(row0);
+  for (int64_t row = row0; row < end; ++row) {
+    const int b = (int)((unsigned)row / (unsigned)p.rows_per_batch);
+    // the vectors of piece i: the gate's (what & 1) or scale and shift (what & 2)
+    auto channels = [&](int i, int at, int what) {
+      const int c = first + i * WAVES * 512, n = p.D - c;
+      float f[8];
+      auto table = [&](const float* v, auto&& put) {
+        if (!v) return;
+        load_floats(v + c, n, f);
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const int c = first + i * WAVES * 512, n = p.D - c;
-        float f[8];
+        for (int e = 0; e < 8; ++e) put(e);
+      };
+      auto mod = [&](const void* base, int64_t stride, auto&& put) {
+        if (!base) return;
+        unpack8<T>(load_piece<T>(reinterpret_cast<const T*>(base) + (int64_t)b * stride + c, n), f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) G[i][e] = p.gate_table || p.gate_mod ? 0.f : 1.f, A[i][e] = 1.f, B[i][e] = 0.f;
-        if (p.gate_table) {
-          load_floats(p.gate_table + c, n, f);
+        for (int e = 0; e < 8; ++e) put(e);
+      };
+      if (what & 1) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) G[i][e] = f[e];
-        }
-        if (p.gate_mod) {
-          unpack8<T>(load_piece<T>(gm + c, n), f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) G[i][e] += f[e];
-        }
-        if (p.post_weight) {
-          load_floats(p.post_weight + c, n, f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) G[i][e] *= f[e];
-        }
-        if (p.table_scale) {
-          load_floats(p.table_scale + c, n, f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) A[i][e] += f[e];
-        }
-        if (p.mod_scale) {
-          unpack8<T>(load_piece<T>(sm + c, n), f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) A[i][e] += f[e];
-        }
-        if (p.pre_weight) {
-          load_floats(p.pre_weight + c, n, f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) A[i][e] *= f[e];
-        }
-        if (p.table_shift) {
-          load_floats(p.table_shift + c, n, f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) B[i][e] = f[e];
-        }
-        if (p.mod_shift) {
-          unpack8<T>(load_piece<T>(tm + c, n), f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) B[i][e] += f[e];
-        }
+        for (int e = 0; e < 8; ++e) G[at][e] = p.gate_table || p.gate_mod ? 0.f : 1.f;
+        table(p.gate_table, [&](int e) { G[at][e] = f[e]; });
+        mod(p.gate_mod, p.gate_stride, [&](int e) { G[at][e] += f[e]; });
+        table(p.post_weight, [&](int e) { G[at][e] *= f[e]; });
       }
+      if (what & 2) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) A[at][e] = 1.f, B[at][e] = 0.f;
+        table(p.table_scale, [&](int e) { A[at][e] += f[e]; });
+        mod(p.mod_scale, p.mod_stride, [&](int e) { A[at][e] += f[e]; });
+        table(p.pre_weight, [&](int e) { A[at][e] *= f[e]; });
+        table(p.table_shift, [&](int e) { B[at][e] = f[e]; });
+        mod(p.mod_shift, p.mod_stride, [&](int e) { B[at][e] += f[e]; });
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e >= n) {
+          if (what & 1) G[at][e] = 0.f;
+          if (what & 2) A[at][e] = B[at][e] = 0.f;
+        }
+    };
+    if (HOLD && b != have) {
+      have = b;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) channels(i, i, 3);
     }
     float x[CH][8];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) unpack8<T>(hv[i], x[i]);
     if (p.y) {
       float u[CH][8], mean = 0.f, rstd = 1.f;
 #pragma unroll
       for (int i = 0; i < CH; ++i) unpack8<T>(yv[i], u[i]);
-      if (p.post) row_statistics<WAVES, CH>(u, p.post, first, p.D, p.eps, scratch, turn, mean, rstd);
+      if (row + 1 < end) fetch(row + 1);
+      if (p.post) row_statistics<WAVES, CH, RAGGED>(u, p.post, first, p.D, p.eps, scratch, turn, mean, rstd);
       T* ho = reinterpret_cast<T*>(p.h_out) + row * p.ldho;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
-        const int c = first + i * WAVES * 512;
-        unpack8<T>(hv[i], x[i]);
+        const int c = first + i * WAVES * 512, at = HOLD ? i : 0;
+        if constexpr (!HOLD) channels(i, 0, 1);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = c + e < p.D ? p.resid_scale * x[i][e] + (u[i][e] - mean) * rstd * G[i][e] : 0.f;
-        if (live) store_piece<T>(ho + c, pack8<T>(x[i]), p.D - c);
+        for (int e = 0; e < 8; ++e) x[i][e] = p.resid_scale * x[i][e] + (u[i][e] - mean) * rstd * G[at][e];
+        row_store<T, RAGGED>(ho + c, pack8<T>(x[i]), p.D - c);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < CH; ++i) unpack8<T>(hv[i], x[i]);
+    } else if (row + 1 < end) {
+      fetch(row + 1);
     }
     if (p.pre == NORM_NONE) continue;
     float mean, rstd;
-    row_statistics<WAVES, CH>(x, p.pre, first, p.D, p.eps, scratch, turn, mean, rstd);
+    row_statistics<WAVES, CH, RAGGED>(x, p.pre, first, p.D, p.eps, scratch, turn, mean, rstd);
     Pack8 nv[CH];
     u16x2 m = {0, 0};
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int c = first + i * WAVES * 512;
+      const int at = HOLD ? i : 0;
+      if constexpr (!HOLD) channels(i, 0, 2);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][e] = c + e < p.D ? (x[i][e] - mean) * rstd * A[i][e] + B[i][e] : 0.f;
+      for (int e = 0; e < 8; ++e) x[i][e] = (x[i][e] - mean) * rstd * A[at][e] + B[at][e];
       nv[i] = pack8<T>(x[i]);
-      m = max_bits(m, nv[i]);
     }
     if (p.q) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) m = max_bits(m, nv[i]);
       const unsigned bits = row_all<WAVES>(fold_bits(m), MaxOp{}, scratch, turn);
       const Int8Scale k = int8_scale<T>(bits);
-      if (live && lane == 0) p.q_scale[row] = k.s;
+      if (lane == 0) p.q_scale[row] = k.s;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int c = first + i * WAVES * 512;
         unpack8<T>(nv[i], x[i]);
-        if (live) store_int8_piece(p.q + row * p.ldq + c, int8_piece(x[i], k), p.D - c);
+        store_int8_piece(p.q + row * p.ldq + c, int8_piece(x[i], k), p.D - c);
       }
     } else {
       T* no = reinterpret_cast<T*>(p.n_out) + row * p.ldn;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int c = first + i * WAVES * 512;
-        if (live) store_piece<T>(no + c, nv[i], p.D - c);
+        row_store<T, RAGGED>(no + c, nv[i], p.D - c);
       }
     }
   }

@@ -9,6 +9,7 @@
 // Operands: rows of 8-bit integers on 16 bytes, any M, N, K.  The last 16-byte piece of a row may reach past column K: it stays inside the aligned 16 bytes that
 // hold a value of the row, and the bytes behind K are masked on the W side (zero times anything is zero).
 #pragma once
+#include "gemm_int8_asm.h"
 #include "row_ops.h"
 
 namespace ecad {
@@ -29,7 +30,7 @@ struct Int8GemmArgs {
   const float* gate_table;
   const void* gate_mod;
   int64_t lda, ldw, ldo, ldr, ldro, gate_stride;
-  int M, N, K, epi, rows_per_batch;
+  int M, N, K, rows_per_batch;
 };
 
 ECAD_DEV i32x4 mfma_i8(const Pack8& a, const Pack8& b, i32x4 c) {
@@ -57,13 +58,6 @@ ECAD_DEV float pinned(float v) {
   asm("" : "+v"(v));
   return v;
 }
-ECAD_DEV float int8_act(float v, int epi) {
-  v = pinned(v);
-  if (epi == I8_GELU) v = pinned(gelu_tanh(v));
-  if (epi == I8_SILU) v = pinned(silu(v));
-  return v;
-}
-
 // XCD-aware order: workgroups b, b + 8, ... share an XCD and get a run of neighbouring tiles, walked in strips of four tile rows, so that the tiles in flight on one
 // L2 share their A and W rows
 ECAD_DEV void int8_tile_of(int bid, int tiles_m, int tiles_n, int& tm, int& tn) {
@@ -76,95 +70,114 @@ ECAD_DEV void int8_tile_of(int bid, int tiles_m, int tiles_n, int& tm, int& tn) 
   tm = 4 * strip + in - tn * rows;
 }
 
-// Epilogue of a wave's block from its accumulators: lane (l15, g) holds row m = 16 i + l15, columns 16 j + 4 g .. + 3 of fragment (i, j).  Two neighbouring fragments
-// swap halves between lane rows, so a lane ends with eight consecutive columns: one 16-byte access per pair of fragments, 64 contiguous bytes of each of 16 rows.
-template <typename T, int FM, int FN, typename AccFn>
-ECAD_DEV void int8_epilogue(const Int8GemmArgs& p, int m_base, int n_base, AccFn&& acc) {
+template <int EPI> ECAD_DEV float int8_act(float v) {
+  v = pinned(v);
+  if constexpr (EPI == I8_GELU) v = pinned(gelu_tanh(v));
+  if constexpr (EPI == I8_SILU) v = pinned(silu(v));
+  return v;
+}
+
+// Epilogue of a tile from its accumulators: lane (l15, g) of a wave holds row m = 16 i + l15, columns 16 j + 4 g .. + 3 of fragment (i, j) of the wave's block at
+// (wm0, wn0) of the tile.
+//   Whole tiles of 16-byte rows without a residual leave straight from the registers: two neighbouring fragments swap halves between lane rows, so a lane ends with
+//   eight consecutive columns -- one 16-byte store per pair, 64 contiguous bytes of each of 16 rows -- and LDS stays free.
+//   Everything else goes through a row-major tile in LDS (the ring is done with) and leaves in a rolled loop of 16-byte pieces of rows: the residual's reads are
+//   contiguous, and edges need one piece of code instead of one per fragment.  (The accumulators can only be named by constants, so whatever stands beside them is
+//   unrolled 64 times: with the edges in there the kernel was 250 KB of code and spent 30 us of a 37 us one-round launch fetching it.)
+template <typename T, int BM, int BN, int FM, int FN, int NT, int EPI, typename AccFn>
+ECAD_DEV void int8_epilogue(const Int8GemmArgs& p, char* smem, int m0, int n0, int wm0, int wn0, AccFn&& acc) {
+  constexpr int CS = BN + 8;  // row stride of the tile in LDS: 16-byte rows, four banks apart
   const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+  const bool direct = EPI != I8_RESID && m0 + BM <= p.M && n0 + BN <= p.N && p.ldo % 8 == 0 && ((uintptr_t)p.out & 15) == 0;
   float sa[FM];
-  const T* gate[FM];
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
-    const int m = m_base + 16 * i + l15 < p.M ? m_base + 16 * i + l15 : p.M - 1;
-    sa[i] = p.sa[m];
-    gate[i] = reinterpret_cast<const T*>(p.gate_mod) + (p.epi == I8_RESID ? (int64_t)(m / p.rows_per_batch) * p.gate_stride : 0);
+    const int m = m0 + wm0 + 16 * i + l15;
+    sa[i] = p.sa[m < p.M ? m : p.M - 1];
   }
-  auto columns = [&](const float* v, int n, f32x4& f) {
-    f = (f32x4){0.f, 0.f, 0.f, 0.f};
-    if (!v) return;
-    if (n + 3 < p.N) {
-      f = reinterpret_cast<const Floats4*>(v + n)->f;
-    } else {
+  auto columns = [&](const float* v, int n) {
+    if (n + 3 < p.N) return reinterpret_cast<const Floats4*>(v + n)->f;
+    f32x4 f = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int r = 0; r < 3; ++r)
-        if (n + r < p.N) f[r] = v[n + r];
-    }
+    for (int r = 0; r < 3; ++r)
+      if (n + r < p.N) f[r] = v[n + r];
+    return f;
   };
-  static_for<(FN + 1) / 2>([&](auto jh) {
-    constexpr int j = 2 * decltype(jh)::value;
-    constexpr bool pair = j + 1 < FN;
-    f32x4 sw[2], bias[2];
+  auto packed = [&](auto ic, auto jc, const f32x4& sw, const f32x4& bias) {
+    const i32x4 a = acc(ic, jc);
+    float o[4];
 #pragma unroll
-    for (int h = 0; h < (pair ? 2 : 1); ++h) {
-      columns(p.sw, n_base + 16 * (j + h) + 4 * g, sw[h]);
-      columns(p.bias, n_base + 16 * (j + h) + 4 * g, bias[h]);
-    }
-    // where this lane's columns lie after the swap
-    const int n = pair ? n_base + 16 * (j + (g & 1)) + 8 * (g >> 1) : n_base + 16 * j + 4 * g;
-    const int left = p.N - n < (pair ? 8 : 4) ? p.N - n : (pair ? 8 : 4);
-    float table[8];
-    if (p.epi == I8_RESID) {
-      if (p.gate_table) load_floats(p.gate_table + n, left, table);
-      else
-#pragma unroll
-        for (int e = 0; e < 8; ++e) table[e] = p.gate_mod ? 0.f : 1.f;
-    }
-    static_for<FM>([&](auto ic) {
-      constexpr int i = decltype(ic)::value;
-      const int m = m_base + 16 * i + l15;
-      Pack8 v;
-      v.u = (u32x4){0, 0, 0, 0};
-#pragma unroll
-      for (int h = 0; h < (pair ? 2 : 1); ++h) {
-        const i32x4 a = h ? acc(ic, std::integral_constant<int, pair ? j + 1 : j>{}) : acc(ic, std::integral_constant<int, j>{});
-        float o[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = int8_act(__builtin_fmaf((float)a[r], sa[i] * sw[h][r], bias[h][r]), p.epi);
-        v.u[2 * h] = pack2<T>(o[0], o[1]);
-        v.u[2 * h + 1] = pack2<T>(o[2], o[3]);
-      }
-      if constexpr (pair) {
-        unsigned a0 = v.u[0], a1 = v.u[1], b0 = v.u[2], b1 = v.u[3];
-        swap_rows16(a0, b0);
-        swap_rows16(a1, b1);
-        v.u = (u32x4){a0, a1, b0, b1};
-      }
-      if (m < p.M) {
-        if (p.out) {
-          T* o = reinterpret_cast<T*>(p.out) + (int64_t)m * p.ldo + n;
-          if (!pair && left == 4) reinterpret_cast<Bytes8*>(o)->u = (u32x2){v.u[0], v.u[1]};
-          else store_piece<T>(o, v, left);
+    for (int r = 0; r < 4; ++r) o[r] = int8_act<EPI>(__builtin_fmaf((float)a[r], sa[decltype(ic)::value] * sw[r], bias[r]));
+    return (u32x2){pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3])};
+  };
+  if (direct) {
+    T* row = reinterpret_cast<T*>(p.out) + (int64_t)(m0 + wm0 + l15) * p.ldo + n0 + wn0;
+    static_for<(FN + 1) / 2>([&](auto jh) {
+      constexpr int j = 2 * decltype(jh)::value, j1 = j + 1 < FN ? j + 1 : j;
+      const int n = n0 + wn0 + 16 * j + 4 * g;
+      const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+      const f32x4 sw0 = columns(p.sw, n), b0 = p.bias ? columns(p.bias, n) : zero;
+      const f32x4 sw1 = columns(p.sw, n + 16 * (j1 - j)), b1 = p.bias ? columns(p.bias, n + 16 * (j1 - j)) : zero;
+      static_for<FM>([&](auto ic) {
+        T* at = row + (int64_t)(16 * decltype(ic)::value) * p.ldo + 16 * j;
+        const u32x2 lo = packed(ic, std::integral_constant<int, j>{}, sw0, b0);
+        if constexpr (j1 > j) {
+          const u32x2 hi = packed(ic, std::integral_constant<int, j1>{}, sw1, b1);
+          unsigned a0 = lo[0], a1 = lo[1], c0 = hi[0], c1 = hi[1];
+          swap_rows16(a0, c0);
+          swap_rows16(a1, c1);
+          *reinterpret_cast<u32x4*>(at + 16 * (g & 1) + 8 * (g >> 1)) = (u32x4){a0, a1, c0, c1};
+        } else {
+          *reinterpret_cast<u32x2*>(at + 4 * g) = lo;
         }
-        if (p.epi == I8_RESID) {
-          float o[8], h[8], gm[8];
-          unpack8<T>(v, o);
-          unpack8<T>(load_piece<T>(reinterpret_cast<const T*>(p.resid) + (int64_t)m * p.ldr + n, left), h);
-          if (p.gate_mod) unpack8<T>(load_piece<T>(gate[i] + n, left), gm);
-          else
-#pragma unroll
-            for (int e = 0; e < 8; ++e) gm[e] = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) h[e] = pinned(__builtin_fmaf(table[e] + gm[e], o[e], h[e]));
-          store_piece<T>(reinterpret_cast<T*>(p.resid_out) + (int64_t)m * p.ldro + n, pack8<T>(h), left);
-        }
-      }
+      });
     });
+    return;
+  }
+  T* tile = reinterpret_cast<T*>(smem);
+  static_for<FN>([&](auto jc) {
+    constexpr int j = decltype(jc)::value;
+    const int n = n0 + wn0 + 16 * j + 4 * g;
+    const f32x4 sw = columns(p.sw, n), bias = p.bias ? columns(p.bias, n) : (f32x4){0.f, 0.f, 0.f, 0.f};
+    static_for<FM>([&](auto ic) { *reinterpret_cast<u32x2*>(tile + (wm0 + 16 * decltype(ic)::value + l15) * CS + wn0 + 16 * j + 4 * g) = packed(ic, jc, sw, bias); });
   });
+  __syncthreads();
+  constexpr int CPR = BN / 8;
+  for (int it = threadIdx.x; it < BM * CPR; it += NT) {
+    const int r = it / CPR, c = (it - r * CPR) * 8, m = m0 + r, n = n0 + c, left = p.N - n;
+    if (m >= p.M || left <= 0) continue;
+    const Pack8 v = lds_read16(tile + r * CS + c);
+    if (EPI != I8_RESID || p.out) store_piece<T>(reinterpret_cast<T*>(p.out) + (int64_t)m * p.ldo + n, v, left);
+    if constexpr (EPI == I8_RESID) {
+      float o[8], h[8], gate[8];
+      unpack8<T>(v, o);
+      unpack8<T>(load_piece<T>(reinterpret_cast<const T*>(p.resid) + (int64_t)m * p.ldr + n, left), h);
+      if (p.gate_table) {
+        load_floats(p.gate_table + n, left, gate);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) gate[e] = p.gate_mod ? 0.f : 1.f;
+      }
+      if (p.gate_mod) {
+        float gm[8];
+        unpack8<T>(load_piece<T>(reinterpret_cast<const T*>(p.gate_mod) + (int64_t)(m / p.rows_per_batch) * p.gate_stride + n, left), gm);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) gate[e] += gm[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] = pinned(__builtin_fmaf(gate[e], o[e], h[e]));
+      store_piece<T>(reinterpret_cast<T*>(p.resid_out) + (int64_t)m * p.ldro + n, pack8<T>(h), left);
+    }
+  }
+}
+constexpr int int8_lds_bytes(int bm, int bn, int stages) {
+  const int ring = stages * (bm + bn) * 128, tile = bm * (bn + 8) * 2;
+  return ring > tile ? ring : tile;
 }
 
 // BM x BN tile on WM x WN waves.  A K-step is 128 bytes of every row of the tile: pieces of eight rows (1 KiB) travel straight to LDS, 16-byte chunks
 // XOR-swizzled by (row >> 1) & 7 on the source side, so that the fragment reads (16 rows x 16 bytes) meet every bank once.  One barrier per step, STAGES steps in a ring.
-template <typename T, int BM, int BN, int WM, int WN, int STAGES>
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, int EPI>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_int8_kernel(const Int8GemmArgs p) {
   constexpr int NW = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
   constexpr int A_BYTES = BM * 128, STAGE_BYTES = (BM + BN) * 128;
@@ -252,13 +265,102 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_int8_kernel(const Int8GemmA
     else step(slot, left, std::true_type{});
     slot = slot + 1 == STAGES ? 0 : slot + 1;
   }
-  int8_epilogue<T, FM, FN>(p, m0 + wm * (BM / WM), n0 + wn * (BN / WN), [&](auto ic, auto jc) -> i32x4 { return acc[decltype(ic)::value][decltype(jc)::value]; });
+  __syncthreads();
+  int8_epilogue<T, BM, BN, FM, FN, NW * 64, EPI>(p, smem, m0, n0, wm * (BM / WM), wn * (BN / WN), [&](auto ic, auto jc) -> i32x4 { return acc[decltype(ic)::value][decltype(jc)::value]; });
+}
+
+// The same product on one wave per SIMD, 256 x BN tiles on four waves: the K loop over whole stages is one hand-placed asm statement (gemm_int8_asm.h, generated by
+// scripts/gen_gemm_i8.py) that leaves the accumulators in AGPRs.  hipcc knows those only as clobbers of the statement: everything that touches them afterwards is asm
+// too, and the build fails if the compiler uses one before the last is read (scripts/audit_agpr.py).
+template <int BN> struct Int8Wide {
+  static constexpr bool tall = BN == 144;                      // waves stacked 4 x 1 (64 x 144 each), else 2 x 2 (128 x BN / 2)
+  static constexpr int FM = tall ? 4 : 8, FN = tall ? 9 : BN / 32, stages = tall ? 3 : 2;
+  static constexpr int fewest = tall ? GEMM_I8_PERIOD_144 : (BN == 256 ? GEMM_I8_PERIOD_256 : GEMM_I8_PERIOD_288);  // stages
+  static constexpr bool ninth = BN == 288;                     // the ninth column of fragments in registers of the caller
+  static constexpr int agpr(int i, int j) { return 4 * ((tall ? 9 : 8) * i + j); }
+};
+
+template <int R> ECAD_DEV i32x4 agpr_read() {
+  i32x4 v;
+  asm volatile("v_accvgpr_read_b32 %0, a%c4\n\tv_accvgpr_read_b32 %1, a%c5\n\tv_accvgpr_read_b32 %2, a%c6\n\tv_accvgpr_read_b32 %3, a%c7"
+               : "=v"(v[0]), "=v"(v[1]), "=v"(v[2]), "=v"(v[3])
+               : "i"(R), "i"(R + 1), "i"(R + 2), "i"(R + 3));
+  return v;
+}
+template <int R> ECAD_DEV void agpr_mfma(const Pack8& w, const Pack8& a) {
+  asm volatile("v_mfma_i32_16x16x64_i8 a[%c2:%c3], %0, %1, a[%c2:%c3]" : : "v"(w.u), "v"(a.u), "i"(R), "i"(R + 3));
+}
+
+ECAD_DEV void vgpr_mfma(i32x4& c, const Pack8& w, const Pack8& a) { asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+v"(c) : "v"(w.u), "v"(a.u)); }
+ECAD_DEV void settle(Pack8& p) { asm volatile("s_nop 4" : "+v"(p.u)); }  // between a vector write and an asm statement that multiplies with it
+
+template <typename T, int BN, int EPI>
+__global__ __launch_bounds__(256) void gemm_int8_wide_kernel(const Int8GemmArgs p) {
+  typedef Int8Wide<BN> G;
+  constexpr int BM = 256, FM = G::FM, FN = G::FN;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+  const unsigned wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm0 = G::tall ? 64 * wave : 128 * (wave & 1), wn0 = G::tall ? 0 : BN / 2 * (wave >> 1);
+  int tm, tn;
+  int8_tile_of(blockIdx.x, (p.M + BM - 1) / BM, (p.N + BN - 1) / BN, tm, tn);
+  const int m0 = tm * BM, n0 = tn * BN;
+  const int8_t* ap = p.A + (int64_t)m0 * p.lda;
+  const int8_t* wp = p.W + (int64_t)n0 * p.ldw;
+  const unsigned ra = p.M - m0 < BM ? p.M - m0 - 1 : BM - 1, rw = p.N - n0 < BN ? p.N - n0 - 1 : BN - 1;
+  i32x4 c8[8];
+  if constexpr (G::ninth) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c8[i] = (i32x4){0, 0, 0, 0};
+  }
+  {
+    const unsigned stages = (unsigned)p.K >> 7, rsa = (unsigned)p.lda, rsw = (unsigned)p.ldw, lds = __builtin_amdgcn_readfirstlane(lds_offset(smem)), zero = 1;
+    const unsigned trips = stages / G::fewest - 1, rem = stages % G::fewest;
+    if constexpr (BN == 256) { GEMM_I8_ASM_256(ap, wp, rsa, rsw, ra, rw, trips, rem, lds, wave, zero); }
+    else if constexpr (BN == 144) { GEMM_I8_ASM_144(ap, wp, rsa, rsw, ra, rw, trips, rem, lds, wave, zero); }
+    else { GEMM_I8_ASM_288(ap, wp, rsa, rsw, ra, rw, trips, rem, lds, wave, zero, c8); }
+  }
+  if (p.K & 127) {  // K behind the last whole stage: fragments straight from memory (a wave's own rows and columns), two matrix instructions per accumulator
+    const int k0 = p.K & ~127;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      Pack8 a[FM], w[FN];
+      const int k = k0 + 64 * s + 16 * g, left = p.K - k;
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const unsigned r = wm0 + 16 * i + l15;
+        a[i].u = (u32x4){0, 0, 0, 0};
+        if (left > 0) a[i] = gload16(ap + (int64_t)(r < ra ? r : ra) * p.lda + k);
+      }
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const unsigned r = wn0 + 16 * j + l15;
+        w[j].u = (u32x4){0, 0, 0, 0};
+        if (left > 0) w[j] = gload16(wp + (int64_t)(r < rw ? r : rw) * p.ldw + k);
+        keep_bytes(w[j], left);
+      }
+      static_for<FN>([&](auto jc) {
+        settle(w[decltype(jc)::value]);
+        static_for<FM>([&](auto ic) {
+          constexpr int i = decltype(ic)::value, j = decltype(jc)::value;
+          if constexpr (j < 8 || G::tall) agpr_mfma<G::agpr(i, j)>(w[j], a[i]);
+          else vgpr_mfma(c8[i], w[j], a[i]);
+        });
+      });
+    }
+    asm volatile("s_nop 15\n\ts_nop 7");  // and the accumulators are read next
+  }
+  int8_epilogue<T, BM, BN, FM, FN, 256, EPI>(p, smem, m0, n0, wm0, wn0, [&](auto ic, auto jc) -> i32x4 {
+    constexpr int i = decltype(ic)::value, j = decltype(jc)::value;
+    if constexpr (j < 8 || G::tall) return agpr_read<G::agpr(i, j)>();
+    else return c8[i];
+  });
 }
 
 // Few rows (M <= 16 FM): the time is the reading of W.  A workgroup owns 16 columns; its waves take turns along K in steps of 64 bytes per row, operands go
 // straight to registers in the matrix instruction's layout (each W byte is used by one wave only: nothing to share through LDS), several steps in flight; the waves'
 // sums meet in LDS.
-template <typename T, int FM, int NW>
+template <typename T, int FM, int NW, int EPI>
 __global__ __launch_bounds__(NW * 64) void gemm_int8_rows_kernel(const Int8GemmArgs p) {
   __shared__ int part[NW][FM * 256];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
@@ -310,10 +412,10 @@ __global__ __launch_bounds__(NW * 64) void gemm_int8_rows_kernel(const Int8GemmA
     int sum = part[0][it];
 #pragma unroll
     for (int w = 1; w < NW; ++w) sum += part[w][it];
-    const float o = int8_act(__builtin_fmaf((float)sum, p.sa[m] * p.sw[n], p.bias ? p.bias[n] : 0.f), p.epi);
+    const float o = int8_act<EPI>(__builtin_fmaf((float)sum, p.sa[m] * p.sw[n], p.bias ? p.bias[n] : 0.f));
     const float rounded = round_elem<T>(o);
-    if (p.out) reinterpret_cast<T*>(p.out)[(int64_t)m * p.ldo + n] = (T)o;
-    if (p.epi == I8_RESID) {
+    if (EPI != I8_RESID || p.out) reinterpret_cast<T*>(p.out)[(int64_t)m * p.ldo + n] = (T)o;
+    if constexpr (EPI == I8_RESID) {
       float gate = p.gate_table ? p.gate_table[n] : (p.gate_mod ? 0.f : 1.f);
       if (p.gate_mod) gate += (float)reinterpret_cast<const T*>(p.gate_mod)[(int64_t)(m / p.rows_per_batch) * p.gate_stride + n];
       reinterpret_cast<T*>(p.resid_out)[(int64_t)m * p.ldro + n] = (T)pinned(__builtin_fmaf(gate, rounded, (float)reinterpret_cast<const T*>(p.resid)[(int64_t)m * p.ldr + n]));

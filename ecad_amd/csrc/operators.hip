@@ -132,64 +132,99 @@ template <typename T> int quantize_t(const OpCtx& ctx, const QuantizeArgs& a, Op
 
 // ---- norms ---------------------------------------------------------------------------------------------------------------------------------------------------
 
+template <typename T, int WAVES, int CH, bool HOLD = true> int launch_norm(const OpCtx& ctx, GateNormArgs& a, int per_cu, OpStatus& st) {
+  // Rows in turn: a lane keeps the channel vectors and has the next row's loads in flight while it works on one.  per_cu: rows that a CU works on at a time (what its
+  // registers hold: 97 / 147 / 209 of 512 per lane at one / two / three pieces); every wave gets at least one row.
+  const int slots = row_slots(WAVES);
+  const int64_t at_once = (int64_t)ctx.num_cus * per_cu;
+  a.rows_per_group = (int)((a.M + at_once - 1) / at_once);
+  const dim3 grid((unsigned)(((int64_t)a.M + (int64_t)slots * a.rows_per_group - 1) / ((int64_t)slots * a.rows_per_group))), block(WAVES > 4 ? WAVES * 64 : 256);
+  if (a.D % 8) hipLaunchKernelGGL((gate_norm_kernel<T, WAVES, CH, true, HOLD>), grid, block, 0, ctx.stream, a);
+  else hipLaunchKernelGGL((gate_norm_kernel<T, WAVES, CH, false, HOLD>), grid, block, 0, ctx.stream, a);
+  return launched(st, "gate_norm");
+}
 template <typename T> int gate_norm_t(const OpCtx& ctx, GateNormArgs& a, OpStatus& st) {
   const int pieces = (a.D + 7) / 8;
-  // rows a wave (or a workgroup of a wide row) takes: enough to reuse the channel vectors, few enough to leave work for the whole chip
-  auto group = [&](int slots) {
-    int r = 1;
-    while (r < 16 && (int64_t)a.M >= (int64_t)2 * r * slots * 8 * ctx.num_cus) r *= 2;
-    a.rows_per_group = r;
-    return dim3((unsigned)((a.M + (int64_t)slots * r - 1) / ((int64_t)slots * r)));
-  };
-#define ECAD_NORM(WAVES, CH) hipLaunchKernelGGL((gate_norm_kernel<T, WAVES, CH>), group(row_slots(WAVES)), dim3(WAVES > 4 ? WAVES * 64 : 256), 0, ctx.stream, a)
-  if (pieces <= 64) ECAD_NORM(1, 1);
-  else if (pieces <= 128) ECAD_NORM(1, 2);
-  else if (pieces <= 192) ECAD_NORM(1, 3);
-  else if (pieces <= 256) ECAD_NORM(4, 1);
-  else if (pieces <= 512) ECAD_NORM(4, 2);
-  else if (pieces <= 1024) ECAD_NORM(4, 4);
-  else if (pieces <= 2048) ECAD_NORM(16, 2);
-  else ECAD_NORM(16, 4);
-#undef ECAD_NORM
-  return launched(st, "gate_norm");
+  if (pieces <= 64) return launch_norm<T, 1, 1>(ctx, a, 20, st);
+  if (pieces <= 128) return launch_norm<T, 1, 2>(ctx, a, 12, st);
+  if (pieces <= 192) return launch_norm<T, 1, 3>(ctx, a, 8, st);
+  if (pieces <= 256) return launch_norm<T, 4, 1>(ctx, a, 5, st);
+  if (pieces <= 512) return launch_norm<T, 4, 2>(ctx, a, 3, st);
+  if (pieces <= 1024) return launch_norm<T, 8, 2>(ctx, a, 1, st);
+  if (pieces <= 2048) return launch_norm<T, 16, 2, false>(ctx, a, 1, st);
+  return launch_norm<T, 16, 4, false>(ctx, a, 1, st);
 }
 
 // ---- products ------------------------------------------------------------------------------------------------------------------------------------------------
 
-template <typename T, int BM, int BN, int WM, int WN, int STAGES> int launch_tile(const OpCtx& ctx, const Int8GemmArgs& a, OpStatus& st) {
-  static std::atomic<uint64_t> done{0};
-  constexpr int bytes = STAGES * (BM + BN) * 128;
-  const int rc = allow_lds(done, (const void*)gemm_int8_kernel<T, BM, BN, WM, WN, STAGES>, bytes, st);
+int64_t tiles_of(const Int8GemmArgs& a, int bm, int bn) { return ((int64_t)a.M + bm - 1) / bm * (((int64_t)a.N + bn - 1) / bn); }
+
+int launch_int8(const OpCtx& ctx, const Int8GemmArgs& a, OpStatus& st, std::atomic<uint64_t>& done, void (*kernel)(const Int8GemmArgs), int bm, int bn, int threads, int bytes) {
+  const int rc = allow_lds(done, (const void*)kernel, bytes, st);
   if (rc) return rc;
-  const int64_t tiles = ((int64_t)a.M + BM - 1) / BM * (((int64_t)a.N + BN - 1) / BN);
+  const int64_t tiles = tiles_of(a, bm, bn);
   if (tiles > 0x7fffffff) return refuse(st, ECAD_E_UNSUPPORTED, "gemm_int8: %lld tiles are more than one launch takes", (long long)tiles);
-  hipLaunchKernelGGL((gemm_int8_kernel<T, BM, BN, WM, WN, STAGES>), dim3((unsigned)tiles), dim3(WM * WN * 64), bytes, ctx.stream, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(threads), bytes, ctx.stream, a);
   return launched(st, "gemm_int8");
 }
+template <typename T, int EPI, int BM, int BN, int WM, int WN, int STAGES> int launch_tile(const OpCtx& ctx, const Int8GemmArgs& a, OpStatus& st) {
+  static std::atomic<uint64_t> done{0};
+  return launch_int8(ctx, a, st, done, gemm_int8_kernel<T, BM, BN, WM, WN, STAGES, EPI>, BM, BN, WM * WN * 64, int8_lds_bytes(BM, BN, STAGES));
+}
+template <typename T, int EPI, int BN> int launch_wide(const OpCtx& ctx, const Int8GemmArgs& a, OpStatus& st) {
+  static std::atomic<uint64_t> done{0};
+  if (a.K / 128 < Int8Wide<BN>::fewest) return refuse(st, ECAD_E_UNSUPPORTED, "gemm_int8: the 256 x %d kernel needs K of at least %d, got %d", BN, Int8Wide<BN>::fewest * 128, a.K);
+  return launch_int8(ctx, a, st, done, gemm_int8_wide_kernel<T, BN, EPI>, 256, BN, 256, int8_lds_bytes(256, BN, Int8Wide<BN>::stages));
+}
 
-template <typename T> int gemm_int8_t(const OpCtx& ctx, const Int8GemmArgs& a, int kernel, OpStatus& st) {
-  if (kernel == ECAD_I8_K_ROWS && a.M > 64) return refuse(st, ECAD_E_UNSUPPORTED, "gemm_int8: the few-rows kernel takes up to 64 rows, got %d", a.M);
-  if (kernel == ECAD_I8_K_AUTO) {
-    auto tiles = [&](int bm, int bn) { return ((int64_t)a.M + bm - 1) / bm * (((int64_t)a.N + bn - 1) / bn); };
-    if (a.M <= 64) kernel = ECAD_I8_K_ROWS;
-    else if (tiles(256, 256) >= ctx.num_cus) kernel = ECAD_I8_K_TILE256;
-    else if (tiles(128, 128) >= ctx.num_cus) kernel = ECAD_I8_K_TILE128;
-    else kernel = ECAD_I8_K_TILE64;
+// Which kernel: the one with the smallest estimated time, rounds of the tiles it needs over the chip times (what a round costs outside the K loop + its K stages), in
+// microseconds as measured with all CUs busy (fp16 / bf16 out, plain epilogue).  Against the measured times of 8192 x 4608 x 1152, 8192 x 1152 x 4608, 4096 x 3456 x 1152,
+// 2048 x 4608 x 1152, 1024 x 1152 x 1152, 601 x 1111 x 4001 and 8192 x 8192 x 4096 the estimate picks the fastest kernel each time (estimates within 25 %); e.g. 8192 x 4608 x
+// 1152: 288 columns (two whole rounds) 62 us, 256 columns (2.25 rounds) 73, 144 columns 74, 128 x 128 77, 64 x 64 122.
+int choose_int8(const OpCtx& ctx, const Int8GemmArgs& a) {
+  struct Tile {
+    int id, bm, bn, per_cu, fewest;
+    double fixed, stage;
+  };
+  static const Tile tiles[] = {{ECAD_I8_K_TILE64, 64, 64, 2, 0, 2.8, 0.44},      {ECAD_I8_K_TILE128, 128, 128, 2, 0, 5.0, 1.2}, {ECAD_I8_K_TILE144, 256, 144, 1, Int8Wide<144>::fewest, 7.0, 1.0},
+                               {ECAD_I8_K_TILE256, 256, 256, 1, Int8Wide<256>::fewest, 6.6, 1.6}, {ECAD_I8_K_TILE288, 256, 288, 1, Int8Wide<288>::fewest, 8.0, 1.72}};
+  if (a.M <= 32) return ECAD_I8_K_ROWS;
+  const int stages = (a.K + 127) / 128;
+  int best = ECAD_I8_K_TILE64;
+  double least = 1e300;
+  for (const Tile& t : tiles) {
+    if (a.K / 128 < t.fewest) continue;
+    const int64_t at_once = (int64_t)t.per_cu * ctx.num_cus;
+    const double us = (double)((tiles_of(a, t.bm, t.bn) + at_once - 1) / at_once) * (t.fixed + t.stage * stages);
+    if (us < least) least = us, best = t.id;
   }
-  switch (kernel) {
+  return best;
+}
+
+template <typename T, int EPI> int gemm_int8_t(const OpCtx& ctx, const Int8GemmArgs& a, int kernel, OpStatus& st) {
+  if (kernel == ECAD_I8_K_ROWS && a.M > 64) return refuse(st, ECAD_E_UNSUPPORTED, "gemm_int8: the few-rows kernel takes up to 64 rows, got %d", a.M);
+  switch (kernel == ECAD_I8_K_AUTO ? choose_int8(ctx, a) : kernel) {
     case ECAD_I8_K_ROWS: {
       const dim3 grid((unsigned)((a.N + 15) / 16));
-      if (a.M <= 16) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 1, 8>), grid, dim3(512), 0, ctx.stream, a);
-      else if (a.M <= 32) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 2, 8>), grid, dim3(512), 0, ctx.stream, a);
-      else hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 4, 8>), grid, dim3(512), 0, ctx.stream, a);
+      if (a.M <= 16) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 1, 8, EPI>), grid, dim3(512), 0, ctx.stream, a);
+      else if (a.M <= 32) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 2, 8, EPI>), grid, dim3(512), 0, ctx.stream, a);
+      else hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 4, 8, EPI>), grid, dim3(512), 0, ctx.stream, a);
       return launched(st, "gemm_int8");
     }
-    case ECAD_I8_K_TILE64: return launch_tile<T, 64, 64, 2, 2, 4>(ctx, a, st);
-    case ECAD_I8_K_TILE128: return launch_tile<T, 128, 128, 2, 2, 2>(ctx, a, st);
-    case ECAD_I8_K_TILE144: return launch_tile<T, 256, 144, 8, 1, 3>(ctx, a, st);
-    case ECAD_I8_K_TILE256: return launch_tile<T, 256, 256, 4, 2, 2>(ctx, a, st);
-    case ECAD_I8_K_TILE288: return launch_tile<T, 256, 288, 4, 2, 2>(ctx, a, st);
+    case ECAD_I8_K_TILE64: return launch_tile<T, EPI, 64, 64, 2, 2, 4>(ctx, a, st);
+    case ECAD_I8_K_TILE128: return launch_tile<T, EPI, 128, 128, 2, 2, 2>(ctx, a, st);
+    case ECAD_I8_K_TILE144: return launch_wide<T, EPI, 144>(ctx, a, st);
+    case ECAD_I8_K_TILE256: return launch_wide<T, EPI, 256>(ctx, a, st);
+    case ECAD_I8_K_TILE288: return launch_wide<T, EPI, 288>(ctx, a, st);
     default: return refuse(st, ECAD_E_INVALID, "gemm_int8: kernel %d unknown", kernel);
+  }
+}
+template <typename T> int gemm_int8_epi(const OpCtx& ctx, const Int8GemmArgs& a, int epi, int kernel, OpStatus& st) {
+  switch (epi) {
+    case I8_GELU: return gemm_int8_t<T, I8_GELU>(ctx, a, kernel, st);
+    case I8_SILU: return gemm_int8_t<T, I8_SILU>(ctx, a, kernel, st);
+    case I8_RESID: return gemm_int8_t<T, I8_RESID>(ctx, a, kernel, st);
+    default: return gemm_int8_t<T, I8_BIAS>(ctx, a, kernel, st);
   }
 }
 
@@ -240,8 +275,8 @@ int op_gemm_int8(const OpCtx& ctx, const EcadInt8Gemm& c, OpStatus& st) noexcept
   Int8GemmArgs a{};
   a.A = c.A; a.W = c.W; a.sa = c.a_scale; a.sw = c.w_scale; a.bias = c.bias; a.out = c.out; a.resid = c.resid; a.resid_out = c.resid_out; a.gate_table = c.gate_table; a.gate_mod = c.gate_mod;
   a.lda = c.lda; a.ldw = c.ldw; a.ldo = c.ldo; a.ldr = c.ldr; a.ldro = c.ldro; a.gate_stride = c.gate_mod_stride;
-  a.M = c.M; a.N = c.N; a.K = c.K; a.epi = c.epi; a.rows_per_batch = c.rows_per_batch > 0 ? c.rows_per_batch : 1;
-  return ctx.dtype == ECAD_DTYPE_F16 ? gemm_int8_t<f16_t>(ctx, a, c.kernel, st) : gemm_int8_t<bf16_t>(ctx, a, c.kernel, st);
+  a.M = c.M; a.N = c.N; a.K = c.K; a.rows_per_batch = c.rows_per_batch > 0 ? c.rows_per_batch : 1;
+  return ctx.dtype == ECAD_DTYPE_F16 ? gemm_int8_epi<f16_t>(ctx, a, c.epi, c.kernel, st) : gemm_int8_epi<bf16_t>(ctx, a, c.epi, c.kernel, st);
 }
 
 int op_gate_norm(const OpCtx& ctx, const EcadGateNorm& c, OpStatus& st) noexcept {

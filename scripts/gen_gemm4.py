@@ -320,6 +320,7 @@ class Gen:
                     I(f"v_xor_b32_e32 {v(T + 6)}, {v(T + 6)}, {v(T + 5)}")
                     I(f"v_lshlrev_b32_e32 {v(T + 6)}, 4, {v(T + 6)}")
                     I(f"v_add_u32_e32 {v(T + 7)}, {s('tmp0')}, {v(T + 4)}")
+                    self.clamp_row(which, T + 7)
                     I(f"v_mad_u32_u24 {v(off + q)}, {v(T + 7)}, {rs}, {v(T + 6)}")
                 continue
             I(f"s_mul_i32 {s('tmp0')}, %[wave], {8 * n}")            # first row of this wave's pieces
@@ -333,6 +334,7 @@ class Gen:
                 I(f"v_lshlrev_b32_e32 {v(T + 6)}, 4, {v(T + 6)}")
                 I(f"v_add_u32_e32 {v(T + 7)}, {8 * q}, {v(T + 4)}")
                 I(f"v_add_u32_e32 {v(T + 7)}, {s('tmp0')}, {v(T + 7)}")
+                self.clamp_row(which, T + 7)
                 I(f"v_mad_u32_u24 {v(off + q)}, {v(T + 7)}, {rs}, {v(T + 6)}")
         I(f"s_lshl_b32 {s('tmp0')}, %[wave], 13")                   # this wave's 8 A pieces
         I(f"s_add_u32 {s('ldsw')}, %[lds], {s('tmp0')}")
@@ -359,7 +361,7 @@ class Gen:
         if self.stage and not self.narrow:
             for r in range(32):
                 I(f"v_mov_b32_e32 {v(self.C8 + r)}, 0")
-        if self.narrow:
+        if self.narrow and self.stage:
             # residual chunks of this lane (resid_prefetch): byte offsets from %[rbase] = &h[m0 + 64 wave][n0]
             I(f"v_lshrrev_b32_e32 {v(T + 6)}, 4, {v(T)}")                        # lane >> 4
             I(f"v_and_b32_e32 {v(T + 7)}, 15, {v(T)}")                           # lane & 15
@@ -418,15 +420,7 @@ class Gen:
         I(f"s_cmp_eq_u32 {s('loop')}, 0")
         I(f"s_cbranch_scc0 {self.lbl('LOOP')}")
         self.L("LAST")
-        for k in range(self.period):
-            left = self.period - 1 - k           # stages after this one
-            if self.narrow and self.stage and left == 1:
-                # the second-to-last stage has no DMA left to issue: the NRES residual loads of the read-modify-write epilogue go out here, behind every operand piece,
-                # so this stage's counted wait lets exactly them stay in flight (vmcnt retires in order) -- an HBM round trip that travels under two stages of MFMAs
-                # and the C-tile staging instead of in front of the row pass (gemm3s.h issues its residual loads in the same place)
-                emit(k, False, self.NRES, False, self.resid_prefetch())
-                continue
-            emit(k, left >= NS - 1, vm if left >= NS - 1 else 0, left == 0)
+        self.last_trip(emit, vm)
         I("s_nop 15")
         I("s_barrier")   # every wave is done with the ring: the epilogue's C tile may overwrite it
         if self.stage:
@@ -437,6 +431,22 @@ class Gen:
                 self.stage_c()
         I(f"s_mov_b32 m0, {s('m0save')}")
         return self.lines
+
+    # what gen_gemm_i8.py's loops do differently
+    def clamp_row(self, which, reg):
+        """rows of the tile that do not exist: nothing here, the tiles are whole"""
+
+    def last_trip(self, emit, vm):
+        NS = self.NS
+        for k in range(self.period):
+            left = self.period - 1 - k           # stages after this one
+            if self.narrow and self.stage and left == 1:
+                # the second-to-last stage has no DMA left to issue: the NRES residual loads of the read-modify-write epilogue go out here, behind every operand piece,
+                # so this stage's counted wait lets exactly them stay in flight (vmcnt retires in order) -- an HBM round trip that travels under two stages of MFMAs
+                # and the C-tile staging instead of in front of the row pass (gemm3s.h issues its residual loads in the same place)
+                emit(k, False, self.NRES, False, self.resid_prefetch())
+                continue
+            emit(k, left >= NS - 1, vm if left >= NS - 1 else 0, left == 0)
 
     NRES = 18
 

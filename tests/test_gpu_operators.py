@@ -112,6 +112,11 @@ SHAPES = [(1, 1, 1), (1, 17, 16), (2, 6912, 1152), (16, 100, 63), (17, 33, 65), 
           (300, 144, 1152), (512, 1152, 4096), (601, 577, 130), (1000, 4608, 1152)]
 
 
+def takes(kernel, M, K):
+    """What the named kernels refuse."""
+    return not (kernel == "rows" and M > 64 or kernel in ("tile256", "tile288") and K < 256 or kernel == "tile144" and K < 384)
+
+
 def product64(a, sa, w, sw, bias):
     acc = a.double() @ w.double().t()  # whole numbers below 2^31: exact
     scaled = acc * sa.double()[:, None] * sw.double()
@@ -133,7 +138,7 @@ def test_gemm_every_kernel_and_epilogue(dtype_name, M, N, K):
         pre, size = product64(a, sa, w, sw, bias if epi != 2 else None)
         first = None
         for kernel in eng.INT8_KERNELS:
-            if kernel == "rows" and M > 64:
+            if not takes(kernel, M, K):
                 continue
             out = eng.op_gemm_int8(epi, a, sa, w, sw, bias if epi != 2 else None, kernel=kernel)
             if first is None:
@@ -162,7 +167,7 @@ def test_gemm_gated_residual(dtype_name, M, N, K, gate):
     base = rand(M, N + 5, seed=9, dtype=dt)
     kept = None
     for kernel in eng.INT8_KERNELS:
-        if kernel == "rows" and M > 64:
+        if not takes(kernel, M, K):
             continue
         wide = base.clone()
         out = torch.empty(M, N, device="cuda", dtype=dt)
