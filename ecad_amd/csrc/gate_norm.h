@@ -14,6 +14,9 @@ namespace ecad {
 
 enum NormKind { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };
 
+// Rows a workgroup works on at a time: four where a row is one wave's, else one (waves of a row meet at barriers, and rows end at different turns).
+constexpr int row_slots(int waves) { return waves == 1 ? 4 : 1; }
+
 struct GateNormArgs {
   const void* h;
   const void* y;
@@ -58,13 +61,6 @@ ECAD_DEV void row_statistics(const float (&x)[CH][8], int kind, int first, int D
   rstd = 1.0f / sqrtf(row_all<WAVES>(sq, AddOp{}, scratch, turn) * inv_d + eps);
 }
 
-template <typename T, bool RAGGED> ECAD_DEV Pack8 row_piece(const T* p, int left) {
-  if constexpr (RAGGED) return load_piece<T>(p, left);
-  Pack8 v;
-  v.u = (u32x4){0, 0, 0, 0};
-  if (left > 0) v.u = reinterpret_cast<const Bytes16*>(p)->u;
-  return v;
-}
 template <typename T, bool RAGGED> ECAD_DEV void row_store(T* p, const Pack8& v, int left) {
   if constexpr (RAGGED) store_piece<T>(p, v, left);
   else if (left > 0) reinterpret_cast<Bytes16*>(p)->u = v.u;
@@ -75,12 +71,11 @@ template <typename T, bool RAGGED> ECAD_DEV void row_store(T* p, const Pack8& v,
 // 26 bytes per element out of L2 against the 8 that the rows themselves move.  They are zero beyond the row, and with them everything that is computed there.
 // HOLD false (rows of more than 8192 values on 16 waves, whose lanes have 128 registers): read anew all the same.
 template <typename T, int WAVES, int CH, bool RAGGED, bool HOLD>
-__global__ __launch_bounds__(WAVES > 4 ? WAVES * 64 : 256) void gate_norm_kernel(const GateNormArgs p) {
-  constexpr int SLOTS = WAVES >= 4 ? 1 : 4 / WAVES;  // rows a workgroup works on at a time
-  __shared__ unsigned scratch_all[SLOTS][2][WAVES];
-  const int slot = WAVES >= 4 ? 0 : __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) / WAVES);
-  unsigned(*scratch)[WAVES] = scratch_all[slot];
-  const int lane = WAVES >= 4 ? threadIdx.x : (threadIdx.x & (64 * WAVES - 1));
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void gate_norm_kernel(const GateNormArgs p) {
+  constexpr int SLOTS = row_slots(WAVES);
+  __shared__ unsigned scratch[2][WAVES];  // (one wave a row: not used)
+  const int slot = WAVES == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+  const int lane = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
   const int first = lane * 8;
   int turn = 0;
   float G[HOLD ? CH : 1][8], A[HOLD ? CH : 1][8], B[HOLD ? CH : 1][8];
@@ -95,51 +90,61 @@ __global__ __launch_bounds__(WAVES > 4 ? WAVES * 64 : 256) void gate_norm_kernel
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int c = first + i * WAVES * 512;
-      hv[i] = row_piece<T, RAGGED>(hrow + c, p.D - c);
-      if (p.y) yv[i] = row_piece<T, RAGGED>(yrow + c, p.D - c);
+      hv[i] = row_load<T, RAGGED>(hrow, c, p.D);
+      if (p.y) yv[i] = row_load<T, RAGGED>(yrow, c, p.D);
     }
   };
   if (row0 < end) fetch(row0);
   for (int64_t row = row0; row < end; ++row) {
     const int b = (int)((unsigned)row / (unsigned)p.rows_per_batch);
-    // the vectors of piece i: the gate's (what & 1) or scale and shift (what & 2)
+    // the vectors of piece i: the gate's (what & 1) or scale and shift (what & 2).  All loads first: each is behind a branch on its pointer, and combined one by one
+    // they would wait for each other (eight round trips to memory in front of the first row: 5 of the 8.5 us of a call with five rows)
     auto channels = [&](int i, int at, int what) {
       const int c = first + i * WAVES * 512, n = p.D - c;
-      float f[8];
-      auto table = [&](const float* v, auto&& put) {
+      float gt[8], pw[8], st[8], ew[8], ht[8];
+      Pack8 gm, sm, hm;
+      auto table = [&](const float* v, float (&f)[8]) {
         if (!v) return;
-        load_floats(v + c, n, f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) put(e);
+        if constexpr (RAGGED) {
+          load_floats(v + c, n, f);
+        } else if (n > 0) {
+          load_floats(v + c, 8, f);
+        }
       };
-      auto mod = [&](const void* base, int64_t stride, auto&& put) {
-        if (!base) return;
-        unpack8<T>(load_piece<T>(reinterpret_cast<const T*>(base) + (int64_t)b * stride + c, n), f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) put(e);
+      auto mod = [&](const void* base, int64_t stride, Pack8& f) {
+        if (base) f = row_load<T, RAGGED>(reinterpret_cast<const T*>(base) + (int64_t)b * stride, c, p.D);
       };
+      if (what & 1) table(p.gate_table, gt), mod(p.gate_mod, p.gate_stride, gm), table(p.post_weight, pw);
+      if (what & 2) table(p.table_scale, st), mod(p.mod_scale, p.mod_stride, sm), table(p.pre_weight, ew), table(p.table_shift, ht), mod(p.mod_shift, p.mod_stride, hm);
+      float f[8];
       if (what & 1) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) G[at][e] = p.gate_table || p.gate_mod ? 0.f : 1.f;
-        table(p.gate_table, [&](int e) { G[at][e] = f[e]; });
-        mod(p.gate_mod, p.gate_stride, [&](int e) { G[at][e] += f[e]; });
-        table(p.post_weight, [&](int e) { G[at][e] *= f[e]; });
+        for (int e = 0; e < 8; ++e) G[at][e] = p.gate_table ? gt[e] : (p.gate_mod ? 0.f : 1.f);
+        unpack8<T>(row_piece<RAGGED>(gm, c, p.D), f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (p.gate_mod) G[at][e] += f[e];
+          if (p.post_weight) G[at][e] *= pw[e];
+          if (e >= n) G[at][e] = 0.f;
+        }
       }
       if (what & 2) {
+        unpack8<T>(row_piece<RAGGED>(sm, c, p.D), f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) A[at][e] = 1.f, B[at][e] = 0.f;
-        table(p.table_scale, [&](int e) { A[at][e] += f[e]; });
-        mod(p.mod_scale, p.mod_stride, [&](int e) { A[at][e] += f[e]; });
-        table(p.pre_weight, [&](int e) { A[at][e] *= f[e]; });
-        table(p.table_shift, [&](int e) { B[at][e] = f[e]; });
-        mod(p.mod_shift, p.mod_stride, [&](int e) { B[at][e] += f[e]; });
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e >= n) {
-          if (what & 1) G[at][e] = 0.f;
-          if (what & 2) A[at][e] = B[at][e] = 0.f;
+        for (int e = 0; e < 8; ++e) {
+          A[at][e] = p.table_scale ? 1.f + st[e] : 1.f;
+          if (p.mod_scale) A[at][e] += f[e];
+          if (p.pre_weight) A[at][e] *= ew[e];
+          if (e >= n) A[at][e] = 0.f;
         }
+        unpack8<T>(row_piece<RAGGED>(hm, c, p.D), f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          B[at][e] = p.table_shift ? ht[e] : 0.f;
+          if (p.mod_shift) B[at][e] += f[e];
+          if (e >= n) B[at][e] = 0.f;
+        }
+      }
     };
     if (HOLD && b != have) {
       have = b;
@@ -148,11 +153,11 @@ __global__ __launch_bounds__(WAVES > 4 ? WAVES * 64 : 256) void gate_norm_kernel
     }
     float x[CH][8];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) unpack8<T>(hv[i], x[i]);
+    for (int i = 0; i < CH; ++i) unpack8<T>(row_piece<RAGGED>(hv[i], first + i * WAVES * 512, p.D), x[i]);
     if (p.y) {
       float u[CH][8], mean = 0.f, rstd = 1.f;
 #pragma unroll
-      for (int i = 0; i < CH; ++i) unpack8<T>(yv[i], u[i]);
+      for (int i = 0; i < CH; ++i) unpack8<T>(row_piece<RAGGED>(yv[i], first + i * WAVES * 512, p.D), u[i]);
       if (row + 1 < end) fetch(row + 1);
       if (p.post) row_statistics<WAVES, CH, RAGGED>(u, p.post, first, p.D, p.eps, scratch, turn, mean, rstd);
       T* ho = reinterpret_cast<T*>(p.h_out) + row * p.ldho;
@@ -212,29 +217,27 @@ struct QuantizeArgs {
 };
 
 // One row per WAVES waves, the whole row in registers between the maximum and the rounding: read once.
-template <typename T, int WAVES, int CH>
-__global__ __launch_bounds__(WAVES > 4 ? WAVES * 64 : 256) void quantize_rows_kernel(const QuantizeArgs p) {
-  constexpr int SLOTS = WAVES >= 4 ? 1 : 4 / WAVES;
-  __shared__ unsigned scratch_all[SLOTS][2][WAVES];
-  const int slot = WAVES >= 4 ? 0 : (threadIdx.x >> 6) / WAVES;
-  const int lane = WAVES >= 4 ? threadIdx.x : (threadIdx.x & (64 * WAVES - 1));
-  const int64_t row_ = (int64_t)blockIdx.x * SLOTS + slot;
-  const bool live = row_ < p.M;
-  const int64_t row = live ? row_ : p.M - 1;
+template <typename T, int WAVES, int CH, bool RAGGED>
+__global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void quantize_rows_kernel(const QuantizeArgs p) {
+  __shared__ unsigned scratch[2][WAVES];
+  const int lane = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
+  const int64_t row = (int64_t)blockIdx.x * row_slots(WAVES) + (WAVES == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+  if (row >= p.M) return;  // whole workgroups, or waves that share nothing
   const T* xrow = reinterpret_cast<const T*>(p.x) + row * p.ldx;
   int turn = 0;
   Pack8 v[CH];
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
-    const int c = (lane + i * WAVES * 64) * 8;
-    v[i] = load_piece<T>(xrow + c, p.K - c);
+    v[i] = row_load<T, RAGGED>(xrow, (lane + i * WAVES * 64) * 8, p.K);
   }
   u16x2 m = {0, 0};
 #pragma unroll
-  for (int i = 0; i < CH; ++i) m = max_bits(m, v[i]);
-  const unsigned bits = row_all<WAVES>(fold_bits(m), MaxOp{}, scratch_all[slot], turn);
+  for (int i = 0; i < CH; ++i) {
+    v[i] = row_piece<RAGGED>(v[i], (lane + i * WAVES * 64) * 8, p.K);
+    m = max_bits(m, v[i]);
+  }
+  const unsigned bits = row_all<WAVES>(fold_bits(m), MaxOp{}, scratch, turn);
   const Int8Scale k = int8_scale<T>(bits);
-  if (!live) return;
   if (lane == 0) p.scale[row] = k.s;
 #pragma unroll
   for (int i = 0; i < CH; ++i) {

@@ -79,13 +79,14 @@ template <int EPI> ECAD_DEV float int8_act(float v) {
 
 // Epilogue of a tile from its accumulators: lane (l15, g) of a wave holds row m = 16 i + l15, columns 16 j + 4 g .. + 3 of fragment (i, j) of the wave's block at
 // (wm0, wn0) of the tile.
+// holds: this wave has sums (the others of a tile that is split along K help to write it out).
 //   Whole tiles of 16-byte rows without a residual leave straight from the registers: two neighbouring fragments swap halves between lane rows, so a lane ends with
 //   eight consecutive columns -- one 16-byte store per pair, 64 contiguous bytes of each of 16 rows -- and LDS stays free.
 //   Everything else goes through a row-major tile in LDS (the ring is done with) and leaves in a rolled loop of 16-byte pieces of rows: the residual's reads are
 //   contiguous, and edges need one piece of code instead of one per fragment.  (The accumulators can only be named by constants, so whatever stands beside them is
 //   unrolled 64 times: with the edges in there the kernel was 250 KB of code and spent 30 us of a 37 us one-round launch fetching it.)
 template <typename T, int BM, int BN, int FM, int FN, int NT, int EPI, typename AccFn>
-ECAD_DEV void int8_epilogue(const Int8GemmArgs& p, char* smem, int m0, int n0, int wm0, int wn0, AccFn&& acc) {
+ECAD_DEV void int8_epilogue(const Int8GemmArgs& p, char* smem, int m0, int n0, int wm0, int wn0, bool holds, AccFn&& acc) {
   constexpr int CS = BN + 8;  // row stride of the tile in LDS: 16-byte rows, four banks apart
   const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
   const bool direct = EPI != I8_RESID && m0 + BM <= p.M && n0 + BN <= p.N && p.ldo % 8 == 0 && ((uintptr_t)p.out & 15) == 0;
@@ -111,6 +112,7 @@ ECAD_DEV void int8_epilogue(const Int8GemmArgs& p, char* smem, int m0, int n0, i
     return (u32x2){pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3])};
   };
   if (direct) {
+    if (!holds) return;
     T* row = reinterpret_cast<T*>(p.out) + (int64_t)(m0 + wm0 + l15) * p.ldo + n0 + wn0;
     static_for<(FN + 1) / 2>([&](auto jh) {
       constexpr int j = 2 * decltype(jh)::value, j1 = j + 1 < FN ? j + 1 : j;
@@ -135,7 +137,7 @@ ECAD_DEV void int8_epilogue(const Int8GemmArgs& p, char* smem, int m0, int n0, i
     return;
   }
   T* tile = reinterpret_cast<T*>(smem);
-  static_for<FN>([&](auto jc) {
+  if (holds) static_for<FN>([&](auto jc) {
     constexpr int j = decltype(jc)::value;
     const int n = n0 + wn0 + 16 * j + 4 * g;
     const f32x4 sw = columns(p.sw, n), bias = p.bias ? columns(p.bias, n) : (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -175,17 +177,19 @@ constexpr int int8_lds_bytes(int bm, int bn, int stages) {
   return ring > tile ? ring : tile;
 }
 
-// BM x BN tile on WM x WN waves.  A K-step is 128 bytes of every row of the tile: pieces of eight rows (1 KiB) travel straight to LDS, 16-byte chunks
-// XOR-swizzled by (row >> 1) & 7 on the source side, so that the fragment reads (16 rows x 16 bytes) meet every bank once.  One barrier per step, STAGES steps in a ring.
-template <typename T, int BM, int BN, int WM, int WN, int STAGES, int EPI>
-__global__ __launch_bounds__(WM * WN * 64) void gemm_int8_kernel(const Int8GemmArgs p) {
-  constexpr int NW = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
-  constexpr int A_BYTES = BM * 128, STAGE_BYTES = (BM + BN) * 128;
-  constexpr int PIECES = (BM + BN) / 8, PPW = (PIECES + NW - 1) / NW;  // not a multiple of the waves: the last ones fetch the first pieces again (same bytes, same place)
+// BM x BN tile on WM x WN waves, KW such groups along K.  A step is 128 bytes of K per row for every group: pieces of eight rows (1 KiB) travel straight to LDS, 16-byte
+// chunks XOR-swizzled by (row >> 1) & 7 on the source side, so that the fragment reads (16 rows x 16 bytes) meet every bank once.  One barrier per step, STAGES steps in
+// a ring.  KW > 1 is for products of few tiles, whose time is the number of steps: the groups' sums meet in LDS (whole numbers: the same bits).
+template <typename T, int BM, int BN, int WM, int WN, int KW, int STAGES, int EPI>
+__global__ __launch_bounds__(WM * WN * KW * 64) void gemm_int8_kernel(const Int8GemmArgs p) {
+  constexpr int NG = WM * WN, NW = NG * KW, FM = BM / WM / 16, FN = BN / WN / 16;
+  constexpr int A_BYTES = BM * 128, GROUP_BYTES = (BM + BN) * 128, STAGE_BYTES = KW * GROUP_BYTES;
+  constexpr int PPG = (BM + BN) / 8, PPW = KW * PPG / NW;  // pieces per group and step, per wave
+  static_assert(KW * PPG % NW == 0, "whole pieces per wave");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave % WM, wn = wave / WM;
+  const int kg = wave / NG, wm = wave % NG % WM, wn = wave % NG / WM;
   const int l15 = lane & 15, g = lane >> 4;
   int tm, tn;
   int8_tile_of(blockIdx.x, (p.M + BM - 1) / BM, (p.N + BN - 1) / BN, tm, tn);
@@ -194,32 +198,25 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_int8_kernel(const Int8GemmA
   const char* w_tile = reinterpret_cast<const char*>(p.W) + (int64_t)n0 * p.ldw;
   const unsigned lds = __builtin_amdgcn_readfirstlane(lds_offset(smem));
 
-  unsigned row_off[PPW], chunk[PPW], dst[PPW];  // lane offset of the row, of the 16-byte chunk in the step; LDS place of the piece
+  unsigned row_off[PPW], chunk[PPW], dst[PPW];  // lane offset of the row; of its 16-byte chunk within the step; LDS place of the piece
   const char* base[PPW];
 #pragma unroll
   for (int i = 0; i < PPW; ++i) {
-    int piece = wave + NW * i;
-    if (piece >= PIECES) piece -= PIECES;
+    const int at = wave * PPW + i, group = at / PPG, piece = at % PPG;
     const bool of_a = piece < BM / 8;
     const int r = (of_a ? piece : piece - BM / 8) * 8 + (lane >> 3);
     const int rows = of_a ? p.M - m0 : p.N - n0;
     row_off[i] = (unsigned)(r < rows ? r : rows - 1) * (unsigned)(of_a ? p.lda : p.ldw);
-    chunk[i] = (unsigned)(((lane & 7) ^ ((r >> 1) & 7)) * 16);
-    dst[i] = __builtin_amdgcn_readfirstlane(piece * 1024);
+    chunk[i] = (unsigned)(group * 128) + (unsigned)(((lane & 7) ^ ((r >> 1) & 7)) * 16);
+    dst[i] = __builtin_amdgcn_readfirstlane(at * 1024);
     base[i] = of_a ? a_tile : w_tile;
   }
-  const int nk = (p.K + 127) >> 7;
-  auto issue = [&](int kt, int slot) {
-    const int k0 = kt * 128;
-    if (k0 + 128 <= p.K) {
+  const int nk = (p.K + 128 * KW - 1) / (128 * KW);
+  auto issue = [&](int kt, int slot) {  // chunks behind the end of K read the start of their row instead (masked below)
 #pragma unroll
-      for (int i = 0; i < PPW; ++i) lds_dma16(base[i] + k0, row_off[i] + chunk[i], lds + slot * STAGE_BYTES + dst[i]);
-    } else {  // the step that holds the end of K: chunks behind it read the start of their row instead (masked below)
-#pragma unroll
-      for (int i = 0; i < PPW; ++i) {
-        const unsigned k = (unsigned)k0 + chunk[i];
-        lds_dma16(base[i], row_off[i] + (k < (unsigned)p.K ? k : 0u), lds + slot * STAGE_BYTES + dst[i]);
-      }
+    for (int i = 0; i < PPW; ++i) {
+      const unsigned k = (unsigned)kt * (128 * KW) + chunk[i];
+      lds_dma16(base[i], row_off[i] + (k < (unsigned)p.K ? k : 0u), lds + slot * STAGE_BYTES + dst[i]);
     }
   };
 
@@ -229,7 +226,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_int8_kernel(const Int8GemmA
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = (i32x4){0, 0, 0, 0};
   const int swz = (l15 >> 1) & 7;
-  const int a_row = (wm * (BM / WM) + l15) * 128, w_row = A_BYTES + (wn * (BN / WN) + l15) * 128;
+  const int a_row = kg * GROUP_BYTES + (wm * (BM / WM) + l15) * 128, w_row = kg * GROUP_BYTES + A_BYTES + (wn * (BN / WN) + l15) * 128;
   auto step = [&](int slot, int left, auto last) {
     const char* st = smem + slot * STAGE_BYTES;
 #pragma unroll
@@ -260,13 +257,29 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_int8_kernel(const Int8GemmA
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     if (kt + STAGES - 1 < nk) issue(kt + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
-    const int left = p.K - kt * 128;
+    const int left = p.K - (kt * KW + kg) * 128;
     if (left >= 128) step(slot, left, std::false_type{});
     else step(slot, left, std::true_type{});
     slot = slot + 1 == STAGES ? 0 : slot + 1;
   }
   __syncthreads();
-  int8_epilogue<T, BM, BN, FM, FN, NW * 64, EPI>(p, smem, m0, n0, wm * (BM / WM), wn * (BN / WN), [&](auto ic, auto jc) -> i32x4 { return acc[decltype(ic)::value][decltype(jc)::value]; });
+  if constexpr (KW > 1) {  // the other groups' sums to the first one
+    i32x4* part = reinterpret_cast<i32x4*>(smem) + (wave % NG) * 64 + lane;
+    constexpr int FRAGS = FM * FN;
+    if (kg > 0) {
+#pragma unroll
+      for (int f = 0; f < FRAGS; ++f) part[((kg - 1) * FRAGS + f) * NG * 64] = acc[f / FN][f % FN];
+    }
+    __syncthreads();
+    if (kg == 0) {
+#pragma unroll
+      for (int f = 0; f < FRAGS; ++f)
+#pragma unroll
+        for (int k = 0; k < KW - 1; ++k) acc[f / FN][f % FN] += part[(k * FRAGS + f) * NG * 64];
+    }
+    __syncthreads();
+  }
+  int8_epilogue<T, BM, BN, FM, FN, NW * 64, EPI>(p, smem, m0, n0, wm * (BM / WM), wn * (BN / WN), kg == 0, [&](auto ic, auto jc) -> i32x4 { return acc[decltype(ic)::value][decltype(jc)::value]; });
 }
 
 // The same product on one wave per SIMD, 256 x BN tiles on four waves: the K loop over whole stages is one hand-placed asm statement (gemm_int8_asm.h, generated by
@@ -350,7 +363,7 @@ __global__ __launch_bounds__(256) void gemm_int8_wide_kernel(const Int8GemmArgs 
     }
     asm volatile("s_nop 15\n\ts_nop 7");  // and the accumulators are read next
   }
-  int8_epilogue<T, BM, BN, FM, FN, 256, EPI>(p, smem, m0, n0, wm0, wn0, [&](auto ic, auto jc) -> i32x4 {
+  int8_epilogue<T, BM, BN, FM, FN, 256, EPI>(p, smem, m0, n0, wm0, wn0, true, [&](auto ic, auto jc) -> i32x4 {
     constexpr int i = decltype(ic)::value, j = decltype(jc)::value;
     if constexpr (j < 8 || G::tall) return agpr_read<G::agpr(i, j)>();
     else return c8[i];

@@ -108,26 +108,26 @@ template <size_t N> bool meets_any(const Region& out, const Region (&others)[N])
 constexpr int MAX_ROW = 32768;       // widest row that the norms hold in registers (1024 lanes x 4 pieces)
 constexpr int MAX_INT8_K = 131071;   // 128^2 K stays below 2^31
 
-constexpr int row_slots(int waves) { return waves >= 4 ? 1 : 4 / waves; }  // rows a workgroup works on at a time
-
 // ---- 8-bit rows ----------------------------------------------------------------------------------------------------------------------------------------------
 
+template <typename T, int WAVES, int CH> int launch_quantize(const OpCtx& ctx, const QuantizeArgs& a, OpStatus& st) {
+  const dim3 grid((unsigned)(((int64_t)a.M + row_slots(WAVES) - 1) / row_slots(WAVES))), block(WAVES == 1 ? 256 : WAVES * 64);
+  if (a.K % 8) hipLaunchKernelGGL((quantize_rows_kernel<T, WAVES, CH, true>), grid, block, 0, ctx.stream, a);
+  else hipLaunchKernelGGL((quantize_rows_kernel<T, WAVES, CH, false>), grid, block, 0, ctx.stream, a);
+  return launched(st, "quantize_int8");
+}
 template <typename T> int quantize_t(const OpCtx& ctx, const QuantizeArgs& a, OpStatus& st) {
   const int pieces = (a.K + 7) / 8;
-  auto grid = [&](int rows) { return dim3((unsigned)(((int64_t)a.M + rows - 1) / rows)); };
-#define ECAD_QUANT(WAVES, CH) hipLaunchKernelGGL((quantize_rows_kernel<T, WAVES, CH>), grid(row_slots(WAVES)), dim3(WAVES > 4 ? WAVES * 64 : 256), 0, ctx.stream, a)
-  if (pieces <= 64) ECAD_QUANT(1, 1);
-  else if (pieces <= 128) ECAD_QUANT(1, 2);
-  else if (pieces <= 192) ECAD_QUANT(1, 3);
-  else if (pieces <= 256) ECAD_QUANT(4, 1);
-  else if (pieces <= 512) ECAD_QUANT(4, 2);
-  else if (pieces <= 768) ECAD_QUANT(4, 3);
-  else if (pieces <= 1024) ECAD_QUANT(4, 4);
-  else if (pieces <= 2048) ECAD_QUANT(4, 8);
-  else if (pieces <= 4096) ECAD_QUANT(16, 4);
-  else ECAD_QUANT(16, 16);
-#undef ECAD_QUANT
-  return launched(st, "quantize_int8");
+  if (pieces <= 64) return launch_quantize<T, 1, 1>(ctx, a, st);
+  if (pieces <= 128) return launch_quantize<T, 1, 2>(ctx, a, st);
+  if (pieces <= 192) return launch_quantize<T, 1, 3>(ctx, a, st);
+  if (pieces <= 256) return launch_quantize<T, 4, 1>(ctx, a, st);
+  if (pieces <= 512) return launch_quantize<T, 4, 2>(ctx, a, st);
+  if (pieces <= 768) return launch_quantize<T, 4, 3>(ctx, a, st);
+  if (pieces <= 1024) return launch_quantize<T, 4, 4>(ctx, a, st);
+  if (pieces <= 2048) return launch_quantize<T, 8, 4>(ctx, a, st);
+  if (pieces <= 4096) return launch_quantize<T, 16, 4>(ctx, a, st);
+  return launch_quantize<T, 16, 16>(ctx, a, st);
 }
 
 // ---- norms ---------------------------------------------------------------------------------------------------------------------------------------------------
@@ -138,7 +138,7 @@ template <typename T, int WAVES, int CH, bool HOLD = true> int launch_norm(const
   const int slots = row_slots(WAVES);
   const int64_t at_once = (int64_t)ctx.num_cus * per_cu;
   a.rows_per_group = (int)((a.M + at_once - 1) / at_once);
-  const dim3 grid((unsigned)(((int64_t)a.M + (int64_t)slots * a.rows_per_group - 1) / ((int64_t)slots * a.rows_per_group))), block(WAVES > 4 ? WAVES * 64 : 256);
+  const dim3 grid((unsigned)(((int64_t)a.M + (int64_t)slots * a.rows_per_group - 1) / ((int64_t)slots * a.rows_per_group))), block(WAVES == 1 ? 256 : WAVES * 64);
   if (a.D % 8) hipLaunchKernelGGL((gate_norm_kernel<T, WAVES, CH, true, HOLD>), grid, block, 0, ctx.stream, a);
   else hipLaunchKernelGGL((gate_norm_kernel<T, WAVES, CH, false, HOLD>), grid, block, 0, ctx.stream, a);
   return launched(st, "gate_norm");
@@ -146,10 +146,10 @@ template <typename T, int WAVES, int CH, bool HOLD = true> int launch_norm(const
 template <typename T> int gate_norm_t(const OpCtx& ctx, GateNormArgs& a, OpStatus& st) {
   const int pieces = (a.D + 7) / 8;
   if (pieces <= 64) return launch_norm<T, 1, 1>(ctx, a, 20, st);
-  if (pieces <= 128) return launch_norm<T, 1, 2>(ctx, a, 12, st);
-  if (pieces <= 192) return launch_norm<T, 1, 3>(ctx, a, 8, st);
+  if (pieces <= 128) return launch_norm<T, 2, 1>(ctx, a, 10, st);
+  if (pieces <= 192) return a.M <= 8 * ctx.num_cus ? launch_norm<T, 3, 1>(ctx, a, 6, st) : launch_norm<T, 1, 3>(ctx, a, 8, st);  // 5 rows 3.9 / 5.6 us, 2048 rows 8.8 / 9.4, 4096 rows 13.9 / 12.5, 32768 rows 75 / 57.5
   if (pieces <= 256) return launch_norm<T, 4, 1>(ctx, a, 5, st);
-  if (pieces <= 512) return launch_norm<T, 4, 2>(ctx, a, 3, st);
+  if (pieces <= 512) return launch_norm<T, 8, 1>(ctx, a, 2, st);
   if (pieces <= 1024) return launch_norm<T, 8, 2>(ctx, a, 1, st);
   if (pieces <= 2048) return launch_norm<T, 16, 2, false>(ctx, a, 1, st);
   return launch_norm<T, 16, 4, false>(ctx, a, 1, st);
@@ -167,9 +167,9 @@ int launch_int8(const OpCtx& ctx, const Int8GemmArgs& a, OpStatus& st, std::atom
   hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(threads), bytes, ctx.stream, a);
   return launched(st, "gemm_int8");
 }
-template <typename T, int EPI, int BM, int BN, int WM, int WN, int STAGES> int launch_tile(const OpCtx& ctx, const Int8GemmArgs& a, OpStatus& st) {
+template <typename T, int EPI, int BM, int BN, int WM, int WN, int KW, int STAGES> int launch_tile(const OpCtx& ctx, const Int8GemmArgs& a, OpStatus& st) {
   static std::atomic<uint64_t> done{0};
-  return launch_int8(ctx, a, st, done, gemm_int8_kernel<T, BM, BN, WM, WN, STAGES, EPI>, BM, BN, WM * WN * 64, int8_lds_bytes(BM, BN, STAGES));
+  return launch_int8(ctx, a, st, done, gemm_int8_kernel<T, BM, BN, WM, WN, KW, STAGES, EPI>, BM, BN, WM * WN * KW * 64, int8_lds_bytes(BM, BN, STAGES * KW));
 }
 template <typename T, int EPI, int BN> int launch_wide(const OpCtx& ctx, const Int8GemmArgs& a, OpStatus& st) {
   static std::atomic<uint64_t> done{0};
@@ -211,8 +211,9 @@ template <typename T, int EPI> int gemm_int8_t(const OpCtx& ctx, const Int8GemmA
       else hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 4, 8, EPI>), grid, dim3(512), 0, ctx.stream, a);
       return launched(st, "gemm_int8");
     }
-    case ECAD_I8_K_TILE64: return launch_tile<T, EPI, 64, 64, 2, 2, 4>(ctx, a, st);
-    case ECAD_I8_K_TILE128: return launch_tile<T, EPI, 128, 128, 2, 2, 2>(ctx, a, st);
+    case ECAD_I8_K_TILE64: return launch_tile<T, EPI, 64, 64, 2, 2, 1, 4>(ctx, a, st);
+    case ECAD_I8_K_TILE64_K2: return launch_tile<T, EPI, 64, 64, 2, 2, 2, 4>(ctx, a, st);
+    case ECAD_I8_K_TILE128: return launch_tile<T, EPI, 128, 128, 2, 2, 1, 2>(ctx, a, st);
     case ECAD_I8_K_TILE144: return launch_wide<T, EPI, 144>(ctx, a, st);
     case ECAD_I8_K_TILE256: return launch_wide<T, EPI, 256>(ctx, a, st);
     case ECAD_I8_K_TILE288: return launch_wide<T, EPI, 288>(ctx, a, st);
@@ -337,7 +338,7 @@ int op_rope_table(const OpCtx& ctx, const RopeTableCall& c, OpStatus& st) noexce
         keep = keep < 0 ? 0 : (keep > 1 ? 1 : keep);
         f = f * keep + f / c.factor * (1 - keep);
       }
-      a.turns[a.pairs] = f / two_pi;
+      a.quarters[a.pairs] = 4.0 * f / two_pi;
       a.axis[a.pairs++] = (unsigned char)x;
     }
   }
@@ -346,8 +347,10 @@ int op_rope_table(const OpCtx& ctx, const RopeTableCall& c, OpStatus& st) noexce
   if (meet(vector(c.table, (int64_t)c.S * a.pairs * 2, 4), vector(c.positions, (int64_t)c.S * c.axes, 4))) return refuse(st, ECAD_E_INVALID, "rope_table: the table overlaps the positions");
   a.positions = c.positions; a.table = c.table; a.positions_float = c.positions_float; a.axes = c.axes; a.S = c.S;
   a.size = c.scaling == ECAD_ROPE_YARN ? (float)(0.1 * log(c.factor) + 1.0) : 1.0f;
-  const int64_t blocks = ((int64_t)c.S * a.pairs + 255) / 256, most = (int64_t)ctx.num_cus * 32;
-  hipLaunchKernelGGL(rope_table_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, ctx.stream, a);
+  a.rows_per_block = a.pairs >= 512 ? 1 : 512 / a.pairs;
+  const int threads = (a.rows_per_block * a.pairs + 63) / 64 * 64;
+  const int64_t blocks = ((int64_t)c.S + a.rows_per_block - 1) / a.rows_per_block, most = (int64_t)ctx.num_cus * 8;
+  hipLaunchKernelGGL(rope_table_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(threads), 0, ctx.stream, a);
   return launched(st, "rope_table");
 }
 

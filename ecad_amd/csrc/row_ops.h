@@ -30,6 +30,33 @@ template <typename T> ECAD_DEV Pack8 load_piece(const T* p, int n) {
   }
   return v;
 }
+// The piece at column c of a row of D elements, zeros beyond its end, in two steps: the load, and behind it (where the piece is used: the load stays in flight until
+// then) what makes it whole.  RAGGED: the row's last piece is not whole; where the row has eight elements the last eight are read in its place and shifted, without
+// branches.  The elements shifted out belong to the piece before: what another lane may be writing to them in place does not matter.
+template <typename T, bool RAGGED> ECAD_DEV Pack8 row_load(const T* row, int c, int D) {
+  Pack8 v;
+  if constexpr (!RAGGED) {
+    v.u = (u32x4){0, 0, 0, 0};
+    if (c < D) v.u = reinterpret_cast<const Bytes16*>(row + c)->u;
+  } else if (D < 8) {
+    v = load_piece<T>(row + c, D - c);
+  } else {
+    v.u = reinterpret_cast<const Bytes16*>(row + (c < D - 8 ? c : D - 8))->u;
+  }
+  return v;
+}
+template <bool RAGGED> ECAD_DEV Pack8 row_piece(const Pack8& raw, int c, int D) {
+  if constexpr (!RAGGED) return raw;
+  const int s = D < 8 || c < D - 8 ? 0 : c - (D - 8);
+  unsigned a = raw.u[0], b = raw.u[1], d = raw.u[2], e = raw.u[3];
+  a = s & 4 ? d : a, b = s & 4 ? e : b, d = s & 4 ? 0u : d, e = s & 4 ? 0u : e;
+  a = s & 2 ? b : a, b = s & 2 ? d : b, d = s & 2 ? e : d, e = s & 2 ? 0u : e;
+  a = s & 1 ? (a >> 16 | b << 16) : a, b = s & 1 ? (b >> 16 | d << 16) : b, d = s & 1 ? (d >> 16 | e << 16) : d, e = s & 1 ? e >> 16 : e;
+  const bool none = s >= 8;
+  Pack8 v;
+  v.u = (u32x4){none ? 0u : a, none ? 0u : b, none ? 0u : d, none ? 0u : e};
+  return v;
+}
 template <typename T> ECAD_DEV void store_piece(T* p, const Pack8& v, int n) {
   if (n >= 8) {
     reinterpret_cast<Bytes16*>(p)->u = v.u;
@@ -107,7 +134,8 @@ template <typename T> ECAD_DEV float bits_value(unsigned b) { return (float)__bu
 // quotient within 1e-5 of the true one, so only a value next to a border can be on the wrong side; its remainder x - n s is exact in fp32 (both are multiples of
 // the last place of the smaller one and it is below s) and decides.  A row with an infinity or a NaN has scale NaN and zeros: its products are NaN, not numbers.
 constexpr float INT8_MAX_F = 127.0f;
-constexpr float INT8_TINY = 1e-30f;  // below: 1 / s could leave the range of fp32, quotients are divided
+constexpr float INT8_TINY = 1e-30f;         // below: 1 / s could leave the range of fp32, quotients are divided
+constexpr float INT8_MAGIC = 12582912.0f;   // 1.5 2^23: adding it rounds to an integer (ties to even) and leaves that integer's two's complement in the low bits
 
 struct Int8Scale {
   float s, inv, half;
@@ -123,32 +151,39 @@ template <typename T> ECAD_DEV Int8Scale int8_scale(unsigned max_magnitude_bits)
   r.half = 0.5f * r.s;
   return r;
 }
-ECAD_DEV int int8_round(float x, const Int8Scale& k) {
-  float n = rintf(x * k.inv);
-  const float d = __builtin_fmaf(-n, k.s, x);
-  if (fabsf(d) >= k.half) {  // on or beyond the border
-    const float step = d > 0.f ? 1.f : -1.f;
-    if (fabsf(d) > k.half || ((int)n & 1)) n += step;
-  }
-  return (int)n;
-}
 // rows whose largest value is below INT8_TINY (bf16 only): the division itself, in 64 bits
-ECAD_DEV int int8_round_tiny(float x, const Int8Scale& k) { return k.s > 0.f ? (int)fmin(fmax(rint((double)x / (double)k.s), -127.0), 127.0) : 0; }
+ECAD_DEV float int8_round_tiny(float x, const Int8Scale& k) { return k.s > 0.f ? (float)fmin(fmax(rint((double)x / (double)k.s), -127.0), 127.0) : 0.f; }
 
-ECAD_DEV unsigned pack_bytes(int a, int b, int c, int d) { return (unsigned)(a & 255) | (unsigned)(b & 255) << 8 | (unsigned)(c & 255) << 16 | (unsigned)d << 24; }
+// low bytes of four registers into one
+ECAD_DEV unsigned gather_bytes(const float* m) {
+  const unsigned lo = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, m[1]), __builtin_bit_cast(unsigned, m[0]), 0x0c0c0400u);
+  const unsigned hi = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, m[3]), __builtin_bit_cast(unsigned, m[2]), 0x0c0c0400u);
+  return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
 
-// eight values of a row to their 8-bit piece (the branches are the row's: the same for all its lanes)
+// eight values of a row to their 8-bit piece (bad and tiny are the row's: the same for all its lanes)
 ECAD_DEV u32x2 int8_piece(const float (&x)[8], const Int8Scale& k) {
-  int n[8];
+  float m[8];
   if (k.bad) return (u32x2){0, 0};
   if (!k.tiny) {
+    float worst = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) n[e] = int8_round(x[e], k);
+    for (int e = 0; e < 8; ++e) {
+      m[e] = __builtin_fmaf(x[e], k.inv, INT8_MAGIC);
+      worst = fmaxf(worst, fabsf(__builtin_fmaf(INT8_MAGIC - m[e], k.s, x[e])));
+    }
+    if (worst >= k.half) {  // one of the eight on or beyond the border
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = __builtin_fmaf(INT8_MAGIC - m[e], k.s, x[e]), step = d > 0.f ? 1.f : -1.f;
+        if (fabsf(d) > k.half || (fabsf(d) == k.half && (__builtin_bit_cast(unsigned, m[e]) & 1))) m[e] += step;
+      }
+    }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) n[e] = int8_round_tiny(x[e], k);
+    for (int e = 0; e < 8; ++e) m[e] = int8_round_tiny(x[e], k) + INT8_MAGIC;
   }
-  return (u32x2){pack_bytes(n[0], n[1], n[2], n[3]), pack_bytes(n[4], n[5], n[6], n[7])};
+  return (u32x2){gather_bytes(m), gather_bytes(m + 4)};
 }
 ECAD_DEV void store_int8_piece(int8_t* p, u32x2 v, int n) {  // rows of 8-bit values start on 16 bytes
   if (n >= 8) {

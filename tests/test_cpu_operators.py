@@ -42,7 +42,7 @@ f32 = torch.zeros
 def test_quantize_refusals(eng):
     with pytest.raises(ValueError, match="torch.float16"):
         eng.op_quantize_int8(torch.zeros(4, 8))
-    with pytest.raises(ValueError, match="shape"):
+    with pytest.raises(ValueError, match="two dimensions"):
         eng.op_quantize_int8(f16(4, 8, 2))
     with pytest.raises(ValueError, match="dense last"):
         eng.op_quantize_int8(f16(8, 4).t())
@@ -56,7 +56,7 @@ def test_gemm_refusals(eng):
     a, w, sa, sw = i8(3, 40), i8(7, 40), f32(3), f32(7)
     call = lambda epi=0, **k: eng.op_gemm_int8(epi, *(k.pop(x, d) for x, d in (("a", a), ("sa", sa), ("w", w), ("sw", sw))), **k)  # noqa: E731
     for bad, match in [
-        (dict(w=i8(7, 41)), "shape"),
+        (dict(w=i8(7, 41)), "w must have shape"),
         (dict(sa=f32(4)), "a_scale"),
         (dict(sw=None), "needed"),
         (dict(bias=f16(7)), "bias"),
@@ -79,7 +79,7 @@ def test_gate_norm_refusals(eng):
         ((h, f16(4, 23), {}), "shape"),
         ((h, y, dict(pre="batch")), "one of"),
         ((h, y, dict(pre_weight=f16(24))), "pre_weight"),
-        ((h, y, dict(gate_mod=f16(24))), "samples"),
+        ((h, y, dict(gate_mod=f16(24))), "two dimensions"),
         ((h, y, dict(mod_shift=f16(3, 24))), "samples"),
         ((h, y, dict(mod_shift=f16(2, 24), mod_scale=f16(2, 48)[:, :24], rows_per_batch=2)), "same stride"),
         ((h, y, dict(pre="none", quantize=True)), "quantize"),
@@ -103,6 +103,8 @@ def test_rope_refusals(eng):
         ((q, k, t), dict(index=torch.zeros(3, dtype=torch.int64)), "int32"),
         ((q, k, t), dict(out=(k, q)), "shape"),
         ((q, k, t), dict(out=(q, None)), "k_out"),
+        ((q.requires_grad_(False), k, f32(3, 8, 2).requires_grad_()), {}, "gradient"),
+        ((q, k, torch.zeros(2, 3, 8).permute(1, 2, 0)), {}, "contiguous"),
         ((q, None, t), dict(out=(q.transpose(1, 2), None)), "shape"),
         ((f16(3, 4, 16), k, t), {}, "shape"),
     ]:
@@ -276,3 +278,15 @@ def test_timed_cases_stay_in_their_ranges():
         case = operators.draw(random.Random(seed))
         work = operators.work(case)
         assert work["bytes"] <= 1.05 * most["bytes"] and work["flops"] <= 1.05 * most["flops"], case
+
+
+def test_gradients_are_refused_while_they_are_recorded(eng):
+    """Under no_grad a parameter may be passed; the call then reaches the library."""
+    x = f16(4, 16).requires_grad_()
+    with pytest.raises(ValueError, match="gradient"):
+        eng.op_gate_norm(f16(4, 16), x)
+    with pytest.raises(ValueError, match="gradient"):
+        eng.op_gate_norm(f16(4, 16), pre_weight=torch.ones(16, requires_grad=True))
+    eng._stream = lambda: 0
+    with torch.no_grad(), pytest.raises(AssertionError, match="ecad_op_gate_norm was called"):
+        eng.op_gate_norm(f16(4, 16), x, pre_weight=torch.ones(16, requires_grad=True))
