@@ -7,7 +7,6 @@ from __future__ import annotations
 
 import ctypes as C
 import os
-import struct
 from pathlib import Path
 
 LIB_NAME = "libecad_hip.so"
@@ -113,13 +112,6 @@ class EcadFluxStats(C.Structure):
     def as_dict(self) -> dict:
         return {name: getattr(self, name) for name, _ in self._fields_}
 
-
-# Arguments of the operators of an 8-bit transformer block (EcadInt8Gemm, EcadGateNorm, EcadRope), packed by struct: members in the header's order, which has no
-# padding (tests/test_cpu_operators.py holds the layouts to the C compiler's).  P pointer, q int64, i int32, f float.
-_HEADS = "PP" + "qqq" + "qqq" + "q"
-INT8_GEMM = struct.Struct("PqPPqPPPqPqPqPPq" + "iiiiii")
-GATE_NORM = struct.Struct("PqPqPqPqPqPPPPPqPPPPq" + "iiiiii" + "ff")
-ROPE = struct.Struct(_HEADS + _HEADS + "PPq" + "iiiiiiii")
 
 _P = C.c_void_p
 _I = C.c_int
@@ -236,3 +228,14 @@ def load() -> C.CDLL:
         raise EcadLibraryError(f"ABI version mismatch: library {lib.ecad_abi_version()}, binding {ABI_VERSION}")
     _lib = lib
     return lib
+
+
+def load_ops():
+    """The native side of the small operators' Python calls (ecad_amd/_ops.so, built next to the library); raise loudly if it is missing."""
+    import torch  # noqa: F401  (its libraries first)
+
+    try:
+        from ecad_amd import _ops
+    except ImportError as e:
+        raise EcadLibraryError(f"ecad_amd/_ops.so cannot be loaded ({e}). Build it with `make -C ecad_amd/csrc`.") from e
+    return _ops

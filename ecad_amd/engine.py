@@ -56,6 +56,7 @@ class EcadEngine:
         self._ctor = dict(num_layers=num_layers, num_heads=num_heads, head_dim=head_dim, in_channels=in_channels, out_channels=out_channels, patch_size=patch_size,
                           sample_size=sample_size, caption_channels=caption_channels, max_batch=max_batch, max_tokens=max_tokens, max_text_tokens=max_text_tokens,
                           dtype=dtype, norm_eps=norm_eps, interpolation_scale=interpolation_scale, device=device, fp8=fp8, use_additional_conditions=use_additional_conditions)
+        self._ops = None  # the native side of the small operators' calls (_native)
         self._donor = None  # the engine whose weights this context reads (kept alive as long as this one)
         self._bits = None
         self.dtype = dtype
@@ -94,6 +95,7 @@ class EcadEngine:
         if getattr(self, "_h", None) and self._h.value:
             self.lib.ecad_destroy(self._h)
             self._h = C.c_void_p()
+            self._ops = self._ops and (self._ops[0], None)
         self._donor = None
 
     def set_ln_fold(self, on: bool) -> None:
@@ -402,88 +404,26 @@ class EcadEngine:
 
     # -- the launches of an 8-bit transformer block ---------------------------------------------
     # Inference only, like every op here: tensors that require a gradient are refused while gradients are recorded.  Work goes to the current stream of the engine's
-    # device; nothing is allocated but the results.  The library refuses outputs that overlap themselves or another argument.  The checks are written for the call that
-    # passes (a small op is a few microseconds of host time): one comparison each, and _refuse finds out what was wrong.
-    def _refuse(self, name: str, t, dtype: torch.dtype, shape: tuple, dense: str = "be contiguous") -> None:
-        if not isinstance(t, torch.Tensor):
-            raise ValueError(f"{name} must be a tensor, got {type(t).__name__}")
-        if t.device != self.device:
-            raise ValueError(f"{name} is on {t.device}, this engine on {self.device}")
-        if t.dtype is not dtype:
-            raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-        if t.shape != tuple(shape):
-            raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-        if not (t.is_contiguous() if dense == "be contiguous" else t.shape[-1] <= 1 or t.stride(-1) == 1):
-            raise ValueError(f"{name} must {dense}, got strides {t.stride()}")
-        if torch.is_grad_enabled():  # what is left: it requires a gradient
-            raise ValueError(f"{name} requires a gradient: this op has none (detach it, or call under torch.no_grad())")
-
-    @staticmethod
-    def _matrix(name: str, t) -> torch.Size:
-        if not isinstance(t, torch.Tensor) or t.dim() != 2:
-            raise ValueError(f"{name} must be a tensor of two dimensions")
-        return t.shape
-
-    def _rows(self, name: str, t, dtype: torch.dtype, shape: tuple) -> int:
-        """Row stride of a matrix with dense rows."""
-        if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == self.device and (t.stride(1) == 1 or shape[1] <= 1) and not t.requires_grad):
-            self._refuse(name, t, dtype, shape, "have a dense last dimension")
-        return t.stride(0) if shape[0] > 1 else shape[1]
-
-    def _vector(self, name: str, t, shape: tuple) -> int:
-        """Address of a contiguous fp32 tensor; 0 for None."""
-        if t is None:
-            return 0
-        if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.shape == shape and t.device == self.device and t.is_contiguous() and not t.requires_grad):
-            self._refuse(name, t, torch.float32, shape)
-        return t.data_ptr()
-
-    def _mod(self, name: str, t, M: int, N: int, rows_per_batch: int) -> tuple[int, int]:
-        """(address, stride between samples) of modulations [samples, N] that cover M rows; (0, 0) for None, stride 0 for one sample."""
-        if t is None:
-            return 0, 0
-        samples = self._matrix(name, t)[0]
-        if not (t.dtype is self.dtype and t.shape[1] == N and t.device == self.device and (t.stride(1) == 1 or N <= 1) and not t.requires_grad):
-            self._refuse(name, t, self.dtype, (samples, N), "have a dense last dimension")
-        if rows_per_batch < 1 or M > samples * rows_per_batch:
-            raise ValueError(f"{name} has {samples} samples of {rows_per_batch} rows, {M} rows are given" if rows_per_batch >= 1 else f"rows_per_batch must be at least 1, got {rows_per_batch}")
-        return t.data_ptr(), t.stride(0) if samples > 1 else 0
-
-    def _new_int8_rows(self, M: int, N: int) -> tuple[torch.Tensor, int]:
-        """[M, N] int8 whose rows start on 16 bytes, and their stride."""
-        stride = (N + 15) & ~15
-        rows = torch.empty((M, stride), device=self.device, dtype=torch.int8)
-        return (rows if stride == N else rows[:, :N]), stride
-
-    def _int8_out(self, name: str, out, M: int, N: int) -> tuple[torch.Tensor, int, torch.Tensor]:
-        """A caller's (q, scale) pair: q, its row stride, scale."""
-        q, scale = out
-        stride = self._rows(name, q, torch.int8, (M, N))
-        if scale is None:
-            raise ValueError(f"{name} must come with its scale")
-        self._vector("scale", scale, (M,))
-        return q, q.stride(0) if M == 1 else stride, scale
-
-    def _stream(self) -> int:
-        """The current stream of the engine's device (torch.cuda.current_stream builds an object around this number, which takes longer than a small launch)."""
-        return torch._C._cuda_getCurrentRawStream(self.device_index)
+    # device; nothing is allocated but the results.  What does not fit together is a ValueError, outputs that overlap themselves or another argument among it.  The
+    # checks and the call are native (csrc/binding.cpp): these launches are a few microseconds, and so has to be what stands in front of them.
+    def _native(self):
+        """(functions, this engine) of ecad_amd/_ops.so; a closed engine is None there."""
+        if not self._h.value:
+            raise RuntimeError("the engine is closed")
+        if self._ops is None:
+            names = ("ecad_op_quantize_int8", "ecad_op_gemm_int8", "ecad_op_gate_norm", "ecad_op_rope_table", "ecad_op_rope", "ecad_last_error")
+            addresses = tuple(C.cast(getattr(self.lib, n), C.c_void_p).value for n in names)
+            ops = L.load_ops()
+            self._ops = ops, ops.engine(addresses, self._h.value, _TORCH2ECAD[self.dtype], self.device_index, torch._C._cuda_getCurrentRawStream)
+        return self._ops
 
     def op_quantize_int8(self, x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Rows to 8-bit integers with one scale each (``ecad_op_quantize_int8``): x [M, K] of the engine's dtype at any row stride -> (q [M, K] int8 whose rows start on
         16 bytes, scale [M] fp32), x ~ q * scale[:, None].  scale = max|row| / 127, q the nearest integer (ties to even) in exact arithmetic.  A row of zeros has
         scale 0; one with an infinity or NaN has scale NaN.  Weights [N, K] (one scale per output channel) go through the same call once.
         ``out``: (q, scale) to write to; q's rows on 16 bytes."""
-        M, K = shape = self._matrix("x", x)
-        ldx = self._rows("x", x, self.dtype, shape)
-        if out is None:
-            q, ldq = self._new_int8_rows(M, K)
-            scale = torch.empty((M,), device=self.device, dtype=torch.float32)
-        else:
-            q, ldq, scale = self._int8_out("q", out, M, K)
-        rc = self.lib.ecad_op_quantize_int8(self._h, x.data_ptr(), ldx, q.data_ptr(), ldq, scale.data_ptr(), M, K, self._stream())
-        if rc:
-            self._raise(rc)
-        return q, scale
+        ops, engine = self._ops or self._native()
+        return ops.quantize_int8(engine, x, out)
 
     INT8_KERNELS = {"auto": 0, "rows": 1, "tile64": 2, "tile128": 3, "tile144": 4, "tile256": 5, "tile288": 6, "tile64k2": 7}
 
@@ -491,37 +431,11 @@ class EcadEngine:
         """A Linear in 8-bit integers (``ecad_op_gemm_int8``): o = act(a_scale[m] w_scale[n] (a @ w.T)[m, n] + bias[n]); a [M, K], w [N, K] int8 with rows on 16 bytes
         (``op_quantize_int8`` makes such), scales and bias fp32.  epi as ``op_gemm``: 0 none, 1 GELU(tanh), 2 SiLU -> o [M, N]; 3: ``out`` (None: not written) takes o, and
         ``resid_out`` (None: ``resid`` itself) takes resid + (gate_table[n] + gate_mod[m // rows_per_batch, n]) * o -> out.  ``kernel``: one by name, the same bits."""
-        M, K = a_shape = self._matrix("a", a)
-        N = self._matrix("w", w)[0]
-        self._rows("a", a, torch.int8, a_shape)
-        self._rows("w", w, torch.int8, (N, K))
-        if a_scale is None or w_scale is None:
-            raise ValueError("a_scale and w_scale are needed")
-        channels, shape = (N,), (M, N)
-        sa, sw, b = self._vector("a_scale", a_scale, (M,)), self._vector("w_scale", w_scale, channels), self._vector("bias", bias, channels)
-        if kernel not in self.INT8_KERNELS:
+        ops, engine = self._ops or self._native()
+        number = self.INT8_KERNELS.get(kernel)
+        if number is None:
             raise ValueError(f"kernel {kernel!r} unknown: one of {', '.join(self.INT8_KERNELS)}")
-        r = ro = gt = gm = ldr = ldro = gs = po = 0
-        ldo = N
-        if epi == 3:
-            if resid is None:
-                raise ValueError("epilogue 3 needs resid")
-            ldr, gt, (gm, gs) = self._rows("resid", resid, self.dtype, shape), self._vector("gate_table", gate_table, channels), self._mod("gate_mod", gate_mod, M, N, rows_per_batch)
-            resid_out = resid if resid_out is None else resid_out
-            ldro = self._rows("resid_out", resid_out, self.dtype, shape)
-            r, ro = resid.data_ptr(), resid_out.data_ptr()
-        elif resid is not None or gate_table is not None or gate_mod is not None or resid_out is not None:
-            raise ValueError("resid and gates belong to epilogue 3")
-        if out is not None:
-            ldo, po = self._rows("out", out, self.dtype, shape), out.data_ptr()
-        elif epi != 3:
-            out = torch.empty(shape, device=self.device, dtype=self.dtype)
-            po = out.data_ptr()
-        args = L.INT8_GEMM.pack(a.data_ptr(), a.stride(0), sa, w.data_ptr(), w.stride(0), sw, b, po, ldo, r, ldr, ro, ldro, gt, gm, gs, M, N, K, epi, rows_per_batch, self.INT8_KERNELS[kernel])
-        rc = self.lib.ecad_op_gemm_int8(self._h, args, self._stream())
-        if rc:
-            self._raise(rc)
-        return out
+        return ops.gemm_int8(engine, epi, a, a_scale, w, w_scale, bias, resid, gate_table, gate_mod, rows_per_batch, out, resid_out, number)
 
     NORMS = {"none": 0, "rms": 1, "layer": 2}
 
@@ -535,52 +449,12 @@ class EcadEngine:
         gate_mod [samples, D] (1 without either), scale and shift in the same way (0 without either); sample = row // rows_per_batch, modulations may be column slices of
         one wider tensor.  Returns (h', n); without y h' is h itself; with pre "none" n is None; ``quantize``: n as (q, scale) of ``op_quantize_int8``, bit for bit.
         ``out_h`` may be h, ``out_n`` may be y (``quantize``: out_n is a (q, scale) pair)."""
-        M, D = shape = self._matrix("h", h)
-        norms, dt = self.NORMS, self.dtype
-        if pre not in norms or post not in norms:
-            raise ValueError(f"pre and post are one of {', '.join(norms)}, got {pre!r} and {post!r}")
-        ldh = self._rows("h", h, dt, shape)
-        new_h, n, q, q_scale = h, None, None, None
-        py = ldy = ph = pn = pq = ldq = ps = 0
-        ldho = ldn = D
-        if y is not None:
-            ldy, py = self._rows("y", y, dt, shape), y.data_ptr()
-            if out_h is None:
-                new_h = torch.empty(shape, device=self.device, dtype=dt)
-            else:
-                new_h, ldho = out_h, self._rows("out_h", out_h, dt, shape)
-            ph = new_h.data_ptr()
-        elif out_h is not None:
-            raise ValueError("out_h without y: h' is h")
-        if pre == "none":
-            if out_n is not None or quantize:
-                raise ValueError("out_n or quantize without a pre-norm")
-        elif quantize:
-            if out_n is None:
-                q, ldq = self._new_int8_rows(M, D)
-                q_scale = torch.empty((M,), device=self.device, dtype=torch.float32)
-            else:
-                q, ldq, q_scale = self._int8_out("out_n", out_n, M, D)
-            pq, ps = q.data_ptr(), q_scale.data_ptr()
-        else:
-            if out_n is None:
-                n = torch.empty(shape, device=self.device, dtype=dt)
-            else:
-                n, ldn = out_n, self._rows("out_n", out_n, dt, shape)
-            pn = n.data_ptr()
-        gm, gs = self._mod("gate_mod", gate_mod, M, D, rows_per_batch)
-        ms, ss = self._mod("mod_shift", mod_shift, M, D, rows_per_batch)
-        mc, cs = self._mod("mod_scale", mod_scale, M, D, rows_per_batch)
-        if ss and cs and ss != cs:
-            raise ValueError(f"mod_shift and mod_scale must have the same stride between samples, got {ss} and {cs}")
-        vec, row = self._vector, (D,)
-        args = L.GATE_NORM.pack(h.data_ptr(), ldh, py, ldy, ph, ldho, pn, ldn, pq, ldq, ps, vec("post_weight", post_weight, row), vec("pre_weight", pre_weight, row), vec("gate_table", gate_table, row),
-                                gm, gs, vec("table_shift", table_shift, row), vec("table_scale", table_scale, row), ms, mc, ss or cs, M, D, rows_per_batch, norms[post], norms[pre], 0, resid_scale,
-                                self.cfg.norm_eps if eps is None else eps)
-        rc = self.lib.ecad_op_gate_norm(self._h, args, self._stream())
-        if rc:
-            self._raise(rc)
-        return new_h, (q, q_scale) if quantize else n
+        ops, engine = self._ops or self._native()
+        before, after = self.NORMS.get(pre), self.NORMS.get(post)
+        if before is None or after is None:
+            raise ValueError(f"pre and post are one of {', '.join(self.NORMS)}, got {pre!r} and {post!r}")
+        return ops.gate_norm(engine, h, y, before, after, pre_weight, post_weight, gate_table, gate_mod, table_shift, table_scale, mod_shift, mod_scale, rows_per_batch, resid_scale,
+                             self.cfg.norm_eps if eps is None else eps, quantize, out_h, out_n)
 
     ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 
@@ -588,79 +462,24 @@ class EcadEngine:
         """Cosines and sines of rotary positions (``ecad_op_rope_table``): positions [S] or [S, axes] int32 or fp32 -> [S, sum(axes_dims) / 2, 2] fp32, angles in 64 bits.
         axes_dims: elements that turn with each axis (even; an int for one axis), e.g. (16, 56, 56) for FLUX's (index, row, column).  scaling "linear" (f / factor), "ntk" (theta
         factor^(d / (d - 2))) or "yarn" (pairs that turn often within ``original_length`` stay, the others are stretched; cosine and sine times 0.1 ln(factor) + 1)."""
-        dims = (axes_dims,) if isinstance(axes_dims, int) else tuple(axes_dims)
-        if not isinstance(positions, torch.Tensor) or positions.dim() not in (1, 2) or positions.dtype not in (torch.int32, torch.float32):
-            raise ValueError("positions must be an int32 or float32 tensor of shape (S,) or (S, axes)")
-        S = positions.shape[0]
-        if (positions.shape[1] if positions.dim() == 2 else 1) != len(dims):
-            raise ValueError(f"positions of shape {tuple(positions.shape)} for {len(dims)} axes")
-        if scaling not in self.ROPE_SCALINGS:
+        ops, engine = self._ops or self._native()
+        number = self.ROPE_SCALINGS.get(scaling)
+        if number is None:
             raise ValueError(f"scaling {scaling!r} unknown: one of {', '.join(self.ROPE_SCALINGS)}")
-        if positions.device != self.device or not positions.is_contiguous() or positions.requires_grad:
-            self._refuse("positions", positions, positions.dtype, positions.shape)
-        shape = (S, max(0, sum(dims)) // 2, 2)
-        if out is None:
-            out = torch.empty(shape, device=self.device, dtype=torch.float32)
-            at = out.data_ptr()
-        else:
-            at = self._vector("out", out, shape)
-        rc = self.lib.ecad_op_rope_table(self._h, positions.data_ptr(), positions.dtype is torch.float32, (C.c_int32 * len(dims))(*dims), len(dims), S, self.ROPE_SCALINGS[scaling], theta, factor,
-                                         original_length, beta_fast, beta_slow, at, self._stream())
-        if rc:
-            self._raise(rc)
-        return out
-
-    def _heads(self, name: str, t, shape: tuple) -> tuple:
-        """Strides (sample, token, head) of [B, S, H, D] with dense heads."""
-        if not (isinstance(t, torch.Tensor) and t.dtype is self.dtype and t.shape == shape and t.device == self.device and (t.stride(3) == 1 or shape[3] <= 1) and not t.requires_grad):
-            self._refuse(name, t, self.dtype, shape, "have dense heads")
-        return t.stride()[:3]
+        return ops.rope_table(engine, positions, (axes_dims,) if isinstance(axes_dims, int) else tuple(axes_dims), theta, number, factor, original_length, beta_fast, beta_slow, out)
 
     def op_rope(self, q, k, table, layout="interleaved", index=None, inverse=False, out=None):
         """Rotary positions applied to heads (``ecad_op_rope``): q [B, S, Hq, D], k [B, S, Hk, D] (or None) at any strides with dense heads, e.g. column slices of a fused
         projection; table [rows, rot / 2, 2] fp32 (``op_rope_table``) with rot <= D: the first rot elements of a head turn, the others stay.  layout "interleaved": pairs
         (2j, 2j + 1), "half": pairs (j, j + rot / 2).  Token s takes table row s, or index[s] / index[b, s] (int32; outside the table: the token does not turn).
         ``inverse`` turns back.  Returns (q', k'): new tensors, or ``out`` = (q_out, k_out), which may be (q, k) themselves."""
+        ops, engine = self._ops or self._native()
         if layout not in ("interleaved", "half"):
             raise ValueError(f"layout {layout!r} unknown: interleaved or half")
-        if not isinstance(q, torch.Tensor) or q.dim() != 4:
-            raise ValueError("q must have shape (samples, tokens, heads, elements)")
-        B, S, Hq, D = shape = q.shape
-        if not isinstance(table, torch.Tensor) or table.dim() != 3 or table.shape[2] != 2:
-            raise ValueError("table must have shape (rows, pairs, 2)")
-        rows, pairs, _ = table.shape
-        at = index_stride = 0
-        if index is not None:
-            if not isinstance(index, torch.Tensor) or index.shape not in ((S,), (B, S)):
-                raise ValueError(f"index must have shape ({S},) or ({B}, {S})")
-            if index.dtype is not torch.int32 or index.device != self.device or (S > 1 and index.stride(-1) != 1):
-                self._refuse("index", index, torch.int32, index.shape, "have a dense last dimension")
-            at, index_stride = index.data_ptr(), index.stride(0) if index.dim() == 2 and B > 1 else 0
-        k_shape, k_out = None, None
-        if k is not None:
-            k_shape = k.shape
-            if len(k_shape) != 4 or k_shape[2] < 1 or k_shape != (B, S, k_shape[2], D):
-                raise ValueError(f"k of shape {tuple(k_shape)} for q of shape {tuple(shape)}")
-        q_strides, k_strides = self._heads("q", q, shape), () if k is None else self._heads("k", k, k_shape)
-        if out is None:
-            q_out = torch.empty(shape, device=self.device, dtype=self.dtype)
-            qo_strides = (S * Hq * D, Hq * D, D)
-            if k is not None:
-                k_out = torch.empty(k_shape, device=self.device, dtype=self.dtype)
-                ko_strides = (S * k_shape[2] * D, k_shape[2] * D, D)
-        else:
-            q_out, k_out = out
-            if (k is None) != (k_out is None):
-                raise ValueError("out must be (q_out, k_out), k_out None where k is None")
-            qo_strides = self._heads("q_out", q_out, shape)
-            ko_strides = () if k is None else self._heads("k_out", k_out, k_shape)
-        keys = (0,) * 9 if k is None else (k.data_ptr(), k_out.data_ptr(), *k_strides, *ko_strides, k_shape[2])
-        args = L.ROPE.pack(q.data_ptr(), q_out.data_ptr(), *q_strides, *qo_strides, Hq, *keys, self._vector("table", table, (rows, pairs, 2)), at, index_stride, B, S, D, 2 * pairs, rows,
-                           layout == "half", bool(inverse), 0)
-        rc = self.lib.ecad_op_rope(self._h, args, self._stream())
-        if rc:
-            self._raise(rc)
-        return q_out, k_out
+        q_out, k_out = (None, None) if out is None else out
+        if out is not None and q_out is None:
+            raise ValueError("out must be (q_out, k_out), k_out None where k is None")
+        return ops.rope(engine, q, k, table, layout == "half", index, inverse, q_out, k_out)
 
 
 class EngineContexts:

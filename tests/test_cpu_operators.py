@@ -2,6 +2,7 @@
 cases of perf/operators.py are made of."""
 import ctypes as C
 import random
+import struct
 import subprocess
 
 import pytest
@@ -11,20 +12,31 @@ from ecad_amd import _lib as L
 from ecad_amd.engine import EcadEngine
 
 
-class _NoLibrary:
-    """Stands in for the shared library: a refused call must not reach it."""
+class _Calls:
+    """Stands in for the shared library: five entry points that say that they were called (a refused call does not get that far)."""
 
-    def __getattr__(self, name):
-        def call(*args):
-            raise AssertionError(f"{name} was called")
+    def __init__(self):
+        P, I, I64, D = C.c_void_p, C.c_int, C.c_int64, C.c_double
+        prototypes = {"quantize_int8": [P, P, I64, P, I64, P, I, I, P], "gemm_int8": [P, P, P], "gate_norm": [P, P, P], "rope_table": [P, P, I, P, I, I, I, D, D, D, D, D, P, P], "rope": [P, P, P]}
+        self.last = C.create_string_buffer(64)
+        self.kept = []
+        for name, types in prototypes.items():
+            def call(*args, name=name):
+                self.last.value = f"{name} was called".encode()
+                return L.ECAD_E_HIP
 
-        return call
+            self.kept.append(C.CFUNCTYPE(I, *types)(call))
+        self.kept.append(C.CFUNCTYPE(P, P)(lambda handle: C.addressof(self.last)))
+        self.addresses = tuple(C.cast(f, P).value for f in self.kept)
 
 
 @pytest.fixture
 def eng():
+    """An engine without a device: CPU tensors are 'its' tensors, and a call that passes the checks ends in a RuntimeError that names it."""
+    calls, ops = _Calls(), L.load_ops()
     e = object.__new__(EcadEngine)
-    e.lib, e._h, e.dtype, e.device, e.cfg = _NoLibrary(), C.c_void_p(), torch.float16, torch.device("cpu"), L.EcadModelCfg()
+    e._h, e.cfg, e.calls = C.c_void_p(), L.EcadModelCfg(), calls
+    e._ops = ops, ops.engine(calls.addresses, 1 << 20, L.ECAD_DTYPE_F16, -1, lambda index: 0)
     return e
 
 
@@ -59,6 +71,8 @@ def test_gemm_refusals(eng):
         (dict(w=i8(7, 41)), "w must have shape"),
         (dict(sa=f32(4)), "a_scale"),
         (dict(sw=None), "needed"),
+        (dict(a=None), "a is needed"),
+        (dict(w=[1]), "must be a tensor, got list"),
         (dict(bias=f16(7)), "bias"),
         (dict(kernel="fast"), "unknown"),
         (dict(resid=f16(3, 7)), "epilogue 3"),
@@ -138,23 +152,28 @@ class _Packed:
         self.data = layout.pack(*(values.get(n) or 0 for n in names))
 
 
+# the argument records of include/ecad_hip.h: members in the header's order, and their struct codes (P pointer, q int64, i int32, f float; no padding)
 GEMM = "A lda a_scale W ldw w_scale bias out ldo resid ldr resid_out ldro gate_table gate_mod gate_mod_stride M N K epi rows_per_batch kernel".split()
 NORM = ("h ldh y ldy h_out ldho n_out ldn q ldq q_scale post_weight pre_weight gate_table gate_mod gate_mod_stride table_shift table_scale mod_shift mod_scale mod_stride "
         "M D rows_per_batch post pre reserved resid_scale eps").split()
 HEADS = "x out sample token head out_sample out_token out_head H".split()
+_HEADS = "PPqqqqqqq"
+INT8_GEMM_CODES = struct.Struct("PqPPqPPPqPqPqPPqiiiiii")
+GATE_NORM_CODES = struct.Struct("PqPqPqPqPqPPPPPqPPPPqiiiiiiff")
+ROPE_CODES = struct.Struct(_HEADS + _HEADS + "PPqiiiiiiii")
 ROPE = [f"{t}.{n}" for t in "qk" for n in HEADS] + "table index index_stride B S D rot table_rows half inverse reserved".split()
 
 
 def _Gemm(**v):
-    return _Packed(L.INT8_GEMM, GEMM, **v)
+    return _Packed(INT8_GEMM_CODES, GEMM, **v)
 
 
 def _Norm(**v):
-    return _Packed(L.GATE_NORM, NORM, **v)
+    return _Packed(GATE_NORM_CODES, NORM, **v)
 
 
 def _Rope(q, k, **v):
-    return _Packed(L.ROPE, ROPE, **{f"q.{n}": x for n, x in q.items()}, **{f"k.{n}": x for n, x in k.items()}, **v)
+    return _Packed(ROPE_CODES, ROPE, **{f"q.{n}": x for n, x in q.items()}, **{f"k.{n}": x for n, x in k.items()}, **v)
 
 
 class _Table(C.Structure):
@@ -247,13 +266,12 @@ def test_library_refusals_rope(library):
 
 
 def test_struct_layouts_match_the_header():
-    """The records that the binding packs by struct: sizes and offsets as the C compiler lays out include/ecad_hip.h."""
-    import struct
+    """The records of these tests and of anyone who binds the library without a C compiler: sizes and offsets as the C compiler lays out include/ecad_hip.h."""
     import tempfile
     from pathlib import Path
 
     root = Path(__file__).resolve().parents[1]
-    records = {"EcadInt8Gemm": (L.INT8_GEMM, GEMM), "EcadGateNorm": (L.GATE_NORM, NORM), "EcadRope": (L.ROPE, ROPE)}
+    records = {"EcadInt8Gemm": (INT8_GEMM_CODES, GEMM), "EcadGateNorm": (GATE_NORM_CODES, NORM), "EcadRope": (ROPE_CODES, ROPE)}
     with tempfile.TemporaryDirectory() as d:
         src = Path(d) / "t.c"
         body = "".join(f'printf("%zu", sizeof({r})); ' + "".join(f'printf(" %zu", offsetof({r}, {n}));' for n in names) + ' printf("\\n");' for r, (_, names) in records.items())
@@ -287,6 +305,52 @@ def test_gradients_are_refused_while_they_are_recorded(eng):
         eng.op_gate_norm(f16(4, 16), x)
     with pytest.raises(ValueError, match="gradient"):
         eng.op_gate_norm(f16(4, 16), pre_weight=torch.ones(16, requires_grad=True))
-    eng._stream = lambda: 0
-    with torch.no_grad(), pytest.raises(AssertionError, match="ecad_op_gate_norm was called"):
+    with torch.no_grad(), pytest.raises(RuntimeError, match="gate_norm was called"):
         eng.op_gate_norm(f16(4, 16), x, pre_weight=torch.ones(16, requires_grad=True))
+
+
+def test_calls_that_fit_reach_the_library(eng):
+    a, w, sa, sw, r = i8(3, 40), i8(7, 40), f32(3), f32(7), f16(3, 7)
+    t, q, k, at = f32(3, 8, 2), f16(2, 3, 4, 16), f16(2, 3, 2, 20)[..., :16], torch.zeros(3, dtype=torch.int32)
+    for name, call in [
+        ("quantize_int8", lambda: eng.op_quantize_int8(f16(4, 9)[:, 1:])),
+        ("quantize_int8", lambda: eng.op_quantize_int8(f16(4, 8), out=(i8(4, 8), f32(4)))),
+        ("gemm_int8", lambda: eng.op_gemm_int8(1, a, sa, w, sw, f32(7), out=f16(3, 9)[:, :7], kernel="tile64")),
+        ("gemm_int8", lambda: eng.op_gemm_int8(3, a, sa, w, sw, resid=r, gate_table=f32(7), gate_mod=f16(2, 20)[:, 3:10], rows_per_batch=2)),
+        ("gate_norm", lambda: eng.op_gate_norm(f16(4, 8), f16(4, 8), pre="none", post="rms", post_weight=f32(8))),
+        ("gate_norm", lambda: eng.op_gate_norm(f16(4, 8), quantize=True, out_n=(i8(4, 8), f32(4)))),
+        ("rope_table", lambda: eng.op_rope_table(at, 16)),
+        ("rope_table", lambda: eng.op_rope_table(f32(5, 3), [16, 56, 56], scaling="yarn", factor=2, original_length=64, out=f32(5, 64, 2))),
+        ("rope", lambda: eng.op_rope(q, k, t, index=at)),
+        ("rope", lambda: eng.op_rope(q, None, t, layout="half", index=at.expand(2, 3), inverse=True, out=(q, None))),
+    ]:
+        with pytest.raises(RuntimeError, match=f"^{name} was called"):
+            call()
+
+
+def test_wrong_kinds_of_arguments(eng):
+    for call in [lambda: eng.op_gate_norm(f16(4, 8), rows_per_batch="2"), lambda: eng.op_gate_norm(f16(4, 8), eps="small"), lambda: eng.op_gemm_int8(None, i8(3, 40), f32(3), i8(7, 40), f32(7)),
+                 lambda: eng.op_rope_table(f32(5), ("16",))]:
+        with pytest.raises(TypeError):
+            call()
+    with pytest.raises(ValueError, match="out of range"):
+        eng.op_gate_norm(f16(4, 8), rows_per_batch=1 << 40)
+    eng._ops = eng._ops[0], None
+    with pytest.raises(RuntimeError, match="closed"):
+        eng.op_quantize_int8(f16(4, 8))
+    with pytest.raises(RuntimeError, match="closed"):
+        eng._ops = None
+        eng.op_quantize_int8(f16(4, 8))
+
+
+def test_native_calls_keep_reference_counts(eng):
+    import sys
+
+    x, out = f16(4, 16), (i8(4, 16), f32(4))
+    before = [sys.getrefcount(o) for o in (x, out, *out, eng._ops[1], None)][:-1]
+    for _ in range(50):
+        with pytest.raises(RuntimeError):
+            eng.op_quantize_int8(x, out=out)
+        with pytest.raises(ValueError):
+            eng.op_gate_norm(x, x[:2])
+    assert [sys.getrefcount(o) for o in (x, out, *out, eng._ops[1], None)][:-1] == before
