@@ -32,19 +32,21 @@ struct GateNormArgs {
   float resid_scale, eps;
 };
 
-// mean (layer) and 1 / sqrt(. + eps) of the values of a row that is spread over WAVES waves, CH pieces per lane; lanes and pieces beyond the row hold zeros.
-// RAGGED: the row's last piece is not whole.
+// Layer: takes the mean off the values of a row that is spread over WAVES waves, CH pieces per lane.  Returns 1 / sqrt(mean square + eps).  Pieces and lanes beyond the row
+// hold zeros before (and less the mean behind: whoever multiplies them does so with zeros).  RAGGED: the row's last piece is not whole.
 template <int WAVES, int CH, bool RAGGED>
-ECAD_DEV void row_statistics(const float (&x)[CH][8], int kind, int first, int D, float eps, unsigned (*scratch)[WAVES], int& turn, float& mean, float& rstd) {
-  const float inv_d = 1.0f / (float)D;
-  mean = 0.f;
+ECAD_DEV float row_statistics(float (&x)[CH][8], int kind, int first, int D, float inv_d, float eps, unsigned (*scratch)[WAVES], int& turn) {
   if (kind == NORM_LAYER) {
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < CH; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum += x[i][e];
-    mean = row_all<WAVES>(sum, AddOp{}, scratch, turn) * inv_d;
+    const float mean = row_all<WAVES>(sum, AddOp{}, scratch, turn) * inv_d;
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[i][e] -= mean;
   }
   float sq = 0.f;
 #pragma unroll
@@ -53,12 +55,12 @@ ECAD_DEV void row_statistics(const float (&x)[CH][8], int kind, int first, int D
     float part = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float d = RAGGED && e >= left ? 0.f : x[i][e] - mean;
+      const float d = RAGGED && e >= left ? 0.f : x[i][e];
       part += d * d;
     }
     sq += left > 0 ? part : 0.f;
   }
-  rstd = 1.0f / sqrtf(row_all<WAVES>(sq, AddOp{}, scratch, turn) * inv_d + eps);
+  return 1.0f / sqrtf(row_all<WAVES>(sq, AddOp{}, scratch, turn) * inv_d + eps);
 }
 
 template <typename T, bool RAGGED> ECAD_DEV void row_store(T* p, const Pack8& v, int left) {
@@ -80,6 +82,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void gate_norm_kerne
   int turn = 0;
   float G[HOLD ? CH : 1][8], A[HOLD ? CH : 1][8], B[HOLD ? CH : 1][8];
   int have = -1;  // the sample that G, A, B belong to
+  const float inv_d = 1.0f / (float)p.D;
   const int64_t row0 = ((int64_t)blockIdx.x * SLOTS + slot) * p.rows_per_group;
   // rows_per_group and M are the same for all waves of a row: they leave the loop together (the barriers inside are a row's own where WAVES > 1)
   const int64_t end = row0 + p.rows_per_group < p.M ? row0 + p.rows_per_group : p.M;
@@ -155,26 +158,31 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void gate_norm_kerne
 #pragma unroll
     for (int i = 0; i < CH; ++i) unpack8<T>(row_piece<RAGGED>(hv[i], first + i * WAVES * 512, p.D), x[i]);
     if (p.y) {
-      float u[CH][8], mean = 0.f, rstd = 1.f;
+      float u[CH][8];
 #pragma unroll
       for (int i = 0; i < CH; ++i) unpack8<T>(row_piece<RAGGED>(yv[i], first + i * WAVES * 512, p.D), u[i]);
       if (row + 1 < end) fetch(row + 1);
-      if (p.post) row_statistics<WAVES, CH, RAGGED>(u, p.post, first, p.D, p.eps, scratch, turn, mean, rstd);
+      if (p.post) {
+        const float rstd = row_statistics<WAVES, CH, RAGGED>(u, p.post, first, p.D, inv_d, p.eps, scratch, turn);
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) u[i][e] *= rstd;
+      }
       T* ho = reinterpret_cast<T*>(p.h_out) + row * p.ldho;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int c = first + i * WAVES * 512, at = HOLD ? i : 0;
         if constexpr (!HOLD) channels(i, 0, 1);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = p.resid_scale * x[i][e] + (u[i][e] - mean) * rstd * G[at][e];
+        for (int e = 0; e < 8; ++e) x[i][e] = __builtin_fmaf(u[i][e], G[at][e], p.resid_scale * x[i][e]);
         row_store<T, RAGGED>(ho + c, pack8<T>(x[i]), p.D - c);
       }
     } else if (row + 1 < end) {
       fetch(row + 1);
     }
     if (p.pre == NORM_NONE) continue;
-    float mean, rstd;
-    row_statistics<WAVES, CH, RAGGED>(x, p.pre, first, p.D, p.eps, scratch, turn, mean, rstd);
+    const float rstd = row_statistics<WAVES, CH, RAGGED>(x, p.pre, first, p.D, inv_d, p.eps, scratch, turn);
     Pack8 nv[CH];
     u16x2 m = {0, 0};
 #pragma unroll
@@ -182,20 +190,19 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void gate_norm_kerne
       const int at = HOLD ? i : 0;
       if constexpr (!HOLD) channels(i, 0, 2);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][e] = (x[i][e] - mean) * rstd * A[at][e] + B[at][e];
+      for (int e = 0; e < 8; ++e) x[i][e] = __builtin_fmaf(x[i][e] * rstd, A[at][e], B[at][e]);
       nv[i] = pack8<T>(x[i]);
     }
     if (p.q) {
 #pragma unroll
       for (int i = 0; i < CH; ++i) m = max_bits(m, nv[i]);
-      const unsigned bits = row_all<WAVES>(fold_bits(m), MaxOp{}, scratch, turn);
-      const Int8Scale k = int8_scale<T>(bits);
+      const Int8Scale k = int8_scale<T>(__builtin_amdgcn_readfirstlane(row_all<WAVES>(fold_bits(m), MaxOp{}, scratch, turn)));
       if (lane == 0) p.q_scale[row] = k.s;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int c = first + i * WAVES * 512;
         unpack8<T>(nv[i], x[i]);
-        store_int8_piece(p.q + row * p.ldq + c, int8_piece(x[i], k), p.D - c);
+        store_int8_piece<RAGGED>(p.q + row * p.ldq + c, int8_piece(x[i], k), p.D - c);
       }
     } else {
       T* no = reinterpret_cast<T*>(p.n_out) + row * p.ldn;
@@ -236,15 +243,14 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void quantize_rows_k
     v[i] = row_piece<RAGGED>(v[i], (lane + i * WAVES * 64) * 8, p.K);
     m = max_bits(m, v[i]);
   }
-  const unsigned bits = row_all<WAVES>(fold_bits(m), MaxOp{}, scratch, turn);
-  const Int8Scale k = int8_scale<T>(bits);
+  const Int8Scale k = int8_scale<T>(__builtin_amdgcn_readfirstlane(row_all<WAVES>(fold_bits(m), MaxOp{}, scratch, turn)));
   if (lane == 0) p.scale[row] = k.s;
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int c = (lane + i * WAVES * 64) * 8;
     float x[8];
     unpack8<T>(v[i], x);
-    store_int8_piece(p.q + row * p.ldq + c, int8_piece(x, k), p.K - c);
+    store_int8_piece<RAGGED>(p.q + row * p.ldq + c, int8_piece(x, k), p.K - c);
   }
 }
 

@@ -186,9 +186,9 @@ int choose_int8(const OpCtx& ctx, const Int8GemmArgs& a) {
     int id, bm, bn, per_cu, fewest;
     double fixed, stage;
   };
-  static const Tile tiles[] = {{ECAD_I8_K_TILE64, 64, 64, 2, 0, 2.8, 0.44},      {ECAD_I8_K_TILE128, 128, 128, 2, 0, 5.0, 1.2}, {ECAD_I8_K_TILE144, 256, 144, 1, Int8Wide<144>::fewest, 7.0, 1.0},
+  static const Tile tiles[] = {{ECAD_I8_K_TILE64, 64, 64, 2, 0, 2.8, 0.44}, {ECAD_I8_K_TILE64_K2, 64, 64, 1, 0, 2.9, 0.32}, {ECAD_I8_K_TILE128, 128, 128, 2, 0, 5.0, 1.2}, {ECAD_I8_K_TILE144, 256, 144, 1, Int8Wide<144>::fewest, 7.0, 1.0},
                                {ECAD_I8_K_TILE256, 256, 256, 1, Int8Wide<256>::fewest, 6.6, 1.6}, {ECAD_I8_K_TILE288, 256, 288, 1, Int8Wide<288>::fewest, 8.0, 1.72}};
-  if (a.M <= 32) return ECAD_I8_K_ROWS;
+  if (a.M <= 32) return ECAD_I8_K_ROWS;  // 32 rows: 6912 x 1152 5.3 us (64 x 64 tiles 5.8), 1152 x 4608 7.9 (11.5), 4096 x 8192 14.0 (18.5); 64 rows: 7.6 (5.8), 12.2 (11.4), 21.0 (18.5)
   const int stages = (a.K + 127) / 128;
   int best = ECAD_I8_K_TILE64;
   double least = 1e300;
@@ -202,13 +202,15 @@ int choose_int8(const OpCtx& ctx, const Int8GemmArgs& a) {
 }
 
 template <typename T, int EPI> int gemm_int8_t(const OpCtx& ctx, const Int8GemmArgs& a, int kernel, OpStatus& st) {
-  if (kernel == ECAD_I8_K_ROWS && a.M > 64) return refuse(st, ECAD_E_UNSUPPORTED, "gemm_int8: the few-rows kernel takes up to 64 rows, got %d", a.M);
+  if (kernel == ECAD_I8_K_ROWS && a.M > 32) return refuse(st, ECAD_E_UNSUPPORTED, "gemm_int8: the few-rows kernel takes up to 32 rows, got %d", a.M);
   switch (kernel == ECAD_I8_K_AUTO ? choose_int8(ctx, a) : kernel) {
     case ECAD_I8_K_ROWS: {
       const dim3 grid((unsigned)((a.N + 15) / 16));
-      if (a.M <= 16) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 1, 8, EPI>), grid, dim3(512), 0, ctx.stream, a);
-      else if (a.M <= 32) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 2, 8, EPI>), grid, dim3(512), 0, ctx.stream, a);
-      else hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 4, 8, EPI>), grid, dim3(512), 0, ctx.stream, a);
+      const bool narrow = (int64_t)grid.x < 2 * (int64_t)ctx.num_cus;  // few workgroups: more of K in flight at a time
+      if (a.M <= 16 && narrow) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 1, 16, EPI>), grid, dim3(1024), 0, ctx.stream, a);
+      else if (a.M <= 16) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 1, 8, EPI>), grid, dim3(512), 0, ctx.stream, a);
+      else if (narrow) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 2, 16, EPI>), grid, dim3(1024), 0, ctx.stream, a);
+      else hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 2, 8, EPI>), grid, dim3(512), 0, ctx.stream, a);
       return launched(st, "gemm_int8");
     }
     case ECAD_I8_K_TILE64: return launch_tile<T, EPI, 64, 64, 2, 2, 1, 4>(ctx, a, st);

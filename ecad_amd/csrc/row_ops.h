@@ -176,7 +176,8 @@ ECAD_DEV u32x2 int8_piece(const float (&x)[8], const Int8Scale& k) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float d = __builtin_fmaf(INT8_MAGIC - m[e], k.s, x[e]), step = d > 0.f ? 1.f : -1.f;
-        if (fabsf(d) > k.half || (fabsf(d) == k.half && (__builtin_bit_cast(unsigned, m[e]) & 1))) m[e] += step;
+        const bool other = fabsf(d) > k.half || (fabsf(d) == k.half && (__builtin_bit_cast(unsigned, m[e]) & 1));
+        m[e] += other ? step : 0.f;
       }
     }
   } else {
@@ -185,10 +186,10 @@ ECAD_DEV u32x2 int8_piece(const float (&x)[8], const Int8Scale& k) {
   }
   return (u32x2){gather_bytes(m), gather_bytes(m + 4)};
 }
-ECAD_DEV void store_int8_piece(int8_t* p, u32x2 v, int n) {  // rows of 8-bit values start on 16 bytes
-  if (n >= 8) {
+template <bool RAGGED> ECAD_DEV void store_int8_piece(int8_t* p, u32x2 v, int n) {  // rows of 8-bit values start on 16 bytes
+  if (n >= (RAGGED ? 8 : 1)) {
     *reinterpret_cast<u32x2*>(p) = v;
-  } else {
+  } else if (RAGGED) {
 #pragma unroll
     for (int e = 0; e < 7; ++e)
       if (e < n) p[e] = (int8_t)(v[e >> 2] >> (8 * (e & 3)));

@@ -294,7 +294,7 @@ int ecad_op_quantize_int8(EcadEngine* e, const void* x, int64_t ldx, int8_t* q, 
 /* o[M,N] = act(a_scale[m] w_scale[n] (A[M,K] @ W[N,K]^T) + bias[n]), the sum in 32-bit integers; epi as ecad_op_gemm: 0 none, 1 GELU(tanh), 2 SiLU, 3 cache write and
  * gated residual: out = o rounded (may be NULL), resid_out = resid + (gate_table[n] + gate_mod[m / rows_per_batch][n]) * out (either or both NULL: gate 1 where
  * neither is given; resid_out may be resid).  kernel: ECAD_I8_K_AUTO, or one by name (the same bits; ECAD_E_UNSUPPORTED if it cannot take the shape). */
-enum { ECAD_I8_K_AUTO = 0, ECAD_I8_K_ROWS = 1 /* up to 64 rows: operands straight to registers, K over the waves */, ECAD_I8_K_TILE64 = 2, ECAD_I8_K_TILE128 = 3, ECAD_I8_K_TILE144 = 4 /* 256 x 144 */,
+enum { ECAD_I8_K_AUTO = 0, ECAD_I8_K_ROWS = 1 /* up to 32 rows: operands straight to registers, K over the waves */, ECAD_I8_K_TILE64 = 2, ECAD_I8_K_TILE128 = 3, ECAD_I8_K_TILE144 = 4 /* 256 x 144 */,
        ECAD_I8_K_TILE256 = 5, ECAD_I8_K_TILE288 = 6 /* 256 x 288 */,
        ECAD_I8_K_TILE64_K2 = 7 /* 64 x 64, two groups of waves along K */ };
 typedef struct EcadInt8Gemm {

@@ -114,7 +114,7 @@ SHAPES = [(1, 1, 1), (1, 17, 16), (2, 6912, 1152), (16, 100, 63), (17, 33, 65), 
 
 def takes(kernel, M, K):
     """What the named kernels refuse."""
-    return not (kernel == "rows" and M > 64 or kernel in ("tile256", "tile288") and K < 256 or kernel == "tile144" and K < 384)
+    return not (kernel == "rows" and M > 32 or kernel in ("tile256", "tile288") and K < 256 or kernel == "tile144" and K < 384)
 
 
 def product64(a, sa, w, sw, bias):
@@ -622,7 +622,7 @@ def test_refusals_reach_the_caller():
     with pytest.raises(ValueError, match="32768"):
         eng.op_gate_norm(h, pre="rms")
     with pytest.raises(ValueError, match="few-rows"):
-        eng.op_gemm_int8(0, int8_rows(65, 16, 1), torch.ones(65, device="cuda"), int8_rows(4, 16, 2), torch.ones(4, device="cuda"), kernel="rows")
+        eng.op_gemm_int8(0, int8_rows(33, 16, 1), torch.ones(33, device="cuda"), int8_rows(4, 16, 2), torch.ones(4, device="cuda"), kernel="rows")
     with pytest.raises(ValueError, match="multiple of 16"):
         eng.op_gemm_int8(0, torch.zeros(4, 40, dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda"), int8_rows(4, 40, 2), torch.ones(4, device="cuda"))
     with pytest.raises(ValueError, match="table has 3 rows"):
