@@ -117,6 +117,11 @@ int64_t rows(const Engine& e, const Tensor& t, const char* name, at::ScalarType 
   check(e, t, name, type, {M, N}, LAST);
   return M > 1 ? t.stride(0) : N;
 }
+// the stride of 8-bit rows (one row: the next multiple of 16)
+int64_t int8_rows(const Engine& e, const Tensor& t, const char* name, int64_t M, int64_t N) {
+  check(e, t, name, at::kChar, {M, N}, LAST);
+  return M > 1 ? t.stride(0) : (N + 15) & ~(int64_t)15;
+}
 const float* vector(const Engine& e, PyObject* o, const char* name, int64_t n) {
   const Tensor* t = maybe(o, name);
   if (!t) return nullptr;
@@ -181,9 +186,7 @@ Int8Out out_int8(const Engine& e, PyObject* given, const char* name, int64_t M, 
     if (!PyTuple_Check(given) || PyTuple_GET_SIZE(given) != 2) refuse("%s must be a pair (q, scale)", name);
     o.q.given = PyTuple_GET_ITEM(given, 0);
     o.scale.given = PyTuple_GET_ITEM(given, 1);
-    const Tensor& q = tensor(o.q.given, "q");
-    rows(e, q, "q", at::kChar, M, N);
-    o.stride = q.stride(0);
+    o.stride = int8_rows(e, tensor(o.q.given, "q"), "q", M, N);
     if (!vector(e, o.scale.given, "scale", M)) refuse("%s must come with its scale", name);
   } else {
     o.stride = (N + 15) & ~(int64_t)15;
@@ -268,9 +271,7 @@ PyObject* gemm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t M = A.size(0), K = A.size(1), N = W.size(0);
     EcadInt8Gemm g{};
     g.epi = integer32(a[1], "epi");
-    rows(e, A, "a", at::kChar, M, K);
-    rows(e, W, "w", at::kChar, N, K);
-    g.A = static_cast<const int8_t*>(A.data_ptr()), g.lda = A.stride(0), g.W = static_cast<const int8_t*>(W.data_ptr()), g.ldw = W.stride(0);
+    g.A = static_cast<const int8_t*>(A.data_ptr()), g.lda = int8_rows(e, A, "a", M, K), g.W = static_cast<const int8_t*>(W.data_ptr()), g.ldw = int8_rows(e, W, "w", N, K);
     g.a_scale = vector(e, a[3], "a_scale", M), g.w_scale = vector(e, a[5], "w_scale", N), g.bias = vector(e, a[6], "bias", N);
     if (a[3] == Py_None || a[5] == Py_None) refuse("a_scale and w_scale are needed");
     PyObject *resid = a[7], *out = a[11], *resid_out = a[12];

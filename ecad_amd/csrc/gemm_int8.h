@@ -361,7 +361,11 @@ __global__ __launch_bounds__(256) void gemm_int8_wide_kernel(const Int8GemmArgs 
         });
       });
     }
-    asm volatile("s_nop 15\n\ts_nop 7");  // and the accumulators are read next
+    // and the accumulators are read next, the ninth column's by ordinary instructions: tied to the wait by the operands
+    if constexpr (G::ninth)
+      asm volatile("s_nop 15\n\ts_nop 7" : "+v"(c8[0]), "+v"(c8[1]), "+v"(c8[2]), "+v"(c8[3]), "+v"(c8[4]), "+v"(c8[5]), "+v"(c8[6]), "+v"(c8[7]));
+    else
+      asm volatile("s_nop 15\n\ts_nop 7");
   }
   int8_epilogue<T, BM, BN, FM, FN, 256, EPI>(p, smem, m0, n0, wm0, wn0, true, [&](auto ic, auto jc) -> i32x4 {
     constexpr int i = decltype(ic)::value, j = decltype(jc)::value;

@@ -182,6 +182,20 @@ def test_gemm_gated_residual(dtype_name, M, N, K, gate):
         assert torch.equal(apart, kept)
 
 
+def test_one_row_takes_any_stride():
+    """A single 8-bit row (a user's own, without padding behind it) as activation, as weight and as the quantiser's output."""
+    eng = small_engine("float16")
+    q = int8_rows(1, 40, 1).clone(memory_format=torch.contiguous_format)
+    assert q.stride() == (40, 1)
+    one = torch.ones(1, device="cuda")
+    out = eng.op_gemm_int8(0, q, one * 1e-3, q, one)
+    near(out, (q.double() ** 2).sum().view(1, 1) * one.double() * (one * 1e-3).double(), 2.0**-20)
+    x, s = rand(1, 41, seed=1, dtype=torch.float16), torch.empty(1, device="cuda")
+    buf = torch.full((1, 41), 99, dtype=torch.int8, device="cuda")
+    eng.op_quantize_int8(x, out=(buf, s))
+    assert all(torch.equal(a, b) for a, b in zip((buf, s), quantized(x)))
+
+
 def test_gemm_largest_sums():
     """All operands at -128 over the longest K: the sum is K 2^14 = 2147467264, just inside 32 bits."""
     eng = small_engine("bfloat16")
