@@ -136,7 +136,35 @@ ECAD_DEV void int8_epilogue(const Int8GemmArgs& p, char* smem, int m0, int n0, i
     });
     return;
   }
+  // the rolled loop in batches of U pieces a thread: a batch's residual and gates are requested before the batch in front of it is worked on, the first one before
+  // the sums are staged (one piece at a time each read was waited for behind the write of the piece before: 8192 x 1152 x 4608 52.5 us)
+  constexpr int CPR = BN / 8, PIECES = BM * CPR / NT, U = PIECES % 6 == 0 ? 6 : (PIECES % 4 == 0 ? 4 : PIECES);
+  static_assert(BM * CPR % NT == 0 && PIECES % U == 0, "whole batches");
+  struct Batch {
+    Pack8 h[U], gm[U];
+    float gt[U][8];
+  };
+  auto where = [&](int b, int u, int& r, int& c) {
+    const int it = (b * U + u) * NT + (int)threadIdx.x;
+    r = it / CPR, c = (it - r * CPR) * 8;
+  };
+  auto request = [&](int b, Batch& x) {
+    if constexpr (EPI == I8_RESID) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        int r, c;
+        where(b, u, r, c);
+        const int m = m0 + r, n = n0 + c, left = p.N - n;
+        if (m >= p.M || left <= 0) continue;
+        x.h[u] = load_piece<T>(reinterpret_cast<const T*>(p.resid) + (int64_t)m * p.ldr + n, left);
+        if (p.gate_table) load_floats(p.gate_table + n, left, x.gt[u]);
+        if (p.gate_mod) x.gm[u] = load_piece<T>(reinterpret_cast<const T*>(p.gate_mod) + (int64_t)(m / p.rows_per_batch) * p.gate_stride + n, left);
+      }
+    }
+  };
   T* tile = reinterpret_cast<T*>(smem);
+  Batch batch;
+  request(0, batch);
   if (holds) static_for<FN>([&](auto jc) {
     constexpr int j = decltype(jc)::value;
     const int n = n0 + wn0 + 16 * j + 4 * g;
@@ -144,31 +172,30 @@ ECAD_DEV void int8_epilogue(const Int8GemmArgs& p, char* smem, int m0, int n0, i
     static_for<FM>([&](auto ic) { *reinterpret_cast<u32x2*>(tile + (wm0 + 16 * decltype(ic)::value + l15) * CS + wn0 + 16 * j + 4 * g) = packed(ic, jc, sw, bias); });
   });
   __syncthreads();
-  constexpr int CPR = BN / 8;
-  for (int it = threadIdx.x; it < BM * CPR; it += NT) {
-    const int r = it / CPR, c = (it - r * CPR) * 8, m = m0 + r, n = n0 + c, left = p.N - n;
-    if (m >= p.M || left <= 0) continue;
-    const Pack8 v = lds_read16(tile + r * CS + c);
-    if (EPI != I8_RESID || p.out) store_piece<T>(reinterpret_cast<T*>(p.out) + (int64_t)m * p.ldo + n, v, left);
-    if constexpr (EPI == I8_RESID) {
-      float o[8], h[8], gate[8];
-      unpack8<T>(v, o);
-      unpack8<T>(load_piece<T>(reinterpret_cast<const T*>(p.resid) + (int64_t)m * p.ldr + n, left), h);
-      if (p.gate_table) {
-        load_floats(p.gate_table + n, left, gate);
-      } else {
+  for (int b = 0; b < PIECES / U; ++b) {
+    const Batch now = batch;
+    if (b + 1 < PIECES / U) request(b + 1, batch);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) gate[e] = p.gate_mod ? 0.f : 1.f;
+    for (int u = 0; u < U; ++u) {
+      int r, c;
+      where(b, u, r, c);
+      const int m = m0 + r, n = n0 + c, left = p.N - n;
+      if (m >= p.M || left <= 0) continue;
+      const Pack8 v = lds_read16(tile + r * CS + c);
+      if (EPI != I8_RESID || p.out) store_piece<T>(reinterpret_cast<T*>(p.out) + (int64_t)m * p.ldo + n, v, left);
+      if constexpr (EPI == I8_RESID) {
+        float o[8], h[8], gm[8];
+        unpack8<T>(v, o);
+        unpack8<T>(now.h[u], h);
+        unpack8<T>(now.gm[u], gm);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float gate = p.gate_table ? now.gt[u][e] : (p.gate_mod ? 0.f : 1.f);
+          if (p.gate_mod) gate += gm[e];
+          h[e] = pinned(__builtin_fmaf(gate, o[e], h[e]));
+        }
+        store_piece<T>(reinterpret_cast<T*>(p.resid_out) + (int64_t)m * p.ldro + n, pack8<T>(h), left);
       }
-      if (p.gate_mod) {
-        float gm[8];
-        unpack8<T>(load_piece<T>(reinterpret_cast<const T*>(p.gate_mod) + (int64_t)(m / p.rows_per_batch) * p.gate_stride + n, left), gm);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) gate[e] += gm[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) h[e] = pinned(__builtin_fmaf(gate[e], o[e], h[e]));
-      store_piece<T>(reinterpret_cast<T*>(p.resid_out) + (int64_t)m * p.ldro + n, pack8<T>(h), left);
     }
   }
 }
@@ -181,7 +208,7 @@ constexpr int int8_lds_bytes(int bm, int bn, int stages) {
 // chunks XOR-swizzled by (row >> 1) & 7 on the source side, so that the fragment reads (16 rows x 16 bytes) meet every bank once.  One barrier per step, STAGES steps in
 // a ring.  KW > 1 is for products of few tiles, whose time is the number of steps: the groups' sums meet in LDS (whole numbers: the same bits).
 template <typename T, int BM, int BN, int WM, int WN, int KW, int STAGES, int EPI>
-__global__ __launch_bounds__(WM * WN * KW * 64) void gemm_int8_kernel(const Int8GemmArgs p) {
+__global__ __launch_bounds__(WM * WN * KW * 64, 2) void gemm_int8_kernel(const Int8GemmArgs p) {
   constexpr int NG = WM * WN, NW = NG * KW, FM = BM / WM / 16, FN = BN / WN / 16;
   constexpr int A_BYTES = BM * 128, GROUP_BYTES = (BM + BN) * 128, STAGE_BYTES = KW * GROUP_BYTES;
   constexpr int PPG = (BM + BN) / 8, PPW = KW * PPG / NW;  // pieces per group and step, per wave
