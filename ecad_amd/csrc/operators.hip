@@ -178,24 +178,36 @@ template <typename T, int EPI, int BN> int launch_wide(const OpCtx& ctx, const I
 }
 
 // Which kernel: the one with the smallest estimated time, rounds of the tiles it needs over the chip times (what a round costs outside the K loop + its K stages), in
-// microseconds as measured with all CUs busy (fp16 / bf16 out, plain epilogue).  Against the measured times of 8192 x 4608 x 1152, 8192 x 1152 x 4608, 4096 x 3456 x 1152,
-// 2048 x 4608 x 1152, 1024 x 1152 x 1152, 601 x 1111 x 4001 and 8192 x 8192 x 4096 the estimate picks the fastest kernel each time (estimates within 25 %); e.g. 8192 x 4608 x
-// 1152: 288 columns (two whole rounds) 62 us, 256 columns (2.25 rounds) 73, 144 columns 74, 128 x 128 77, 64 x 64 122.
+// microseconds; a stage costs more the fuller the chip is (operands from L2, and the clock under load).  Fitted to the times below and thirteen other shapes: the pick is
+// the fastest kernel at 19 of 20 (8000 x 500 x 3000: 18 % off).  Measured, us, plain epilogue:
+//                        64 x 64   64 x 64, K over two   128 x 128   256 x 144   256 x 256   256 x 288
+//   601 x 1111 x 4001     16.5        13.1                32.9        39.9        60.9        64.0
+//   1024 x 1152 x 1152     7.3        10.7                10.8        13.1        18.9        19.4
+//   2048 x 4608 x 1152    30.4        44.6                24.8        17.6        21.1        23.8
+//   4096 x 3456 x 1152    44.8        67.1                28.1        30.2        23.0        24.7
+//   8192 x 4608 x 1152   111.4       171.5                64.3        62.1        61.1        52.3
+//   8192 x 1152 x 4608    83.5        95.8                69.7        39.4        48.4        52.8
+//   8192 x 8192 x 4096   502         614                 314         287         232         257
 int choose_int8(const OpCtx& ctx, const Int8GemmArgs& a) {
   struct Tile {
     int id, bm, bn, per_cu, fewest;
-    double fixed, stage;
+    double round, stage, full, least;  // a stage: stage + full * (share of the chip in use), at least `least`
   };
-  static const Tile tiles[] = {{ECAD_I8_K_TILE64, 64, 64, 2, 0, 2.8, 0.44}, {ECAD_I8_K_TILE64_K2, 64, 64, 1, 0, 2.9, 0.32}, {ECAD_I8_K_TILE128, 128, 128, 2, 0, 5.0, 1.2}, {ECAD_I8_K_TILE144, 256, 144, 1, Int8Wide<144>::fewest, 7.0, 1.0},
-                               {ECAD_I8_K_TILE256, 256, 256, 1, Int8Wide<256>::fewest, 6.6, 1.6}, {ECAD_I8_K_TILE288, 256, 288, 1, Int8Wide<288>::fewest, 8.0, 1.72}};
+  static const Tile tiles[] = {{ECAD_I8_K_TILE64, 64, 64, 2, 0, 2.0, 0.42, 0.06, 0},
+                               {ECAD_I8_K_TILE64_K2, 64, 64, 1, 0, 2.2, 0.25, 0.06, 0},
+                               {ECAD_I8_K_TILE128, 128, 128, 2, 0, 2.6, 0.75, 0.4, 0},
+                               {ECAD_I8_K_TILE144, 256, 144, 1, Int8Wide<144>::fewest, 7.0, 0.62, 0.25, 0},
+                               {ECAD_I8_K_TILE256, 256, 256, 1, Int8Wide<256>::fewest, 7.0, 0.5, 1.1, 1.1},
+                               {ECAD_I8_K_TILE288, 256, 288, 1, Int8Wide<288>::fewest, 8.0, 0.5, 1.35, 1.2}};
   if (a.M <= 32) return ECAD_I8_K_ROWS;  // 32 rows: 6912 x 1152 5.3 us (64 x 64 tiles 5.8), 1152 x 4608 7.9 (11.5), 4096 x 8192 14.0 (18.5); 64 rows: 7.6 (5.8), 12.2 (11.4), 21.0 (18.5)
   const int stages = (a.K + 127) / 128;
   int best = ECAD_I8_K_TILE64;
   double least = 1e300;
   for (const Tile& t : tiles) {
     if (a.K / 128 < t.fewest) continue;
-    const int64_t at_once = (int64_t)t.per_cu * ctx.num_cus;
-    const double us = (double)((tiles_of(a, t.bm, t.bn) + at_once - 1) / at_once) * (t.fixed + t.stage * stages);
+    const int64_t n = tiles_of(a, t.bm, t.bn), at_once = (int64_t)t.per_cu * ctx.num_cus, rounds = (n + at_once - 1) / at_once;
+    const double stage = t.stage + t.full * (double)n / (double)(rounds * at_once);
+    const double us = (double)rounds * (t.round + (stage > t.least ? stage : t.least) * stages);
     if (us < least) least = us, best = t.id;
   }
   return best;
