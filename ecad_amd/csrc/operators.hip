@@ -28,6 +28,9 @@ int launched(OpStatus& st, const char* what) {
   return e == hipSuccess ? ECAD_OK : refuse(st, ECAD_E_HIP, "%s: launch failed: %s", what, hipGetErrorString(e));
 }
 
+// threads of a launch are counted in 32 bits
+bool fits(int64_t blocks, int threads) { return blocks <= 0x7fffffff && blocks * threads <= 0xffffffffll; }
+
 bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 // more than 64 KiB of LDS has to be asked for once per kernel and device
@@ -110,10 +113,19 @@ constexpr int MAX_INT8_K = 131071;   // 128^2 K stays below 2^31
 
 // ---- 8-bit rows ----------------------------------------------------------------------------------------------------------------------------------------------
 
-template <typename T, int WAVES, int CH> int launch_quantize(const OpCtx& ctx, const QuantizeArgs& a, OpStatus& st) {
-  const dim3 grid((unsigned)(((int64_t)a.M + row_slots(WAVES) - 1) / row_slots(WAVES))), block(WAVES == 1 ? 256 : WAVES * 64);
-  if (a.K % 8) hipLaunchKernelGGL((quantize_rows_kernel<T, WAVES, CH, true>), grid, block, 0, ctx.stream, a);
-  else hipLaunchKernelGGL((quantize_rows_kernel<T, WAVES, CH, false>), grid, block, 0, ctx.stream, a);
+template <typename T, int WAVES, int CH> int launch_quantize(const OpCtx& ctx, const QuantizeArgs& whole, OpStatus& st) {
+  constexpr int slots = row_slots(WAVES), threads = WAVES == 1 ? 256 : WAVES * 64;
+  constexpr int64_t most = 0xffffffffll / threads * slots < 0x7fffffff ? 0xffffffffll / threads * slots : 0x7fffffff;  // rows of one launch
+  for (int64_t row = 0; row < whole.M; row += most) {
+    QuantizeArgs a = whole;
+    a.x = reinterpret_cast<const T*>(whole.x) + row * whole.ldx;
+    a.q += row * whole.ldq;
+    a.scale += row;
+    a.M = (int)(whole.M - row < most ? whole.M - row : most);
+    const dim3 grid((unsigned)(((int64_t)a.M + slots - 1) / slots));
+    if (a.K % 8) hipLaunchKernelGGL((quantize_rows_kernel<T, WAVES, CH, true>), grid, dim3(threads), 0, ctx.stream, a);
+    else hipLaunchKernelGGL((quantize_rows_kernel<T, WAVES, CH, false>), grid, dim3(threads), 0, ctx.stream, a);
+  }
   return launched(st, "quantize_int8");
 }
 template <typename T> int quantize_t(const OpCtx& ctx, const QuantizeArgs& a, OpStatus& st) {
@@ -163,7 +175,7 @@ int launch_int8(const OpCtx& ctx, const Int8GemmArgs& a, OpStatus& st, std::atom
   const int rc = allow_lds(done, (const void*)kernel, bytes, st);
   if (rc) return rc;
   const int64_t tiles = tiles_of(a, bm, bn);
-  if (tiles > 0x7fffffff) return refuse(st, ECAD_E_UNSUPPORTED, "gemm_int8: %lld tiles are more than one launch takes", (long long)tiles);
+  if (!fits(tiles, threads)) return refuse(st, ECAD_E_UNSUPPORTED, "gemm_int8: %lld tiles are more than one launch takes", (long long)tiles);
   hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(threads), bytes, ctx.stream, a);
   return launched(st, "gemm_int8");
 }
@@ -199,13 +211,14 @@ int choose_int8(const OpCtx& ctx, const Int8GemmArgs& a) {
                                {ECAD_I8_K_TILE144, 256, 144, 1, Int8Wide<144>::fewest, 7.0, 0.62, 0.25, 0},
                                {ECAD_I8_K_TILE256, 256, 256, 1, Int8Wide<256>::fewest, 7.0, 0.5, 1.1, 1.1},
                                {ECAD_I8_K_TILE288, 256, 288, 1, Int8Wide<288>::fewest, 8.0, 0.5, 1.35, 1.2}};
-  if (a.M <= 32) return ECAD_I8_K_ROWS;  // 32 rows: 6912 x 1152 5.3 us (64 x 64 tiles 5.8), 1152 x 4608 7.9 (11.5), 4096 x 8192 14.0 (18.5); 64 rows: 7.6 (5.8), 12.2 (11.4), 21.0 (18.5)
+  if (a.M <= 32 && fits(((int64_t)a.N + 15) / 16, 1024)) return ECAD_I8_K_ROWS;  // 32 rows: 6912 x 1152 5.3 us (64 x 64 tiles 5.8), 1152 x 4608 7.9 (11.5), 4096 x 8192 14.0 (18.5); 64 rows: 7.6 (5.8), 12.2 (11.4), 21.0 (18.5)
   const int stages = (a.K + 127) / 128;
   int best = ECAD_I8_K_TILE64;
   double least = 1e300;
   for (const Tile& t : tiles) {
-    if (a.K / 128 < t.fewest) continue;
-    const int64_t n = tiles_of(a, t.bm, t.bn), at_once = (int64_t)t.per_cu * ctx.num_cus, rounds = (n + at_once - 1) / at_once;
+    const int64_t n = tiles_of(a, t.bm, t.bn);
+    if (a.K / 128 < t.fewest || !fits(n, t.id == ECAD_I8_K_TILE64_K2 ? 512 : 256)) continue;
+    const int64_t at_once = (int64_t)t.per_cu * ctx.num_cus, rounds = (n + at_once - 1) / at_once;
     const double stage = t.stage + t.full * (double)n / (double)(rounds * at_once);
     const double us = (double)rounds * (t.round + (stage > t.least ? stage : t.least) * stages);
     if (us < least) least = us, best = t.id;
@@ -217,7 +230,8 @@ template <typename T, int EPI> int gemm_int8_t(const OpCtx& ctx, const Int8GemmA
   if (kernel == ECAD_I8_K_ROWS && a.M > 32) return refuse(st, ECAD_E_UNSUPPORTED, "gemm_int8: the few-rows kernel takes up to 32 rows, got %d", a.M);
   switch (kernel == ECAD_I8_K_AUTO ? choose_int8(ctx, a) : kernel) {
     case ECAD_I8_K_ROWS: {
-      const dim3 grid((unsigned)((a.N + 15) / 16));
+      const dim3 grid((unsigned)(((int64_t)a.N + 15) / 16));
+      if (!fits(grid.x, 1024)) return refuse(st, ECAD_E_UNSUPPORTED, "gemm_int8: %d columns are more than one launch of the few-rows kernel takes", a.N);
       const bool narrow = (int64_t)grid.x < 2 * (int64_t)ctx.num_cus;  // few workgroups: more of K in flight at a time
       if (a.M <= 16 && narrow) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 1, 16, EPI>), grid, dim3(1024), 0, ctx.stream, a);
       else if (a.M <= 16) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 1, 8, EPI>), grid, dim3(512), 0, ctx.stream, a);
@@ -280,6 +294,7 @@ int op_gemm_int8(const OpCtx& ctx, const EcadInt8Gemm& c, OpStatus& st) noexcept
   if ((c.out && c.M > 1 && c.ldo < c.N) || (c.epi == I8_RESID && c.M > 1 && (c.ldr < c.N || c.ldro < c.N))) return refuse(st, ECAD_E_INVALID, "gemm_int8: row strides of the outputs are shorter than %d", c.N);
   if (c.epi == I8_RESID && c.rows_per_batch < 1) return refuse(st, ECAD_E_INVALID, "gemm_int8: rows_per_batch must be at least 1");
   const bool gated = c.epi == I8_RESID;
+  if (gated && c.gate_mod_stride < 0) return refuse(st, ECAD_E_INVALID, "gemm_int8: a stride is negative");
   const int64_t samples = gated ? ((int64_t)c.M - 1) / c.rows_per_batch + 1 : 0;
   const Region out = matrix(c.out, c.M, c.N, c.ldo, 2), resid_out = matrix(gated ? c.resid_out : nullptr, c.M, c.N, c.ldro, 2), resid = matrix(gated ? c.resid : nullptr, c.M, c.N, c.ldr, 2);
   const Region in[] = {matrix(c.A, c.M, c.K, c.lda, 1), matrix(c.W, c.N, c.K, c.ldw, 1), vector(c.a_scale, c.M, 4), vector(c.w_scale, c.N, 4), vector(c.bias, c.N, 4),
@@ -313,6 +328,7 @@ int op_gate_norm(const OpCtx& ctx, const EcadGateNorm& c, OpStatus& st) noexcept
   if (!aligned(c.h, 2) || !aligned(c.y, 2) || !aligned(c.h_out, 2) || !aligned(c.n_out, 2) || !aligned(c.gate_mod, 2) || !aligned(c.mod_shift, 2) || !aligned(c.mod_scale, 2) || !aligned(c.post_weight, 4) ||
       !aligned(c.pre_weight, 4) || !aligned(c.gate_table, 4) || !aligned(c.table_shift, 4) || !aligned(c.table_scale, 4))
     return refuse(st, ECAD_E_INVALID, "gate_norm: pointers are not aligned to their type");
+  if (c.gate_mod_stride < 0 || c.mod_stride < 0) return refuse(st, ECAD_E_INVALID, "gate_norm: a stride is negative");
   const int64_t samples = ((int64_t)c.M - 1) / c.rows_per_batch + 1;
   const Region h = matrix(c.h, c.M, c.D, c.ldh, 2), y = matrix(c.y, c.M, c.D, c.ldy, 2), ho = matrix(c.y ? c.h_out : nullptr, c.M, c.D, c.ldho, 2), no = matrix(c.n_out, c.M, c.D, c.ldn, 2),
                q = matrix(c.q, c.M, c.D, c.ldq, 1), qs = vector(c.q ? c.q_scale : nullptr, c.M, 4);
@@ -369,13 +385,15 @@ int op_rope_table(const OpCtx& ctx, const RopeTableCall& c, OpStatus& st) noexce
 }
 
 int op_rope(const OpCtx& ctx, const EcadRope& c, OpStatus& st) noexcept {
-  if (c.B < 0 || c.S < 0 || c.q.H < 1 || c.k.H < 0 || c.q.H > (1 << 20) || c.k.H > (1 << 20) || c.D < 2 || c.rot < 2 || c.rot % 2 || c.rot > c.D || c.table_rows < 0)
+  if (c.B < 0 || c.S < 0 || c.q.H < 1 || c.k.H < 0 || c.q.H > (1 << 20) || c.k.H > (1 << 20) || c.D < 2 || c.D > (1 << 24) || c.rot < 2 || c.rot % 2 || c.rot > c.D || c.table_rows < 0)
     return refuse(st, ECAD_E_INVALID, "rope: %d samples of %d tokens, %lld + %lld heads of %d elements, %d of them turned (even, 2 to the head's size)", c.B, c.S,
                   (long long)c.q.H, (long long)c.k.H, c.D, c.rot);
   if (c.B == 0 || c.S == 0) return ECAD_OK;
   if (!c.q.x || !c.q.out || (c.k.H && (!c.k.x || !c.k.out)) || !c.table) return refuse(st, ECAD_E_INVALID, "rope: NULL pointer");
   if (!aligned(c.q.x, 2) || !aligned(c.q.out, 2) || !aligned(c.k.x, 2) || !aligned(c.k.out, 2) || !aligned(c.table, 4) || !aligned(c.index, 4)) return refuse(st, ECAD_E_INVALID, "rope: pointers are not aligned to their type");
   if (!c.index && c.table_rows < c.S) return refuse(st, ECAD_E_INVALID, "rope: the table has %d rows for %d tokens", c.table_rows, c.S);
+  auto negative = [](const EcadRopeHeads& x) { return x.sample < 0 || x.token < 0 || x.head < 0 || x.out_sample < 0 || x.out_token < 0 || x.out_head < 0; };
+  if (negative(c.q) || (c.k.H && negative(c.k)) || c.index_stride < 0) return refuse(st, ECAD_E_INVALID, "rope: a stride is negative");
   const bool q_in = c.q.x == c.q.out, k_in = c.k.H == 0 || c.k.x == c.k.out;
   if (c.k.H && q_in != k_in) return refuse(st, ECAD_E_INVALID, "rope: queries and keys are both turned in place or both not");
   auto same = [](const EcadRopeHeads& x) { return x.sample == x.out_sample && x.token == x.out_token && x.head == x.out_head; };
@@ -395,9 +413,11 @@ int op_rope(const OpCtx& ctx, const EcadRope& c, OpStatus& st) noexcept {
   a.groups = (int)((c.q.H + c.k.H + ROPE_HEADS - 1) / ROPE_HEADS);
   const int64_t per_token = (int64_t)a.units * a.groups;
   if (per_token > (1 << 24)) return refuse(st, ECAD_E_UNSUPPORTED, "rope: %lld pieces a token", (long long)per_token);
-  a.tokens_per_block = per_token >= 256 ? 1 : (int)(256 / per_token);
+  constexpr int64_t most = 1 << 23;  // workgroups; more tokens than that: several turns of one
+  const int64_t one = per_token >= 256 ? 1 : 256 / per_token, many = (a.tokens + most - 1) / most;
+  if (many > one && many * per_token > 0x7fffffff) return refuse(st, ECAD_E_UNSUPPORTED, "rope: %lld tokens are more than one launch takes", (long long)a.tokens);
+  a.tokens_per_block = (int)(many > one ? many : one);
   const int64_t blocks = (a.tokens + a.tokens_per_block - 1) / a.tokens_per_block;
-  if (blocks > 0x7fffffff) return refuse(st, ECAD_E_UNSUPPORTED, "rope: %lld tokens are more than one launch takes", (long long)a.tokens);
   const dim3 grid((unsigned)blocks), block(256);
   if (ctx.dtype == ECAD_DTYPE_F16) {
     if (c.half) hipLaunchKernelGGL((rope_kernel<f16_t, true>), grid, block, 0, ctx.stream, a);

@@ -4,6 +4,8 @@ import ctypes as C
 import random
 import struct
 import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -354,3 +356,23 @@ def test_native_calls_keep_reference_counts(eng):
         with pytest.raises(ValueError):
             eng.op_gate_norm(x, x[:2])
     assert [sys.getrefcount(o) for o in (x, out, *out, eng._ops[1], None)][:-1] == before
+
+
+def test_library_refuses_negative_strides(library):
+    gemm = dict(A=AT, lda=48, a_scale=AT, W=AT, ldw=48, w_scale=AT, out=2 * AT, ldo=7, M=3, N=7, K=40, rows_per_batch=1, epi=3, resid=3 * AT, ldr=7, resid_out=3 * AT, ldro=7, gate_mod=5 * AT)
+    norm = dict(h=AT, ldh=24, y=2 * AT, ldy=24, h_out=AT, ldho=24, n_out=2 * AT, ldn=24, M=4, D=24, rows_per_batch=1, post=1, pre=2, resid_scale=1.0, eps=1e-6, gate_mod=5 * AT, mod_scale=6 * AT)
+    heads = dict(x=AT, out=2 * AT, sample=192, token=64, head=16, out_sample=192, out_token=64, out_head=16, H=4)
+    rope = dict(q=heads, k=dict(heads, x=3 * AT, out=4 * AT, H=2), table=5 * AT, B=2, S=3, D=16, rot=16, table_rows=3)
+    calls = [("op_gemm_int8", _Gemm, dict(gemm, gate_mod_stride=-7)), ("op_gate_norm", _Norm, dict(norm, gate_mod_stride=-24)), ("op_gate_norm", _Norm, dict(norm, mod_stride=-24)),
+             ("op_rope", _Rope, dict(rope, index=6 * AT, index_stride=-3))]
+    calls += [("op_rope", _Rope, dict(rope, **{part: dict(rope[part], **{name: -16})})) for part in "qk" for name in ("sample", "token", "head", "out_head")]
+    for name, struct_of, args in calls:
+        rc, msg = library(name, struct_of(**args))
+        assert rc == L.ECAD_E_INVALID and "negative" in msg, (name, args, rc, msg)
+
+
+def test_generated_loops_are_what_their_generator_writes():
+    """ecad_amd/csrc/gemm_int8_asm.h is generated and committed: `--check` writes it anew in memory and compares."""
+    root = Path(__file__).resolve().parents[1]
+    r = subprocess.run([sys.executable, str(root / "scripts" / "gen_gemm_i8.py"), "--check"], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr[-400:]

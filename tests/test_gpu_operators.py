@@ -378,6 +378,38 @@ def test_row_offsets_beyond_32_bits():
     near(out[0, -3:], rope64(x[:, -3:], table[-3:], "half")[0])
 
 
+def test_more_rows_than_one_launch_counts():
+    """A launch has fewer than 2^32 threads: 2^26 rows at four to a workgroup, 2^24 at one, as many tiles of 64 rows are more."""
+    eng, dt = small_engine("float16"), torch.float16
+    for M, K in ((2**26 + 5, 8), (2**24 + 3, 1544)):
+        x = torch.zeros(M, K, device="cuda", dtype=dt)
+        at = [0, 1, M // 2, M - 6, M - 3, M - 1]
+        x[at] = rand(len(at), K, seed=1, dtype=dt)
+        q, s = eng.op_quantize_int8(x)
+        rq, rs = quantized(x[at])
+        assert torch.equal(q[at], rq) and torch.equal(s[at], rs)
+        assert int((s != 0).sum()) == len(at)
+        del x, q, s
+    M = 2**30 + 65
+    a = torch.ones(M, 16, device="cuda", dtype=torch.int8)
+    w, one = int8_rows(1, 16, 2), torch.ones(1, device="cuda")
+    out = eng.op_gemm_int8(0, a, one.expand(M).contiguous(), w, one)
+    assert bool((out == w.sum(dtype=torch.int32).to(dt)).all())
+    with pytest.raises(ValueError, match="more than one launch"):
+        eng.op_gemm_int8(0, a, out.float().view(-1), w, one, kernel="tile64")
+
+
+def test_rope_of_more_tokens_than_one_launch_counts():
+    eng, dt = small_engine("float16"), torch.float16
+    B, S = 70_000, 65_536  # 256 tokens of one pair a workgroup: more than 2^24 of those
+    table = eng.op_rope_table(torch.arange(S, device="cuda", dtype=torch.int32), 2)
+    x = torch.ones(1, device="cuda", dtype=dt).expand(B * S * 2).contiguous().view(B, S, 1, 2)
+    expected = rope64(x[:1], table, "half")[0]
+    eng.op_rope(x, None, table, layout="half", out=(x, None))
+    near(x[:1], expected)
+    assert all(torch.equal(part, x[:1].expand_as(part)) for part in x.split(7000))
+
+
 # ---- rotary positions -----------------------------------------------------------------------------------------------------------------------------------------
 
 
