@@ -71,14 +71,19 @@ template <typename T, bool RAGGED> ECAD_DEV void row_store(T* p, const Pack8& v,
 // A row on WAVES waves, CH pieces of eight elements per lane; every wave (or workgroup of a wider row) takes rows_per_group consecutive rows, the next one's
 // loads in flight while one is worked on.  The channel vectors g, 1 + s, t of a sample stay in registers from row to row: read anew for every row they are up to
 // 26 bytes per element out of L2 against the 8 that the rows themselves move.  They are zero beyond the row, and with them everything that is computed there.
-// HOLD false (rows of more than 8192 values on 16 waves, whose lanes have 128 registers): read anew all the same.
+// HOLD false (rows of more than 8192 values on 16 waves, whose lanes have 128 registers): read anew all the same, and from 16384 values on nothing is in flight ahead.
+// Bound by memory: 8 bytes per value (7 with 8-bit rows out), at the 5.15 TB/s of a large copy 14.7 us for 8192 x 1152 (18.1 measured, a launch being 1.9 of them),
+// 104 us for 16384 x 4096 (109), 58.6 us for 32768 x 1152 (57.6: 5.2 TB/s), 52 us for 4096 x 8192 (45: part of it from the last-level cache).  Rows beyond 8192 values:
+// 2048 x 16384 82 us (3.3 TB/s), 2048 x 32768 156 us (3.4): one row per CU at a time, and the channel vectors out of L2 for each.  Few rows: 5 x 1153 4.8 us:
+// a launch, the loads of the row and its vectors, four meetings of the row's waves.
 template <typename T, int WAVES, int CH, bool RAGGED, bool HOLD>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void gate_norm_kernel(const GateNormArgs p) {
   constexpr int SLOTS = row_slots(WAVES);
+  constexpr bool AHEAD = HOLD || CH <= 2;  // the next row's loads are in flight while one is worked on
   __shared__ unsigned scratch[2][WAVES];  // (one wave a row: not used)
   const int slot = WAVES == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
   const int lane = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
-  const int first = lane * 8;
+  int first = lane * 8;
   int turn = 0;
   float G[HOLD ? CH : 1][8], A[HOLD ? CH : 1][8], B[HOLD ? CH : 1][8];
   int have = -1;  // the sample that G, A, B belong to
@@ -97,8 +102,17 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void gate_norm_kerne
       if (p.y) yv[i] = row_load<T, RAGGED>(yrow, c, p.D);
     }
   };
-  if (row0 < end) fetch(row0);
+  if (AHEAD && row0 < end) fetch(row0);
   for (int64_t row = row0; row < end; ++row) {
+    // one piece after the other, its addresses made for it: ahead of the loop and side by side they took 200 registers that are not there (2048 x 32768: 555 us)
+    auto next_piece = [&]() {
+      if constexpr (!HOLD) {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" : "+v"(first));
+      }
+    };
+    next_piece();
+    if constexpr (!AHEAD) fetch(row);
     const int b = (int)((unsigned)row / (unsigned)p.rows_per_batch);
     // the vectors of piece i: the gate's (what & 1) or scale and shift (what & 2).  All loads first: each is behind a branch on its pointer, and combined one by one
     // they would wait for each other (eight round trips to memory in front of the first row: 5 of the 8.5 us of a call with five rows)
@@ -155,13 +169,16 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void gate_norm_kerne
       for (int i = 0; i < CH; ++i) channels(i, i, 3);
     }
     float x[CH][8];
+    auto unpack_h = [&](int i) { unpack8<T>(row_piece<RAGGED>(hv[i], first + i * WAVES * 512, p.D), x[i]); };
+    if (AHEAD || !p.y) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) unpack8<T>(row_piece<RAGGED>(hv[i], first + i * WAVES * 512, p.D), x[i]);
+      for (int i = 0; i < CH; ++i) unpack_h(i);
+    }
     if (p.y) {
       float u[CH][8];
 #pragma unroll
       for (int i = 0; i < CH; ++i) unpack8<T>(row_piece<RAGGED>(yv[i], first + i * WAVES * 512, p.D), u[i]);
-      if (row + 1 < end) fetch(row + 1);
+      if (AHEAD && row + 1 < end) fetch(row + 1);
       if (p.post) {
         const float rstd = row_statistics<WAVES, CH, RAGGED>(u, p.post, first, p.D, inv_d, p.eps, scratch, turn);
 #pragma unroll
@@ -173,12 +190,14 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void gate_norm_kerne
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int c = first + i * WAVES * 512, at = HOLD ? i : 0;
+        if constexpr (!HOLD) next_piece();
+        if constexpr (!AHEAD) unpack_h(i);
         if constexpr (!HOLD) channels(i, 0, 1);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[i][e] = __builtin_fmaf(u[i][e], G[at][e], p.resid_scale * x[i][e]);
         row_store<T, RAGGED>(ho + c, pack8<T>(x[i]), p.D - c);
       }
-    } else if (row + 1 < end) {
+    } else if (AHEAD && row + 1 < end) {
       fetch(row + 1);
     }
     if (p.pre == NORM_NONE) continue;
@@ -188,10 +207,11 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void gate_norm_kerne
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int at = HOLD ? i : 0;
-      if constexpr (!HOLD) channels(i, 0, 2);
+      if constexpr (!HOLD) next_piece(), channels(i, 0, 2);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[i][e] = __builtin_fmaf(x[i][e] * rstd, A[at][e], B[at][e]);
       nv[i] = pack8<T>(x[i]);
+      if constexpr (!HOLD) asm volatile("" : "+v"(nv[i].u));  // now, not where it is stored
     }
     if (p.q) {
 #pragma unroll
@@ -200,6 +220,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void gate_norm_kerne
       if (lane == 0) p.q_scale[row] = k.s;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
+        next_piece();
         const int c = first + i * WAVES * 512;
         unpack8<T>(nv[i], x[i]);
         store_int8_piece<RAGGED>(p.q + row * p.ldq + c, int8_piece(x[i], k), p.D - c);
@@ -208,6 +229,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void gate_norm_kerne
       T* no = reinterpret_cast<T*>(p.n_out) + row * p.ldn;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
+        next_piece();
         const int c = first + i * WAVES * 512;
         row_store<T, RAGGED>(no + c, nv[i], p.D - c);
       }
@@ -223,7 +245,8 @@ struct QuantizeArgs {
   int M, K;
 };
 
-// One row per WAVES waves, the whole row in registers between the maximum and the rounding: read once.
+// One row per WAVES waves, the whole row in registers between the maximum and the rounding: read once.  Bound by memory, 3 bytes per value: 8192 x 4608 19.5 to 22 us
+// (5.1 to 5.8 TB/s; a copy moves 5.15), 8192 x 1152 7.8 us (3.6 TB/s with its launch), 601 x 4001 4.2 us.
 template <typename T, int WAVES, int CH, bool RAGGED>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void quantize_rows_kernel(const QuantizeArgs p) {
   __shared__ unsigned scratch[2][WAVES];

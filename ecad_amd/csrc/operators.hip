@@ -146,7 +146,8 @@ template <typename T> int quantize_t(const OpCtx& ctx, const QuantizeArgs& a, Op
 
 template <typename T, int WAVES, int CH, bool HOLD = true> int launch_norm(const OpCtx& ctx, GateNormArgs& a, int per_cu, OpStatus& st) {
   // Rows in turn: a lane keeps the channel vectors and has the next row's loads in flight while it works on one.  per_cu: rows that a CU works on at a time (what its
-  // registers hold: 97 / 147 / 209 of 512 per lane at one / two / three pieces); every wave gets at least one row.
+  // registers hold: 115 / 165 / 230 of 512 per lane at one / two / three pieces); every wave gets at least one row.  One wave a row, three pieces: 8 was the
+  // best of 4, 8, 12, 16, 24 and 32 at 8192 and 32768 rows of 1152.
   const int slots = row_slots(WAVES);
   const int64_t at_once = (int64_t)ctx.num_cus * per_cu;
   a.rows_per_group = (int)((a.M + at_once - 1) / at_once);
