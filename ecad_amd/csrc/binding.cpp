@@ -216,12 +216,10 @@ void* stream(const Engine& e) {
   if (!s && PyErr_Occurred()) throw python_error();
   return s;
 }
-// f: the entry point alone (it does not throw; the interpreter's lock is released around it)
+// f: the entry point alone.  The interpreter's lock stays held: the call only launches, in less time than handing the lock over and back may take, and an engine has one
+// last error -- two threads that are refused at once would write it at once.
 template <typename F> void launch(const Engine& e, F&& f) {
-  void* s = stream(e);
-  PyThreadState* state = PyEval_SaveThread();
-  const int rc = f(s);
-  PyEval_RestoreThread(state);
+  const int rc = f(stream(e));
   if (rc == ECAD_OK) return;
   const char* m = e.last_error(e.handle);
   const std::string message = m && *m ? m : "error " + std::to_string(rc);

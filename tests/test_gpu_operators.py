@@ -4,6 +4,7 @@ definitions in 64 bits.
 Tolerances, per element and fixed before the first run: one rounding to the storage type, eps / 2 of the value (plus half of the smallest fp16 step), and the fp32
 arithmetic in front of it, a stated multiple of 2^-24 of the magnitudes that enter the sum (`extra`).  8-bit integers and their scales are exact."""
 import math
+import threading
 
 import pytest
 import torch
@@ -660,6 +661,47 @@ def test_calls_on_two_streams_at_once():
     for i in range(2):
         for got in outs[i]:
             assert all(torch.equal(a, b) for a, b in zip(got, alone[i]))
+
+
+def test_two_threads_share_an_engine():
+    """Calls and refusals of two threads on one engine: results are right, and each thread is told what it did wrong itself."""
+    eng, dt = small_engine("float16"), torch.float16
+    x = rand(64, 64, seed=1, dtype=dt)
+    q, s = eng.op_quantize_int8(x)
+    rq, rs = quantized(x)
+    wrong = []
+
+    def quantiser():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(300):
+                try:
+                    eng.op_quantize_int8(x, out=(x.view(torch.int8)[:, :64], s))
+                except ValueError as e:
+                    wrong.extend([str(e)] if "quantize_int8" not in str(e) else [])
+                out = eng.op_quantize_int8(x)
+            torch.cuda.current_stream().synchronize()
+            wrong.extend(["quantised"] if not (torch.equal(out[0], rq) and torch.equal(out[1], rs)) else [])
+
+    def norm():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(300):
+                try:
+                    eng.op_gate_norm(x, pre="rms", out_n=x)
+                except ValueError as e:
+                    wrong.extend([str(e)] if "gate_norm" not in str(e) else [])
+                n = eng.op_gate_norm(x, pre="layer")[1]
+            torch.cuda.current_stream().synchronize()
+            wrong.extend(["norm"] if not torch.equal(n, first) else [])
+
+    first = eng.op_gate_norm(x, pre="layer")[1]
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=f) for f in (quantiser, norm)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
 
 
 def test_refusals_reach_the_caller():
