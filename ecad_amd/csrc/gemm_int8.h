@@ -2,8 +2,8 @@
 //
 //   o[m][n] = act(sa[m] sw[n] sum_k A[m][k] W[n][k] + bias[n]),   epilogue 3: resid'[m][n] = resid[m][n] + (gt[n] + gm[sample][n]) T(o[m][n])
 //
-// The sums are whole numbers in 32 bits (K < 2^17: 127^2 K < 2^31), so no order of K changes them and every kernel here gives the same bits.  The product of the
-// two scales, the bias, the activation and the gate are fp32; o is rounded once to the storage type, and the residual takes the rounded o (it is what a cache of
+// The sums are whole numbers in 32 bits (K < 2^17: 127^2 K < 2^31), so no order of K changes them and every kernel here gives the same bits.  The scales
+// (the token's first: their own product could leave the normal range of fp32 where the result does not), the bias, the activation and the gate are fp32; o is rounded once to the storage type, and the residual takes the rounded o (it is what a cache of
 // the sub-layer holds and replays).  A row whose scale is NaN comes out NaN.
 //
 // Operands: rows of 8-bit integers on 16 bytes, any M, N, K.  The last 16-byte piece of a row may reach past column K: it stays inside the aligned 16 bytes that
@@ -108,7 +108,7 @@ ECAD_DEV void int8_epilogue(const Int8GemmArgs& p, char* smem, int m0, int n0, i
     const i32x4 a = acc(ic, jc);
     float o[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] = int8_act<EPI>(__builtin_fmaf((float)a[r], sa[decltype(ic)::value] * sw[r], bias[r]));
+    for (int r = 0; r < 4; ++r) o[r] = int8_act<EPI>(__builtin_fmaf((float)a[r] * sa[decltype(ic)::value], sw[r], bias[r]));
     return (u32x2){pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3])};
   };
   if (direct) {
@@ -314,8 +314,8 @@ __global__ __launch_bounds__(WM * WN * KW * 64, 2) void gemm_int8_kernel(const I
 // The same product on one wave per SIMD, 256 x BN tiles on four waves: the K loop over whole stages is one hand-placed asm statement (gemm_int8_asm.h, generated by
 // scripts/gen_gemm_i8.py) that leaves the accumulators in AGPRs.  hipcc knows those only as clobbers of the statement: everything that touches them afterwards is asm
 // too, and the build fails if the compiler uses one before the last is read (scripts/audit_agpr.py).
-// 8192 x 8192 x 4096: 232 us, 2360 TOP/s (a library's 8192^3: 2330).  8192 x 1152 x 4608: 39.4 us (2210 TOP/s), 50 with the gated residual; 8192 x 4608 x 1152: 52.3 us
-// (1660), 57 with GELU; 4096 x 3456 x 1152: 23.5 us (1390).  Bound by the stream of operands into LDS: a piece holds its wave 60 to 180 cycles, and a stage of the 256 x 144
+// 8192 x 8192 x 4096: 232 us, 2360 TOP/s (a library's 8192^3: 2330).  8192 x 1152 x 4608: 39.4 us (2210 TOP/s), 50 with the gated residual; 8192 x 4608 x 1152: 52 to
+// 57 us (1520 to 1660, as the clock allows), 57 to 62 with GELU; 4096 x 3456 x 1152: 23.5 us (1390).  Bound by the stream of operands into LDS: a piece holds its wave 60 to 180 cycles, and a stage of the 256 x 144
 // tile takes 1 us with 0.5 us of matrix instructions in it (their pipe is busy 36 % of a CU's cycles at K 1152, 40 % at 4608); then by the epilogue, which has the chip to
 // itself in a launch of one round.
 template <int BN> struct Int8Wide {
@@ -462,7 +462,7 @@ __global__ __launch_bounds__(NW * 64) void gemm_int8_rows_kernel(const Int8GemmA
     int sum = part[0][it];
 #pragma unroll
     for (int w = 1; w < NW; ++w) sum += part[w][it];
-    const float o = int8_act<EPI>(__builtin_fmaf((float)sum, p.sa[m] * p.sw[n], p.bias ? p.bias[n] : 0.f));
+    const float o = int8_act<EPI>(__builtin_fmaf((float)sum * p.sa[m], p.sw[n], p.bias ? p.bias[n] : 0.f));
     const float rounded = round_elem<T>(o);
     if (EPI != I8_RESID || p.out) reinterpret_cast<T*>(p.out)[(int64_t)m * p.ldo + n] = (T)o;
     if constexpr (EPI == I8_RESID) {

@@ -208,6 +208,22 @@ def test_gemm_largest_sums():
         near(out, torch.full((20, 20), K * 2.0**14 * 2.0**-31, device="cuda", dtype=torch.float64))
 
 
+@pytest.mark.parametrize("kernel", ["rows", "tile64", "tile64k2", "tile128", "tile144", "tile256", "tile288"])
+def test_gemm_scales_whose_product_leaves_fp32(kernel):
+    """1e-23 * 1e-21 is seven steps above zero in fp32, the result 1e-37 is not; and a sum of zero stays zero where the scales' product would be infinite."""
+    eng, M, N, K = small_engine("bfloat16"), 30, 40, 1152
+    a, w = int8_rows(M, K, 1), int8_rows(N, K, 2)
+    a.fill_(100)
+    w.fill_(90)
+    one = torch.ones(64, device="cuda")
+    out = eng.op_gemm_int8(0, a, one[:M] * 1e-23, w, one[:N] * 1e-21, kernel=kernel)
+    ref = torch.full((M, N), 9000.0 * K, device="cuda", dtype=torch.float64) * float((one * 1e-23)[0].double() * (one * 1e-21)[0].double())
+    near(out, ref, 2.0**-22 * ref)
+    w[:, ::2] = -90
+    out = eng.op_gemm_int8(0, a, one[:M] * 1e30, w, one[:N] * 1e30, one[:N] * 3, kernel=kernel)
+    assert bool((out == 3).all())
+
+
 def test_gemm_offsets_beyond_32_bits():
     eng, dt = small_engine("float16"), torch.float16
     M, N, K = 300_003, 8192, 16
