@@ -128,7 +128,7 @@ const float* vector(const Engine& e, PyObject* o, const char* name, int64_t n) {
   check(e, *t, name, at::kFloat, {n}, WHOLE);
   return static_cast<const float*>(t->data_ptr());
 }
-// modulations [samples, N] that cover M rows; stride 0 for one sample
+// modulations [samples, N] that cover M rows, and the stride between samples: 0 where the rows are one sample's, or where all samples share one (an expanded view)
 struct Mod {
   const void* p = nullptr;
   int64_t stride = 0;
@@ -140,7 +140,7 @@ Mod modulation(const Engine& e, PyObject* o, const char* name, int64_t M, int64_
   check(e, t, name, e.dtype, {samples, N}, LAST);
   if (rows_per_batch < 1) refuse("rows_per_batch must be at least 1, got %lld", (long long)rows_per_batch);
   if (M > samples * rows_per_batch) refuse("%s has %lld samples of %lld rows, %lld rows are given", name, (long long)samples, (long long)rows_per_batch, (long long)M);
-  return {t.data_ptr(), samples > 1 ? t.stride(0) : 0};
+  return {t.data_ptr(), M > rows_per_batch ? t.stride(0) : 0};
 }
 int32_t size32(int64_t v, const char* what) {
   if (v > INT32_MAX) refuse("%s %lld is more than these operators index", what, (long long)v);
@@ -315,8 +315,8 @@ PyObject* gate_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     g.table_shift = vector(e, a[9], "table_shift", D), g.table_scale = vector(e, a[10], "table_scale", D);
     const Mod gm = modulation(e, a[8], "gate_mod", M, D, g.rows_per_batch), ms = modulation(e, a[11], "mod_shift", M, D, g.rows_per_batch), mc = modulation(e, a[12], "mod_scale", M, D, g.rows_per_batch);
     g.gate_mod = gm.p, g.gate_mod_stride = gm.stride, g.mod_shift = ms.p, g.mod_scale = mc.p;
-    if (ms.stride && mc.stride && ms.stride != mc.stride) refuse("mod_shift and mod_scale must have the same stride between samples, got %lld and %lld", (long long)ms.stride, (long long)mc.stride);
-    g.mod_stride = ms.stride ? ms.stride : mc.stride;
+    if (ms.p && mc.p && ms.stride != mc.stride) refuse("mod_shift and mod_scale must have the same stride between samples, got %lld and %lld (one that all samples share may be a table)", (long long)ms.stride, (long long)mc.stride);
+    g.mod_stride = ms.p ? ms.stride : mc.stride;
     Out nh, nn;
     Int8Out q;
     if (y) {

@@ -447,7 +447,9 @@ class EcadEngine:
 
         pre / post: "none", "rms", "layer" (with ``pre_weight`` / ``post_weight`` fp32 [D] where given; ``eps`` None: the engine's norm_eps).  gate = gate_table fp32 [D] +
         gate_mod [samples, D] (1 without either), scale and shift in the same way (0 without either); sample = row // rows_per_batch, modulations may be column slices of
-        one wider tensor.  Returns (h', n); without y h' is h itself; with pre "none" n is None; ``quantize``: n as (q, scale) of ``op_quantize_int8``, bit for bit.
+        one wider tensor.  Over more than one sample mod_shift and mod_scale have the same stride between samples: both per sample, or both expanded from one row (a shared one
+        beside one per sample goes into its table).  Returns (h', n); without y h' is h itself; with pre "none" n is None; ``quantize``: n as (q, scale) of
+        ``op_quantize_int8``, bit for bit.
         ``out_h`` may be h, ``out_n`` may be y (``quantize``: out_n is a (q, scale) pair)."""
         ops, engine = self._ops or self._native()
         before, after = self.NORMS.get(pre), self.NORMS.get(post)

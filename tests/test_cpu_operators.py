@@ -376,3 +376,57 @@ def test_generated_loops_are_what_their_generator_writes():
     root = Path(__file__).resolve().parents[1]
     r = subprocess.run([sys.executable, str(root / "scripts" / "gen_gemm_i8.py"), "--check"], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr[-400:]
+
+
+# ---- calls that go through: an engine whose library answers that all is well ----------------------------------------------------------------------------------------
+
+
+class _Accepts:
+    """Five entry points that return 0; `records` holds what the three that take one were given, by member name."""
+
+    def __init__(self):
+        P, I, I64, D = C.c_void_p, C.c_int, C.c_int64, C.c_double
+        self.records, self.kept = [], []
+
+        def record_of(codes, names):
+            def call(handle, record, stream):
+                self.records.append(dict(zip(names, codes.unpack(C.string_at(record, codes.size)))))
+                return 0
+
+            return C.CFUNCTYPE(I, P, P, P)(call)
+
+        self.kept.append(C.CFUNCTYPE(I, P, P, I64, P, I64, P, I, I, P)(lambda *args: 0))
+        self.kept += [record_of(INT8_GEMM_CODES, GEMM), record_of(GATE_NORM_CODES, NORM)]
+        self.kept.append(C.CFUNCTYPE(I, P, P, I, P, I, I, I, D, D, D, D, D, P, P)(lambda *args: 0))
+        self.kept += [record_of(ROPE_CODES, ROPE), C.CFUNCTYPE(P, P)(lambda handle: None)]
+        self.addresses = tuple(C.cast(f, P).value for f in self.kept)
+
+
+@pytest.fixture
+def accepting():
+    calls, ops = _Accepts(), L.load_ops()
+    e = object.__new__(EcadEngine)
+    e._h, e.cfg, e.calls = C.c_void_p(), L.EcadModelCfg(), calls
+    e._ops = ops, ops.engine(calls.addresses, 1 << 20, L.ECAD_DTYPE_F16, -1, lambda index: 0)
+    return e
+
+
+def test_modulations_reach_the_library_with_strides_that_hold_for_both(accepting):
+    """Shift and scale have one stride between samples in the library: one that all samples share (stride 0) beside one per sample would be read past its end."""
+    h, shared, own = f16(4, 24), f16(1, 24).expand(4, 24), f16(4, 72)[:, :24]
+    for pair in ((shared, own), (own, shared)):
+        for kw in ({}, dict(quantize=True)):
+            with pytest.raises(ValueError, match="same stride"):
+                accepting.op_gate_norm(h, mod_shift=pair[0], mod_scale=pair[1], **kw)
+    assert not accepting.calls.records
+    for kw, stride in [
+        (dict(mod_shift=shared, mod_scale=shared), 0),
+        (dict(mod_shift=own, mod_scale=own), 72),
+        (dict(mod_shift=shared), 0),
+        (dict(mod_scale=own), 72),
+        (dict(mod_shift=shared, mod_scale=own, rows_per_batch=4), 0),  # one sample: nothing lies between samples
+        (dict(mod_shift=f16(2, 24), mod_scale=own, rows_per_batch=5), 0),
+        (dict(mod_shift=f16(1, 24), mod_scale=own, rows_per_batch=4), 0),
+    ]:
+        accepting.op_gate_norm(h, **kw)
+        assert accepting.calls.records.pop()["mod_stride"] == stride, kw

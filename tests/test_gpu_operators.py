@@ -733,3 +733,32 @@ def test_refusals_reach_the_caller():
         eng.op_rope(rand(1, 4, 1, 8, dtype=torch.float16), None, torch.zeros(3, 4, 2, device="cuda"))
     with pytest.raises(ValueError, match="is on cpu"):
         eng.op_quantize_int8(torch.zeros(2, 8, dtype=torch.float16))
+
+
+@pytest.mark.parametrize("dtype_name", DTYPES)
+def test_gate_norm_modulations_shared_by_all_samples(dtype_name):
+    """A modulation expanded over the samples; a shared one beside one per sample is refused, as modulations it would be read with the other's stride, and goes into its table."""
+    dt, eng = getattr(torch, dtype_name), small_engine(dtype_name)
+    M, D, rows = 37, 200, 10
+    h, y, par = norm_inputs(M, D, dt, 4, dict(mod_shift=True, mod_scale=True, gate_mod=True), seed=11)
+    own_shift, own_scale = par["mod_shift"], par["mod_scale"]
+    one = dict(mod_shift=own_shift[1:2], mod_scale=own_scale[2:3])
+    shared = {k: v.expand(4, D) for k, v in one.items()}
+    for par in (dict(shared, gate_mod=par["gate_mod"][:1].expand(4, D)), dict(mod_shift=shared["mod_shift"]), dict(mod_scale=shared["mod_scale"])):
+        nh, n = eng.op_gate_norm(h, y, pre="layer", rows_per_batch=rows, **par)
+        rh, sh, rn, sn = gate_norm64(h, y, "layer", "none", 1.0, 1e-6, rows, **par)
+        near(nh, rh, 2.0**-19 * sh)
+        near(n, rn, 2.0**-19 * sn)
+    for mixed in (dict(mod_shift=shared["mod_shift"], mod_scale=own_scale), dict(mod_shift=own_shift, mod_scale=shared["mod_scale"])):
+        for quantize in (False, True):
+            with pytest.raises(ValueError, match="same stride"):
+                eng.op_gate_norm(h, y, pre="layer", rows_per_batch=rows, quantize=quantize, **mixed)
+        nh, n = eng.op_gate_norm(h, y, pre="layer", rows_per_batch=M, **mixed)  # all rows are one sample's: the strides do not matter
+        rh, sh, rn, sn = gate_norm64(h, y, "layer", "none", 1.0, 1e-6, M, **mixed)
+        near(n, rn, 2.0**-19 * sn)
+    for mixed in (dict(table_shift=one["mod_shift"][0].float(), mod_scale=own_scale), dict(mod_shift=own_shift, table_scale=one["mod_scale"][0].float())):
+        nh, n = eng.op_gate_norm(h, y, pre="layer", rows_per_batch=rows, **mixed)
+        rh, sh, rn, sn = gate_norm64(h, y, "layer", "none", 1.0, 1e-6, rows, **mixed)
+        near(n, rn, 2.0**-19 * sn)
+        _, (q, s) = eng.op_gate_norm(h, y, pre="layer", rows_per_batch=rows, quantize=True, **mixed)
+        assert all(torch.equal(a, b) for a, b in zip((q, s), quantized(n)))
