@@ -187,7 +187,8 @@ Int8Out out_int8(const Engine& e, PyObject* given, const char* name, int64_t M, 
     o.q.given = PyTuple_GET_ITEM(given, 0);
     o.scale.given = PyTuple_GET_ITEM(given, 1);
     o.stride = int8_rows(e, tensor(o.q.given, "q"), "q", M, N);
-    if (!vector(e, o.scale.given, "scale", M)) refuse("%s must come with its scale", name);
+    if (o.scale.given == Py_None) refuse("%s must come with its scale", name);
+    (void)vector(e, o.scale.given, "scale", M);
   } else {
     o.stride = (N + 15) & ~(int64_t)15;
     Tensor rows = fresh(e, {M, o.stride}, at::kChar);
