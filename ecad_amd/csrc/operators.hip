@@ -316,12 +316,12 @@ int op_gate_norm(const OpCtx& ctx, const EcadGateNorm& c, OpStatus& st) noexcept
   if (c.post < NORM_NONE || c.post > NORM_LAYER || c.pre < NORM_NONE || c.pre > NORM_LAYER) return refuse(st, ECAD_E_INVALID, "gate_norm: norm kinds are 0 (none), 1 (rms), 2 (layer)");
   if (!(c.eps >= 0.f) || !(fabsf(c.resid_scale) < INFINITY)) return refuse(st, ECAD_E_INVALID, "gate_norm: eps %g, residual scale %g", (double)c.eps, (double)c.resid_scale);
   if (c.rows_per_batch < 1) return refuse(st, ECAD_E_INVALID, "gate_norm: rows_per_batch must be at least 1");
-  if (!c.y && (c.post != NORM_NONE || c.post_weight || c.gate_table || c.gate_mod || c.resid_scale != 1.f || c.pre == NORM_NONE))
-    return refuse(st, ECAD_E_INVALID, "gate_norm: without y there is no gate, post-norm or residual scale, and the pre-norm is what is left to do");
   if (c.pre == NORM_NONE && (c.pre_weight || c.table_shift || c.table_scale || c.mod_shift || c.mod_scale || c.n_out || c.q))
     return refuse(st, ECAD_E_INVALID, "gate_norm: weight, modulation and output of a pre-norm that is 'none'");
   if (c.post == NORM_NONE && c.post_weight) return refuse(st, ECAD_E_INVALID, "gate_norm: weight of a post-norm that is 'none'");
-  if (c.M == 0) return ECAD_OK;
+  if (c.M == 0) return ECAD_OK;  // an empty y may be NULL: it says nothing about the call
+  if (!c.y && (c.post != NORM_NONE || c.post_weight || c.gate_table || c.gate_mod || c.resid_scale != 1.f || c.pre == NORM_NONE))
+    return refuse(st, ECAD_E_INVALID, "gate_norm: without y there is no gate, post-norm or residual scale, and the pre-norm is what is left to do");
   if (!c.h || (c.y && !c.h_out) || (c.pre != NORM_NONE && !c.n_out == !c.q) || (c.q && !c.q_scale)) return refuse(st, ECAD_E_INVALID, "gate_norm: NULL pointer, or both n and its 8-bit rows asked for");
   const int64_t least = c.M > 1 ? c.D : 0;
   if (c.ldh < least || (c.y && (c.ldy < least || c.ldho < least)) || (c.n_out && c.ldn < least)) return refuse(st, ECAD_E_INVALID, "gate_norm: a row stride is shorter than %d", c.D);

@@ -1,7 +1,8 @@
 """Calls of the operators of an 8-bit transformer block that the documentation allows, without a GPU: an engine whose library answers that all is well."""
-import torch
+import pytest
 
-from test_cpu_operators import accepting, f16, f32, i8  # noqa: F401  (accepting: a fixture)
+from ecad_amd import _lib as L
+from test_cpu_operators import AT, _Norm, accepting, f16, f32, i8, library  # noqa: F401  (accepting, library: fixtures)
 
 
 def test_no_rows_into_given_8bit_outputs(accepting):  # noqa: F811
@@ -12,3 +13,13 @@ def test_no_rows_into_given_8bit_outputs(accepting):  # noqa: F811
     assert got[0] is out[0] and got[1] is out[1]
     _, got = accepting.op_gate_norm(x[:0], pre="rms", quantize=True, out_n=out)
     assert got[0] is out[0] and got[1] is out[1]
+
+
+@pytest.mark.parametrize("asks", [dict(post=1), dict(post=2, post_weight=AT), dict(pre=0, n_out=None), dict(gate_table=AT), dict(gate_mod=AT), dict(resid_scale=0.5)])
+def test_no_rows_of_a_sublayer(library, asks):  # noqa: F811
+    """h and y of zero rows have no addresses, and a NULL y is not a call without y there."""
+    norm = dict(h=AT, ldh=24, y=2 * AT, ldy=24, h_out=AT, ldho=24, n_out=2 * AT, ldn=24, M=4, D=24, rows_per_batch=1, post=0, pre=2, resid_scale=1.0, eps=1e-6)
+    empty = dict(M=0, h=None, y=None, h_out=None, n_out=None)
+    assert library("op_gate_norm", _Norm(**{**norm, **asks, **empty})) == (0, "")
+    rc, msg = library("op_gate_norm", _Norm(**{**norm, **asks, "y": None}))
+    assert rc == L.ECAD_E_INVALID and "without y" in msg

@@ -16,5 +16,10 @@ def test_no_rows():
     out = (q[:0, :24], s[:0])
     assert eng.op_quantize_int8(x[:0], out=out)[0] is out[0]
     assert eng.op_gate_norm(x[:0], pre="rms", quantize=True, out_n=out)[1][1] is out[1]
+    for kw in (dict(pre="rms", post="rms"), dict(pre="layer", gate_table=torch.ones(24, device="cuda")), dict(pre="rms", resid_scale=0.5)):
+        nh, n = eng.op_gate_norm(x[:0], x[:0], **kw)
+        assert nh.shape == n.shape == (0, 24)
+    nh, n = eng.op_gate_norm(x[:0], x[:0], pre="none")
+    assert nh.shape == (0, 24) and n is None
     torch.cuda.synchronize()
     assert bool((q == 9).all()) and bool((s == 9).all())
