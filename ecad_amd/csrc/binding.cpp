@@ -100,9 +100,12 @@ enum Dense { WHOLE, LAST };  // contiguous, or the last dimension only
 
 bool dense(const Tensor& t, Dense how) { return how == WHOLE ? t.is_contiguous() : t.dim() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1; }
 
-// on the engine's device, of that type and shape; gradients are not recorded by these operators
+// a tangent of forward-mode differentiation (of the tensor, or of what it is a view of); none where that mode is switched off
+bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
+
+// on the engine's device, of that type and shape; gradients are not recorded by these operators, tangents not carried on
 void check(const Engine& e, const Tensor& t, const char* name, at::ScalarType type, at::IntArrayRef shape, Dense how) {
-  if (t.scalar_type() == type && t.device() == e.device && t.sizes() == shape && dense(t, how) && !(t.requires_grad() && c10::GradMode::is_enabled())) return;
+  if (t.scalar_type() == type && t.device() == e.device && t.sizes() == shape && dense(t, how) && !(t.requires_grad() && c10::GradMode::is_enabled()) && !has_tangent(t)) return;
   if (t.device() != e.device) refuse("%s is on %s, this engine on %s", name, t.device().str().c_str(), e.device.str().c_str());
   if (t.scalar_type() != type) {
     auto of = [](at::ScalarType s) { return s == at::kHalf ? "torch.float16" : s == at::kBFloat16 ? "torch.bfloat16" : s == at::kFloat ? "torch.float32" : s == at::kChar ? "torch.int8" : s == at::kInt ? "torch.int32" : at::toString(s); };
@@ -110,6 +113,7 @@ void check(const Engine& e, const Tensor& t, const char* name, at::ScalarType ty
   }
   if (t.sizes() != shape) refuse("%s must have shape %s, got %s", name, text(shape).c_str(), text(t.sizes()).c_str());
   if (!dense(t, how)) refuse("%s must %s, got strides %s", name, how == WHOLE ? "be contiguous" : "have a dense last dimension", text(t.strides()).c_str());
+  if (has_tangent(t)) refuse("%s has a forward-mode tangent: this op carries none on (take unpack_dual(...).primal, or switch forward gradients off)", name);
   refuse("%s requires a gradient: this op has none (detach it, or call under torch.no_grad())", name);
 }
 // a row stride (one row: the width, whatever the tensor says)

@@ -1,5 +1,7 @@
 """Calls of the operators of an 8-bit transformer block that the documentation allows, without a GPU: an engine whose library answers that all is well."""
 import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
 
 from ecad_amd import _lib as L
 from test_cpu_operators import AT, _Norm, accepting, f16, f32, i8, library  # noqa: F401  (accepting, library: fixtures)
@@ -23,3 +25,19 @@ def test_no_rows_of_a_sublayer(library, asks):  # noqa: F811
     assert library("op_gate_norm", _Norm(**{**norm, **asks, **empty})) == (0, "")
     rc, msg = library("op_gate_norm", _Norm(**{**norm, **asks, "y": None}))
     assert rc == L.ECAD_E_INVALID and "without y" in msg
+
+
+def test_forward_mode_tangents_are_refused(accepting):  # noqa: F811
+    """Of a tensor, of what it is a view of, of an output that would be written behind its tangent; not where forward gradients are switched off."""
+    h, w = f16(4, 24), f32(24)
+    with forward_ad.dual_level():
+        dual, wide = forward_ad.make_dual(h, f16(4, 24)), forward_ad.make_dual(f16(4, 48), f16(4, 48))
+        for call in [lambda: accepting.op_gate_norm(dual), lambda: accepting.op_gate_norm(wide[:, :24]), lambda: accepting.op_gate_norm(h, pre_weight=forward_ad.make_dual(w, w)),
+                     lambda: accepting.op_gate_norm(h, h.clone(), out_h=dual), lambda: accepting.op_quantize_int8(dual)]:
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):  # no_grad is the other mode's
+                call()
+            with torch.inference_mode():
+                call()
+        accepting.op_gate_norm(forward_ad.unpack_dual(dual).primal)
