@@ -4,9 +4,11 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <ATen/TracerMode.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 
 #include <cstdarg>
 #include <memory>
@@ -54,7 +56,16 @@ std::string text(at::IntArrayRef v) {
 
 // ---- arguments ---------------------------------------------------------------------------------------------------------------------------------------------------
 
+// These calls pass torch's dispatcher by: a tracer would see the allocation of a result and nothing that fills it.
+void refuse_tracing() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  const bool recorded = Modes::any_modes_set() && (Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FAKE) || Modes::get_mode(Key::FUNCTIONAL));
+  if (recorded || at::tracer::impl::is_dispatch_enabled()) throw std::runtime_error("this op cannot be traced: it is a call into the library that a recorded graph would not hold");
+}
+
 const Engine& engine_of(PyObject* o) {
+  refuse_tracing();
   if (o == Py_None) throw std::runtime_error("the engine is closed");
   void* p = PyCapsule_GetPointer(o, ENGINE);
   if (!p) throw python_error();
@@ -103,9 +114,16 @@ bool dense(const Tensor& t, Dense how) { return how == WHOLE ? t.is_contiguous()
 // a tangent of forward-mode differentiation (of the tensor, or of what it is a view of); none where that mode is switched off
 bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
 
-// on the engine's device, of that type and shape; gradients are not recorded by these operators, tangents not carried on
+// a tensor of another kind that stands for values it does not hold itself (fake, wrapped by a transform, a subclass with a dispatch of its own)
+bool stands_in(const Tensor& t) {
+  static const c10::DispatchKeySet kinds({c10::DispatchKey::Python, c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::Batched});
+  return t.key_set().has_any(kinds);
+}
+
+// on the engine's device, of that type and shape, with memory of its own; gradients are not recorded by these operators, tangents not carried on
 void check(const Engine& e, const Tensor& t, const char* name, at::ScalarType type, at::IntArrayRef shape, Dense how) {
-  if (t.scalar_type() == type && t.device() == e.device && t.sizes() == shape && dense(t, how) && !(t.requires_grad() && c10::GradMode::is_enabled()) && !has_tangent(t)) return;
+  if (t.scalar_type() == type && t.device() == e.device && t.sizes() == shape && dense(t, how) && !(t.requires_grad() && c10::GradMode::is_enabled()) && !has_tangent(t) && !stands_in(t)) return;
+  if (stands_in(t)) throw std::runtime_error(std::string(name) + " is a tensor that holds no values itself (traced, transformed, or a subclass with a dispatch of its own)");
   if (t.device() != e.device) refuse("%s is on %s, this engine on %s", name, t.device().str().c_str(), e.device.str().c_str());
   if (t.scalar_type() != type) {
     auto of = [](at::ScalarType s) { return s == at::kHalf ? "torch.float16" : s == at::kBFloat16 ? "torch.bfloat16" : s == at::kFloat ? "torch.float32" : s == at::kChar ? "torch.int8" : s == at::kInt ? "torch.int32" : at::toString(s); };
@@ -274,7 +292,7 @@ PyObject* gemm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t M = A.size(0), K = A.size(1), N = W.size(0);
     EcadInt8Gemm g{};
     g.epi = integer32(a[1], "epi");
-    g.A = static_cast<const int8_t*>(A.data_ptr()), g.lda = int8_rows(e, A, "a", M, K), g.W = static_cast<const int8_t*>(W.data_ptr()), g.ldw = int8_rows(e, W, "w", N, K);
+    g.lda = int8_rows(e, A, "a", M, K), g.A = static_cast<const int8_t*>(A.data_ptr()), g.ldw = int8_rows(e, W, "w", N, K), g.W = static_cast<const int8_t*>(W.data_ptr());
     g.a_scale = vector(e, a[3], "a_scale", M), g.w_scale = vector(e, a[5], "w_scale", N), g.bias = vector(e, a[6], "bias", N);
     if (a[3] == Py_None || a[5] == Py_None) refuse("a_scale and w_scale are needed");
     PyObject *resid = a[7], *out = a[11], *resid_out = a[12];
@@ -312,10 +330,10 @@ PyObject* gate_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor* y = maybe(a[2], "y");
     const int64_t M = h.size(0), D = h.size(1);
     EcadGateNorm g{};
-    g.h = h.data_ptr(), g.ldh = rows(e, h, "h", e.dtype, M, D);
+    g.ldh = rows(e, h, "h", e.dtype, M, D), g.h = h.data_ptr();
     g.pre = integer32(a[3], "pre"), g.post = integer32(a[4], "post"), g.rows_per_batch = integer32(a[13], "rows_per_batch");
     const bool quantize = truth(a[16]);
-    if (y) g.y = y->data_ptr(), g.ldy = rows(e, *y, "y", e.dtype, M, D);
+    if (y) g.ldy = rows(e, *y, "y", e.dtype, M, D), g.y = y->data_ptr();
     g.pre_weight = vector(e, a[5], "pre_weight", D), g.post_weight = vector(e, a[6], "post_weight", D), g.gate_table = vector(e, a[7], "gate_table", D);
     g.table_shift = vector(e, a[9], "table_shift", D), g.table_scale = vector(e, a[10], "table_scale", D);
     const Mod gm = modulation(e, a[8], "gate_mod", M, D, g.rows_per_batch), ms = modulation(e, a[11], "mod_shift", M, D, g.rows_per_batch), mc = modulation(e, a[12], "mod_scale", M, D, g.rows_per_batch);

@@ -41,3 +41,40 @@ def test_forward_mode_tangents_are_refused(accepting):  # noqa: F811
             with torch.inference_mode():
                 call()
         accepting.op_gate_norm(forward_ad.unpack_dual(dual).primal)
+
+
+def test_tracing_is_refused(accepting):  # noqa: F811
+    """A tracer would record the allocation of the result and nothing that fills it."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    h, out = f16(4, 24), f16(4, 24)
+    norm = lambda x: accepting.op_gate_norm(x)[1]  # noqa: E731
+    for trace in (lambda: make_fx(norm)(h), lambda: make_fx(norm, tracing_mode="fake")(h), lambda: torch.jit.trace(norm, (h,), check_trace=False)):
+        with pytest.raises(RuntimeError, match="traced"):
+            trace()
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        with pytest.raises(RuntimeError, match="traced"):
+            norm(h)
+        with pytest.raises(RuntimeError, match="traced"):
+            accepting.op_gate_norm(h, out_n=out)  # nothing fake in it: it would run
+    fake = mode.from_tensor(h)
+    for call in (lambda: norm(fake), lambda: accepting.op_gate_norm(h, pre_weight=mode.from_tensor(f32(24))), lambda: torch.func.functionalize(norm)(h)):
+        with pytest.raises(RuntimeError, match="holds no values"):
+            call()
+    for transform in (lambda: torch.func.jvp(norm, (h,), (h,)), lambda: torch.func.grad(lambda x: norm(x).sum())(h), lambda: torch.vmap(norm)(f16(2, 4, 24))):
+        with pytest.raises(RuntimeError):
+            transform()
+    assert not accepting.calls.records
+
+
+def test_modes_that_only_watch_are_not_tracing(accepting):  # noqa: F811
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    with Watch():
+        accepting.op_gate_norm(f16(4, 24))
+    assert len(accepting.calls.records) == 1
