@@ -120,9 +120,15 @@ bool stands_in(const Tensor& t) {
   return t.key_set().has_any(kinds);
 }
 
+// values that are not what the memory says: the lazily negated ones of x.conj().imag, the zeros without memory of forward-mode differentiation
+bool lazy(const Tensor& t) {
+  static const c10::DispatchKeySet kinds({c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor});
+  return t.key_set().has_any(kinds);
+}
+
 // on the engine's device, of that type and shape, with memory of its own; gradients are not recorded by these operators, tangents not carried on
 void check(const Engine& e, const Tensor& t, const char* name, at::ScalarType type, at::IntArrayRef shape, Dense how) {
-  if (t.scalar_type() == type && t.device() == e.device && t.sizes() == shape && dense(t, how) && !(t.requires_grad() && c10::GradMode::is_enabled()) && !has_tangent(t) && !stands_in(t)) return;
+  if (t.scalar_type() == type && t.device() == e.device && t.sizes() == shape && dense(t, how) && !(t.requires_grad() && c10::GradMode::is_enabled()) && !has_tangent(t) && !stands_in(t) && !lazy(t)) return;
   if (stands_in(t)) throw std::runtime_error(std::string(name) + " is a tensor that holds no values itself (traced, transformed, or a subclass with a dispatch of its own)");
   if (t.device() != e.device) refuse("%s is on %s, this engine on %s", name, t.device().str().c_str(), e.device.str().c_str());
   if (t.scalar_type() != type) {
@@ -131,6 +137,7 @@ void check(const Engine& e, const Tensor& t, const char* name, at::ScalarType ty
   }
   if (t.sizes() != shape) refuse("%s must have shape %s, got %s", name, text(shape).c_str(), text(t.sizes()).c_str());
   if (!dense(t, how)) refuse("%s must %s, got strides %s", name, how == WHOLE ? "be contiguous" : "have a dense last dimension", text(t.strides()).c_str());
+  if (lazy(t)) refuse("%s is lazily negated or a zero without memory: its memory does not hold its values (resolve_neg(), or clone it)", name);
   if (has_tangent(t)) refuse("%s has a forward-mode tangent: this op carries none on (take unpack_dual(...).primal, or switch forward gradients off)", name);
   refuse("%s requires a gradient: this op has none (detach it, or call under torch.no_grad())", name);
 }

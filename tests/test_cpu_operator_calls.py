@@ -78,3 +78,14 @@ def test_modes_that_only_watch_are_not_tracing(accepting):  # noqa: F811
     with Watch():
         accepting.op_gate_norm(f16(4, 24))
     assert len(accepting.calls.records) == 1
+
+
+def test_lazily_negated_tensors_are_refused(accepting):  # noqa: F811
+    """Their memory holds the values with the other sign, a zero tensor's holds nothing."""
+    h, w = f16(4, 24), torch.complex(torch.ones(1), torch.ones(1)).conj().imag
+    assert w.is_neg() and w.is_contiguous()
+    for call in [lambda: accepting.op_gate_norm(f16(4, 1), pre_weight=w), lambda: accepting.op_gate_norm(h, h.clone(), out_h=torch._neg_view(h)), lambda: accepting.op_quantize_int8(torch._neg_view(h)),
+                 lambda: accepting.op_quantize_int8(torch._efficientzerotensor(4, 24, dtype=torch.float16))]:
+        with pytest.raises(ValueError, match="lazily negated"):
+            call()
+    accepting.op_gate_norm(f16(4, 1), pre_weight=w.resolve_neg())
