@@ -180,13 +180,19 @@ int32_t size32(int64_t v, const char* what) {
 
 Tensor fresh(const Engine& e, at::IntArrayRef shape, at::ScalarType type) { return at::empty(shape, at::TensorOptions().dtype(type).device(e.device)); }
 
+// behind the launch: a tensor of the caller's has other values now, and whoever has saved it for a backward pass is told so (inference tensors count no versions)
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // an output: the caller's tensor, or a new one
 struct Out {
   PyObject* given = nullptr;
   Tensor made;
   const Tensor& t() const { return given ? THPVariable_Unpack(given) : made; }
-  PyObject* object() {
+  PyObject* object() {  // once, behind the launch
     if (given) {
+      written(t());
       Py_INCREF(given);
       return given;
     }
@@ -323,6 +329,7 @@ PyObject* gemm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (kept) g.out = o.t().data_ptr();
     g.M = size32(M, "row count"), g.N = size32(N, "width"), g.K = size32(K, "depth"), g.kernel = integer32(a[13], "kernel");
     launch(e, [&](void* s) { return e.gemm(e.handle, &g, s); });
+    if (g.epi == 3) written(THPVariable_Unpack(resid_out));
     if (kept) return o.object();
     Py_RETURN_NONE;
   });

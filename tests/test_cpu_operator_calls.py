@@ -4,7 +4,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 from ecad_amd import _lib as L
-from test_cpu_operators import AT, _Norm, accepting, f16, f32, i8, library  # noqa: F401  (accepting, library: fixtures)
+from test_cpu_operators import AT, _Norm, accepting, eng, f16, f32, i8, library  # noqa: F401  (accepting, eng, library: fixtures)
 
 
 def test_no_rows_into_given_8bit_outputs(accepting):  # noqa: F811
@@ -89,3 +89,41 @@ def test_lazily_negated_tensors_are_refused(accepting):  # noqa: F811
         with pytest.raises(ValueError, match="lazily negated"):
             call()
     accepting.op_gate_norm(f16(4, 1), pre_weight=w.resolve_neg())
+
+
+def test_what_is_written_in_place_has_a_new_version(accepting, eng):  # noqa: F811
+    """Autograd's saved tensors are checked by it."""
+    h, y, n, q8, s = f16(4, 24), f16(4, 24), f16(4, 24), i8(4, 24), f32(4)
+    w, sw, r, r2, o, t, pos = i8(24, 24), f32(24), f16(4, 24), f16(4, 24), f16(4, 24), f32(3, 8, 2), torch.zeros(3, dtype=torch.int32)
+    q, k, q2, k2 = f16(2, 3, 4, 16), f16(2, 3, 2, 16), f16(2, 3, 4, 16), f16(2, 3, 2, 16)
+    for outs, ins, call in [
+        ([q8, s], [h], lambda e: e.op_quantize_int8(h, out=(q8, s))),
+        ([o], [q8, s, w, sw], lambda e: e.op_gemm_int8(0, q8, s, w, sw, out=o)),
+        ([r], [q8, s, w, sw], lambda e: e.op_gemm_int8(3, q8, s, w, sw, resid=r)),
+        ([r2, o], [r], lambda e: e.op_gemm_int8(3, q8, s, w, sw, resid=r, resid_out=r2, out=o)),
+        ([h, y], [], lambda e: e.op_gate_norm(h, y, out_h=h, out_n=y)),
+        ([n], [h], lambda e: e.op_gate_norm(h, out_n=n)),
+        ([q8, s], [h], lambda e: e.op_gate_norm(h, quantize=True, out_n=(q8, s))),
+        ([t], [pos], lambda e: e.op_rope_table(pos, 16, out=t)),
+        ([q, k], [t], lambda e: e.op_rope(q, k, t, out=(q, k))),
+        ([q2, k2], [q, k, t], lambda e: e.op_rope(q, k, t, out=(q2, k2))),
+    ]:
+        before = [x._version for x in outs + ins]
+        call(accepting)
+        assert [x._version - b for x, b in zip(outs + ins, before)] == [1] * len(outs) + [0] * len(ins)
+        before = [x._version for x in outs]
+        with pytest.raises(RuntimeError, match="was called"):  # a launch that failed has written nothing
+            call(eng)
+        assert [x._version for x in outs] == before
+    wide = f16(4, 48)
+    accepting.op_gate_norm(h, out_n=wide[:, :24])  # a view's version is its base's
+    assert wide._version == 1
+    x = torch.ones(4, 24, dtype=torch.float16, requires_grad=True)
+    product = x * h
+    accepting.op_gate_norm(h, y, out_h=h)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+    with torch.inference_mode():
+        inside = f16(4, 24)
+        accepting.op_gate_norm(h, out_n=inside)
+    accepting.op_gate_norm(h, out_n=inside)  # no version to count
