@@ -40,11 +40,12 @@
 #include "attention_w472.h"
 #include "gemm3s.h"
 #include "gemm3s8.h"
+#include "last_error.h"
 #include "operators.h"
 
 namespace ecad {
 
-static std::string g_create_error;
+static LastError g_create_error;
 constexpr int PROJ_PAD = 144;  // proj_out rows padded to one GEMM tile column
 
 #define HIPCHK(expr)                                                                         \
@@ -64,7 +65,7 @@ static const char* kclass_names[KC_COUNT] = {
 struct EngineBase {
   EcadModelCfg cfg;
   int dev = 0;
-  std::string err;
+  LastError err;
   virtual ~EngineBase() {}
   int fail(int code, const char* fmt, ...) {
     char buf[1024];
@@ -72,7 +73,7 @@ struct EngineBase {
     va_start(ap, fmt);
     vsnprintf(buf, sizeof buf, fmt, ap);
     va_end(ap);
-    err = buf;
+    err.set(buf);
     return code;
   }
   virtual int init() = 0;
@@ -2254,9 +2255,7 @@ template <typename F> int run_operator(EngineBase* E, void* stream, F&& op) {
       rc = op(OpCtx{E->cfg.dtype, op_num_cus(E->dev), (hipStream_t)stream}, st);
     }
   }
-  if (rc) {
-    try { E->err = st.msg; } catch (...) {}
-  }
+  if (rc) E->err.set(st.msg);
   return rc;
 }
 }  // namespace
@@ -2266,23 +2265,23 @@ extern "C" {
 int ecad_abi_version(void) { return ECAD_ABI_VERSION; }
 
 int ecad_create(const EcadModelCfg* cfg, int device, EcadEngine** out) {
-  if (!cfg || !out) { g_create_error = "NULL argument"; return ECAD_E_INVALID; }
+  if (!cfg || !out) { g_create_error.set("NULL argument"); return ECAD_E_INVALID; }
   int ndev = 0;
-  if (hipGetDeviceCount(&ndev) != hipSuccess || ndev == 0) { g_create_error = "no HIP device visible"; return ECAD_E_HIP; }
-  if (device < 0 || device >= ndev) { g_create_error = "device index out of range"; return ECAD_E_INVALID; }
+  if (hipGetDeviceCount(&ndev) != hipSuccess || ndev == 0) { g_create_error.set("no HIP device visible"); return ECAD_E_HIP; }
+  if (device < 0 || device >= ndev) { g_create_error.set("device index out of range"); return ECAD_E_INVALID; }
   EngineBase* impl = nullptr;
   if (cfg->dtype == ECAD_DTYPE_F16) impl = new EngineT<f16_t>();
   else if (cfg->dtype == ECAD_DTYPE_BF16) impl = new EngineT<bf16_t>();
-  else { g_create_error = "dtype must be ECAD_DTYPE_F16 or ECAD_DTYPE_BF16"; return ECAD_E_INVALID; }
+  else { g_create_error.set("dtype must be ECAD_DTYPE_F16 or ECAD_DTYPE_BF16"); return ECAD_E_INVALID; }
   impl->cfg = *cfg;
   impl->dev = device;
   int rc = impl->init();
-  if (rc) { g_create_error = impl->err; delete impl; return rc; }
+  if (rc) { g_create_error.set(impl->err.get()); delete impl; return rc; }
   *out = new EcadEngine{impl};
   return ECAD_OK;
 }
 void ecad_destroy(EcadEngine* e) { if (e) { delete e->impl; delete e; } }
-const char* ecad_last_error(const EcadEngine* e) { return e ? e->impl->err.c_str() : g_create_error.c_str(); }
+const char* ecad_last_error(const EcadEngine* e) { return e ? e->impl->err.get() : g_create_error.get(); }
 
 #define ENG(e) if (!(e)) return ECAD_E_INVALID; EngineBase* E = (e)->impl
 

@@ -92,7 +92,9 @@ typedef struct EcadEngine EcadEngine;
 /* Replaces PixArtTransformer2DEdited.__init__/_post_init (pixart_transformer_2d_edited.py:23-102). */
 int ecad_create(const EcadModelCfg* cfg, int device, EcadEngine** out);
 void ecad_destroy(EcadEngine* e);
-const char* ecad_last_error(const EcadEngine* e); /* e may be NULL: last create() error */
+/* Message of the calling thread's last failed call on e, or, where it had none, of the engine's; e may be NULL: of ecad_create.  Good until this thread's next failed call or
+ * next question.  Never NULL. */
+const char* ecad_last_error(const EcadEngine* e);
 int ecad_abi_version(void);
 
 /* Replaces from_pretrained + init_cached_transformer_blocks weight copy (:104-153).  `name` is the

@@ -1,4 +1,7 @@
 """Calls of the operators of an 8-bit transformer block that the documentation allows, without a GPU: an engine whose library answers that all is well."""
+import ctypes as C
+import threading
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -127,3 +130,29 @@ def test_what_is_written_in_place_has_a_new_version(accepting, eng):  # noqa: F8
         inside = f16(4, 24)
         accepting.op_gate_norm(h, out_n=inside)
     accepting.op_gate_norm(h, out_n=inside)  # no version to count
+
+
+def test_every_thread_finds_its_own_message():
+    """Calls that fail in two threads at once; both without a device (no configuration, and a device that is not there)."""
+    lib, wrong = L.load(), []
+
+    def fail(call, says):
+        for _ in range(4000):
+            if call() == 0 or lib.ecad_last_error(None) not in says:
+                wrong.append(lib.ecad_last_error(None))
+                return
+
+    cfg, handle = L.EcadModelCfg(), C.c_void_p()
+    calls = [(lambda: lib.ecad_create(None, 0, None), (b"NULL argument",)), (lambda: lib.ecad_create(C.byref(cfg), 1 << 20, C.byref(handle)), (b"no HIP device visible", b"device index out of range"))]
+    threads = [threading.Thread(target=fail, args=c) for c in calls * 2]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    assert calls[0][0]() != 0 and lib.ecad_last_error(None) == b"NULL argument"
+    seen = []
+    t = threading.Thread(target=lambda: seen.append(lib.ecad_last_error(None)))  # a thread that had none: the last one of all
+    t.start()
+    t.join()
+    assert seen == [b"NULL argument"]
