@@ -10,9 +10,11 @@
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 
+#include <chrono>
 #include <cstdarg>
 #include <memory>
 #include <string>
+#include <thread>
 #include <utility>
 
 #include "../../include/ecad_hip.h"
@@ -34,6 +36,8 @@ struct Engine {
   c10::Device device{c10::DeviceType::CPU};
   PyObject* stream_of;  // callable(device index) -> hipStream_t as an integer
   PyObject* index;
+  int running = 0;      // calls in the library; read and written with the interpreter's lock
+  bool closed = false;
 };
 const char* const ENGINE = "ecad_amd._ops.Engine";
 
@@ -64,12 +68,15 @@ void refuse_tracing() {
   if (recorded || at::tracer::impl::is_dispatch_enabled()) throw std::runtime_error("this op cannot be traced: it is a call into the library that a recorded graph would not hold");
 }
 
-const Engine& engine_of(PyObject* o) {
-  refuse_tracing();
-  if (o == Py_None) throw std::runtime_error("the engine is closed");
+Engine& held(PyObject* o) {
   void* p = PyCapsule_GetPointer(o, ENGINE);
   if (!p) throw python_error();
   return *static_cast<Engine*>(p);
+}
+Engine& engine_of(PyObject* o) {
+  refuse_tracing();
+  if (o == Py_None || held(o).closed) throw std::runtime_error("the engine is closed");
+  return held(o);
 }
 const Tensor* maybe(PyObject* o, const char* name) {
   if (o == Py_None) return nullptr;
@@ -252,12 +259,17 @@ void* stream(const Engine& e) {
   if (!s && PyErr_Occurred()) throw python_error();
   return s;
 }
-// f: the entry point alone.  The interpreter's lock stays held: the call only launches, in less time than handing the lock over and back may take, and an engine has one
-// last error -- two threads that are refused at once would write it at once.
-template <typename F> void launch(const Engine& e, F&& f) {
-  const int rc = f(stream(e));
+// f: the entry point alone, without the interpreter's lock: a launch waits where the device's queue is full, and the other threads do not.  close() waits for it.
+template <typename F> void launch(Engine& e, F&& f) {
+  void* const s = stream(e);
+  if (e.closed) throw std::runtime_error("the engine is closed");  // (by a thread that ran meanwhile)
+  ++e.running;
+  PyThreadState* const state = PyEval_SaveThread();
+  const int rc = f(s);
+  PyEval_RestoreThread(state);
+  --e.running;
   if (rc == ECAD_OK) return;
-  const char* m = e.last_error(e.handle);
+  const char* m = e.last_error(e.handle);  // this thread's own
   const std::string message = m && *m ? m : "error " + std::to_string(rc);
   if (rc == ECAD_E_INVALID || rc == ECAD_E_UNSUPPORTED) throw Refused{message};
   throw std::runtime_error(message);
@@ -283,7 +295,7 @@ template <typename F> PyObject* guarded(F&& f) {
 PyObject* quantize_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     arguments(n, 3);
-    const Engine& e = engine_of(a[0]);
+    Engine& e = engine_of(a[0]);
     const Tensor& x = matrix(a[1], "x");
     const int64_t M = x.size(0), K = x.size(1), ldx = rows(e, x, "x", e.dtype, M, K);
     const int32_t m = size32(M, "row count"), k = size32(K, "width");
@@ -300,7 +312,7 @@ PyObject* quantize_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* gemm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     arguments(n, 14);
-    const Engine& e = engine_of(a[0]);
+    Engine& e = engine_of(a[0]);
     const Tensor &A = matrix(a[2], "a"), &W = matrix(a[4], "w");
     const int64_t M = A.size(0), K = A.size(1), N = W.size(0);
     EcadInt8Gemm g{};
@@ -339,7 +351,7 @@ PyObject* gemm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* gate_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     arguments(n, 19);
-    const Engine& e = engine_of(a[0]);
+    Engine& e = engine_of(a[0]);
     const Tensor& h = matrix(a[1], "h");
     const Tensor* y = maybe(a[2], "y");
     const int64_t M = h.size(0), D = h.size(1);
@@ -395,7 +407,7 @@ PyObject* gate_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* rope_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     arguments(n, 10);
-    const Engine& e = engine_of(a[0]);
+    Engine& e = engine_of(a[0]);
     const Tensor& p = tensor(a[1], "positions");
     const bool floats = p.scalar_type() == at::kFloat;
     if ((p.dim() != 1 && p.dim() != 2) || (!floats && p.scalar_type() != at::kInt)) refuse("positions must be an int32 or float32 tensor of shape (S,) or (S, axes)");
@@ -432,7 +444,7 @@ PyObject* rope_table(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     arguments(n, 9);
-    const Engine& e = engine_of(a[0]);
+    Engine& e = engine_of(a[0]);
     const Tensor& q = tensor(a[1], "q");
     if (q.dim() != 4) refuse("q must have shape (samples, tokens, heads, elements)");
     const int64_t B = q.size(0), S = q.size(1), D = q.size(3);
@@ -490,6 +502,21 @@ void forget(PyObject* capsule) {
   delete e;
 }
 
+// (engine): no call starts behind this one, and those that run have left the library when it returns
+PyObject* close(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    arguments(n, 1);
+    Engine& e = held(a[0]);
+    e.closed = true;
+    while (e.running) {
+      PyThreadState* const state = PyEval_SaveThread();
+      std::this_thread::sleep_for(std::chrono::microseconds(50));
+      PyEval_RestoreThread(state);
+    }
+    Py_RETURN_NONE;
+  });
+}
+
 // (addresses of the six entry points, engine handle, dtype: 0 fp16 / 1 bf16, device index or -1 for the CPU, stream_of)
 PyObject* engine(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -526,6 +553,7 @@ PyObject* engine(PyObject*, PyObject* const* a, Py_ssize_t n) {
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)> PyCFunction fast() { return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(F)); }
 
 PyMethodDef methods[] = {{"engine", fast<engine>(), METH_FASTCALL, "What an engine gives its calls."},
+                         {"close", fast<close>(), METH_FASTCALL, "No more calls on an engine; waits for those that run."},
                          {"quantize_int8", fast<quantize_int8>(), METH_FASTCALL, "EcadEngine.op_quantize_int8"},
                          {"gemm_int8", fast<gemm_int8>(), METH_FASTCALL, "EcadEngine.op_gemm_int8"},
                          {"gate_norm", fast<gate_norm>(), METH_FASTCALL, "EcadEngine.op_gate_norm"},

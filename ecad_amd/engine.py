@@ -93,9 +93,11 @@ class EcadEngine:
 
     def close(self):
         if getattr(self, "_h", None) and self._h.value:
-            self.lib.ecad_destroy(self._h)
-            self._h = C.c_void_p()
-            self._ops = self._ops and (self._ops[0], None)
+            h, self._h = self._h, C.c_void_p()
+            if self._ops:
+                self._ops[0].close(self._ops[1])  # (calls of other threads have left the library)
+                self._ops = self._ops[0], None
+            self.lib.ecad_destroy(h)
         self._donor = None
 
     def set_ln_fold(self, on: bool) -> None:

@@ -1,12 +1,15 @@
 """Calls of the operators of an 8-bit transformer block that the documentation allows, without a GPU: an engine whose library answers that all is well."""
 import ctypes as C
+import subprocess
 import threading
+import time
 
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
 from ecad_amd import _lib as L
+from ecad_amd.engine import EcadEngine
 from test_cpu_operators import AT, _Norm, accepting, eng, f16, f32, i8, library  # noqa: F401  (accepting, eng, library: fixtures)
 
 
@@ -156,3 +159,59 @@ def test_every_thread_finds_its_own_message():
     t.start()
     t.join()
     assert seen == [b"NULL argument"]
+
+
+@pytest.fixture
+def slow(tmp_path):
+    """An engine whose launches take 0.3 s, as one does while the device's queue is full; `left` counts those that have returned, and `destroyed` what it was when the engine went."""
+    (tmp_path / "slow.c").write_text("""#include <unistd.h>
+int left, destroyed = -1;
+int launch(void) { usleep(300000); ++left; return 0; }
+const char* last_error(void* e) { return ""; }
+void destroy(void* e) { destroyed = left; }
+""")
+    subprocess.run(["gcc", "-shared", "-fPIC", str(tmp_path / "slow.c"), "-o", str(tmp_path / "slow.so")], check=True)
+    lib, ops = C.CDLL(str(tmp_path / "slow.so")), L.load_ops()
+    at = lambda name: C.cast(getattr(lib, name), C.c_void_p).value  # noqa: E731
+    e = object.__new__(EcadEngine)
+    e._h, e.cfg, e._donor = C.c_void_p(1 << 20), L.EcadModelCfg(), None
+    e.lib = type("Library", (), {"ecad_destroy": staticmethod(lib.destroy)})
+    e._ops = ops, ops.engine((at("launch"),) * 5 + (at("last_error"),), 1 << 20, L.ECAD_DTYPE_F16, -1, lambda index: 0)
+    e.count = lambda name: C.c_int.in_dll(lib, name).value
+    return e
+
+
+def test_a_launch_that_waits_stops_no_other_thread(slow):
+    x = f16(4, 24)
+    caller = threading.Thread(target=lambda: slow.op_quantize_int8(x))
+    longest, t = 0.0, time.perf_counter()
+    caller.start()
+    while caller.is_alive():
+        longest, t = max(longest, time.perf_counter() - t), time.perf_counter()
+        time.sleep(0.005)
+    assert slow.count("left") == 1 and longest < 0.25
+
+
+def test_closing_waits_for_the_calls_of_other_threads(slow):
+    x, seen = f16(4, 24), []
+
+    def call():
+        for _ in range(3):
+            try:
+                slow.op_quantize_int8(x)
+            except RuntimeError as e:
+                seen.append(str(e))
+                return
+
+    callers = [threading.Thread(target=call) for _ in range(2)]
+    for t in callers:
+        t.start()
+    time.sleep(0.1)
+    slow.close()
+    assert slow.count("destroyed") == 2
+    for t in callers:
+        t.join()
+    assert seen == ["the engine is closed"] * 2 and slow.count("left") == 2
+    with pytest.raises(RuntimeError, match="closed"):
+        slow.op_quantize_int8(x)
+    slow.close()
