@@ -1,8 +1,10 @@
 """Calls of the operators of an 8-bit transformer block that the documentation allows, without a GPU: an engine whose library answers that all is well."""
 import ctypes as C
 import subprocess
+import sys
 import threading
 import time
+from pathlib import Path
 
 import pytest
 import torch
@@ -215,3 +217,16 @@ def test_closing_waits_for_the_calls_of_other_threads(slow):
     with pytest.raises(RuntimeError, match="closed"):
         slow.op_quantize_int8(x)
     slow.close()
+
+
+def test_the_library_is_built_without_torch():
+    """The default target where Python has no torch (here: no site packages) is the library alone; where it has, the binding too, without a path to that torch in it."""
+    root = Path(__file__).resolve().parents[1]
+    make = lambda python: subprocess.run(["make", "-n", "-B", "-C", str(root / "ecad_amd" / "csrc"), f"PYTHON={python}"], capture_output=True, text=True)  # noqa: E731
+    without, beside = make(f"{sys.executable} -I -S"), make(sys.executable)
+    for run in (without, beside):
+        assert run.returncode == 0 and not run.stderr and "operators.hip" in run.stdout and "-o ../libecad_hip.so" in run.stdout, run.stderr
+    assert "binding.cpp" not in without.stdout and "no torch" in without.stdout
+    assert "binding.cpp" in beside.stdout
+    dynamic = subprocess.run(["readelf", "-d", str(root / "ecad_amd" / "_ops.so")], capture_output=True, text=True, check=True).stdout
+    assert "RPATH" not in dynamic and "RUNPATH" not in dynamic
