@@ -21,7 +21,9 @@ struct RopeTableArgs {
 };
 
 // The angle is counted in quarter turns and reduced in 64 bits: the remainder of p (2 f / pi) from the nearest whole one, |r| <= 1/2, is one fma; only r pi / 2 becomes
-// fp32, so a position of 10^7 is as exact as position 1.  On |a| <= pi / 4 the Taylor sums below end 2e-9 (sine, a^9) and 2e-10 (cosine, a^10) from the function.
+// fp32, so a position of 10^7 is as exact as position 1.  (The frequency itself has 53 bits: the angle
+// is off by 2^-53 of it, which is all of a turn from 2^53 turns on.  Positions beyond come out on the circle, somewhere.)  On |a| <= pi / 4 the Taylor sums below end 2e-9 (sine, a^9) and 2e-10 (cosine, a^10) from the function;
+// their fp32 arithmetic, with the rounding of a, stays within 4.5 2^-24 (64-bit sums would end at 2^-24 of the value, for a table whose rows meet 16-bit heads).
 // A thread keeps its pair (frequency and axis are read once) and steps through rows; half a dozen 64-bit operations per pair keep the kernel near its stores (8
 // bytes per pair): 131072 x 64 pairs in 15.8 us (4.3 TB/s; with a division per pair to find the row 22.9), 16384 x 64 in 5.0.
 __global__ __launch_bounds__(1024) void rope_table_kernel(const RopeTableArgs p) {
@@ -33,8 +35,13 @@ __global__ __launch_bounds__(1024) void rope_table_kernel(const RopeTableArgs p)
   for (int64_t row = (int64_t)blockIdx.x * p.rows_per_block + r0; row < p.S; row += step) {
     const int64_t at = row * p.axes + axis;
     const double pos = p.positions_float ? (double)reinterpret_cast<const float*>(p.positions)[at] : (double)reinterpret_cast<const int32_t*>(p.positions)[at];
-    const double whole = rint(pos * quarters);
-    const float a = (float)(__builtin_fma(pos, quarters, -whole) * 1.5707963267948966);
+    double whole = rint(pos * quarters), rest = __builtin_fma(pos, quarters, -whole);
+    if (fabs(whole) >= 0x1p50) {  // (fp32 positions only) the product's own rounding is no longer small: whole quarters are left in the rest
+      const double more = rint(rest);
+      rest -= more;
+      whole = 4.0 * (0.25 * whole - floor(0.25 * whole)) + 4.0 * (0.25 * more - floor(0.25 * more));
+    }
+    const float a = (float)(rest * 1.5707963267948966);
     const float a2 = a * a;
     const float sn = a * (1.f + a2 * (-1.f / 6 + a2 * (1.f / 120 + a2 * (-1.f / 5040 + a2 * (1.f / 362880)))));
     const float cs = 1.f + a2 * (-0.5f + a2 * (1.f / 24 + a2 * (-1.f / 720 + a2 * (1.f / 40320 + a2 * (-1.f / 3628800)))));

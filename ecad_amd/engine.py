@@ -463,7 +463,8 @@ class EcadEngine:
     ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 
     def op_rope_table(self, positions, axes_dims, theta=10000.0, scaling="none", factor=1.0, original_length=0, beta_fast=32.0, beta_slow=1.0, out=None) -> torch.Tensor:
-        """Cosines and sines of rotary positions (``ecad_op_rope_table``): positions [S] or [S, axes] int32 or fp32 -> [S, sum(axes_dims) / 2, 2] fp32, angles in 64 bits.
+        """Cosines and sines of rotary positions (``ecad_op_rope_table``): positions [S] or [S, axes] int32 or fp32 -> [S, sum(axes_dims) / 2, 2] fp32: angles reduced in 64 bits, their
+        functions within 4.5 * 2^-24.
         axes_dims: elements that turn with each axis (even; an int for one axis), e.g. (16, 56, 56) for FLUX's (index, row, column).  scaling "linear" (f / factor), "ntk" (theta
         factor^(d / (d - 2))) or "yarn" (pairs that turn often within ``original_length`` stay, the others are stretched; cosine and sine times 0.1 ln(factor) + 1)."""
         ops, engine = self._ops or self._native()

@@ -340,7 +340,8 @@ typedef struct EcadGateNorm {
 } EcadGateNorm;
 int ecad_op_gate_norm(EcadEngine* e, const EcadGateNorm* args, void* stream);
 
-/* table[S][pairs][2] = m (cos, sin)(p[s][axis(j)] f_j), angles in 64 bits.  positions [S][axes] int32 (positions_float 0) or fp32 (1); the pairs of the axes follow each
+/* table[S][pairs][2] = m (cos, sin)(p[s][axis(j)] f_j): the angle is reduced in 64 bits, the functions of what remains are fp32 sums, within 4.5 * 2^-24 m of the true ones
+ * wherever the 64-bit angle is (positions of 2^53 / f and beyond have no place in the turn: they come out on the circle, somewhere).  positions [S][axes] int32 (positions_float 0) or fp32 (1); the pairs of the axes follow each
  * other, axes_dims[a] / 2 (host array) on axis a, f = theta^(-2 j / axes_dims[a]).  Scalings for positions beyond the trained ones, by `factor`:
  *   LINEAR  f / factor
  *   NTK     theta * factor^(d / (d - 2)) in place of theta (axes of two elements: theta)

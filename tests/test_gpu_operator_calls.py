@@ -23,3 +23,15 @@ def test_no_rows():
     assert nh.shape == (0, 24) and n is None
     torch.cuda.synchronize()
     assert bool((q == 9).all()) and bool((s == 9).all())
+
+
+def test_rope_table_of_positions_without_a_place_in_the_turn():
+    """Beyond 2^53 quarters the angle's 64 bits do not say where in the turn it is; cosine and sine are still those of one angle: each within 4.5 * 2^-24, so their squares' sum
+    within 2 * 4.5 * 2^-24 * (|c| + |s|) <= 13 * 2^-24 of 1."""
+    pos = torch.tensor([2.0**49, 2.0**50, 2.0**51, 2.0**52, 1e16, 1e17, -1e17, 1.3e18, -1.3e18, 1e20, 7e25, 1e30, -2e35, 3.4e38], device="cuda")
+    for dims in (2, 64):
+        table = small_engine().op_rope_table(pos, dims, theta=500000.0).double()
+        assert float(((table**2).sum(-1) - 1).abs().max()) <= 13 * STEP
+    near_ones = torch.tensor([2.0**30, -(2.0**33), 2.0**36], device="cuda")  # the angle is off by 2^-53 of it at most: 2^-17 at 2^36
+    ref, _ = table64(near_ones, (2,))
+    assert float((small_engine().op_rope_table(near_ones, 2).double() - ref).abs().max()) <= 4.5 * STEP + 2.0**-17
