@@ -397,7 +397,8 @@ int op_rope(const OpCtx& ctx, const EcadRope& c, OpStatus& st) noexcept {
   if (negative(c.q) || (c.k.H && negative(c.k)) || c.index_stride < 0) return refuse(st, ECAD_E_INVALID, "rope: a stride is negative");
   const bool q_in = c.q.x == c.q.out, k_in = c.k.H == 0 || c.k.x == c.k.out;
   if (c.k.H && q_in != k_in) return refuse(st, ECAD_E_INVALID, "rope: queries and keys are both turned in place or both not");
-  auto same = [](const EcadRopeHeads& x) { return x.sample == x.out_sample && x.token == x.out_token && x.head == x.out_head; };
+  // (a stride over one sample, token or head is never taken)
+  auto same = [&](const EcadRopeHeads& x) { return (c.B == 1 || x.sample == x.out_sample) && (c.S == 1 || x.token == x.out_token) && (x.H == 1 || x.head == x.out_head); };
   if (q_in && (!same(c.q) || (c.k.H && !same(c.k)))) return refuse(st, ECAD_E_INVALID, "rope: in place needs the same strides on both sides");
   auto in_of = [&](const EcadRopeHeads& x) { return Region{x.H ? (const char*)x.x : nullptr, {1, c.B, c.S, x.H}, {0, 2 * x.sample, 2 * x.token, 2 * x.head}, (int64_t)2 * c.D}; };
   auto out_of = [&](const EcadRopeHeads& x) { return Region{x.H ? (const char*)x.out : nullptr, {1, c.B, c.S, x.H}, {0, 2 * x.out_sample, 2 * x.out_token, 2 * x.out_head}, (int64_t)2 * c.D}; };

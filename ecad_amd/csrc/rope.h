@@ -36,7 +36,7 @@ __global__ __launch_bounds__(1024) void rope_table_kernel(const RopeTableArgs p)
     const int64_t at = row * p.axes + axis;
     const double pos = p.positions_float ? (double)reinterpret_cast<const float*>(p.positions)[at] : (double)reinterpret_cast<const int32_t*>(p.positions)[at];
     double whole = rint(pos * quarters), rest = __builtin_fma(pos, quarters, -whole);
-    if (fabs(whole) >= 0x1p50) {  // (fp32 positions only) the product's own rounding is no longer small: whole quarters are left in the rest
+    if (fabs(whole) >= 0x1p50) {  // the product's own rounding is no longer small: whole quarters are left in the rest
       const double more = rint(rest);
       rest -= more;
       whole = 4.0 * (0.25 * whole - floor(0.25 * whole)) + 4.0 * (0.25 * more - floor(0.25 * more));

@@ -35,3 +35,19 @@ def test_rope_table_of_positions_without_a_place_in_the_turn():
     near_ones = torch.tensor([2.0**30, -(2.0**33), 2.0**36], device="cuda")  # the angle is off by 2^-53 of it at most: 2^-17 at 2^36
     ref, _ = table64(near_ones, (2,))
     assert float((small_engine().op_rope_table(near_ones, 2).double() - ref).abs().max()) <= 4.5 * STEP + 2.0**-17
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_rope_in_place_through_another_view(layout):
+    """One token a sample, one sample, one head: the stride of such a dimension differs from view to view and means nothing."""
+    eng, dt = small_engine("float16"), torch.float16
+    table = eng.op_rope_table(torch.arange(9, device="cuda", dtype=torch.int32) + 5, 24)
+    for B, S, H in ((4, 1, 3), (1, 9, 3), (5, 9, 1), (1, 1, 1)):
+        wide = rand(B, S, 2 * H, 24, seed=B + S, dtype=dt)
+        q, k = wide[:, :, :H], wide[:, :, H:]
+        expected = eng.op_rope(q, k, table, layout=layout)
+        strides = [x if n > 1 else 7 + i for i, (n, x) in enumerate(zip(q.shape, q.stride()))]
+        outs = tuple(x.as_strided(x.shape, strides, x.storage_offset()) for x in (q, k))
+        assert outs[0].stride() != q.stride()
+        eng.op_rope(q, k, table, layout=layout, out=outs)
+        assert torch.equal(q, expected[0]) and torch.equal(k, expected[1])
