@@ -390,7 +390,7 @@ int op_rope(const OpCtx& ctx, const EcadRope& c, OpStatus& st) noexcept {
     return refuse(st, ECAD_E_INVALID, "rope: %d samples of %d tokens, %lld + %lld heads of %d elements, %d of them turned (even, 2 to the head's size)", c.B, c.S,
                   (long long)c.q.H, (long long)c.k.H, c.D, c.rot);
   if (c.B == 0 || c.S == 0) return ECAD_OK;
-  if (!c.q.x || !c.q.out || (c.k.H && (!c.k.x || !c.k.out)) || !c.table) return refuse(st, ECAD_E_INVALID, "rope: NULL pointer");
+  if (!c.q.x || !c.q.out || (c.k.H && (!c.k.x || !c.k.out)) || (!c.table && c.table_rows)) return refuse(st, ECAD_E_INVALID, "rope: NULL pointer");  // (no rows: every index lies outside)
   if (!aligned(c.q.x, 2) || !aligned(c.q.out, 2) || !aligned(c.k.x, 2) || !aligned(c.k.out, 2) || !aligned(c.table, 4) || !aligned(c.index, 4)) return refuse(st, ECAD_E_INVALID, "rope: pointers are not aligned to their type");
   if (!c.index && c.table_rows < c.S) return refuse(st, ECAD_E_INVALID, "rope: the table has %d rows for %d tokens", c.table_rows, c.S);
   auto negative = [](const EcadRopeHeads& x) { return x.sample < 0 || x.token < 0 || x.head < 0 || x.out_sample < 0 || x.out_token < 0 || x.out_head < 0; };

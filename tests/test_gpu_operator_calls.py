@@ -51,3 +51,17 @@ def test_rope_in_place_through_another_view(layout):
         assert outs[0].stride() != q.stride()
         eng.op_rope(q, k, table, layout=layout, out=outs)
         assert torch.equal(q, expected[0]) and torch.equal(k, expected[1])
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_rope_with_an_empty_table(layout):
+    """Every index lies outside it: no token turns."""
+    eng, q = small_engine("float16"), rand(2, 5, 3, 24, seed=1, dtype=torch.float16)
+    table, index = torch.empty(0, 8, 2, device="cuda"), torch.zeros(5, dtype=torch.int32, device="cuda")
+    out, _ = eng.op_rope(q, None, table, layout=layout, index=index)
+    assert torch.equal(out, q)
+    x = q.clone()
+    eng.op_rope(x, None, table, layout=layout, index=index, out=(x, None))
+    assert torch.equal(x, q)
+    with pytest.raises(ValueError, match="0 rows for 5 tokens"):
+        eng.op_rope(q, None, table, layout=layout)
