@@ -2,10 +2,10 @@
 """Build audit of the kernels whose K loops are generated asm statements (gemm4.h, gemm2w4.h, attention_w4.h): hipcc knows the AGPRs only as clobbers of the statement,
 so once the statement is behind it they are free registers to its allocator -- and a C++ epilogue short of VGPRs spills INTO them.  That is harmless after the last
 accumulator read (`g4_acc`: v_accvgpr_read inside its own small asm statements) and silently wrong before it (round 5: the read-modify-write epilogue of gemm2w4.h; the
-fix was to round the accumulators into the C tile inside the statement).  This script compiles the two translation units to assembly and reports, per kernel, compiler-issued
+fix was to round the accumulators into the C tile inside the statement).  This script compiles the translation units to assembly and reports, per kernel, compiler-issued
 AGPR accesses (outside ;;#ASMSTART .. ;;#ASMEND) and whether any of them comes before the kernel's last accumulator read.  Exit status 1 on a hazard.
 
-    python scripts/audit_agpr.py                        # compiles both units with the product flags (~4 minutes of hipcc)
+    python scripts/audit_agpr.py                        # compiles all units with the product flags (~8 minutes of hipcc)
     python scripts/audit_agpr.py --asm build/engine-hip-amdgcn-amd-amdhsa-gfx950.s ...   # audits the assembly the product build kept (-save-temps): what the Makefile runs
 
 The product build runs the second form on the very assembly its objects were made from (ecad_amd/csrc/Makefile), so `make` -- and with it `__graft_entry__.build()` -- fails on
@@ -19,7 +19,10 @@ import tempfile
 from pathlib import Path
 
 ROOT = Path(__file__).resolve().parents[1]
-FLAGS = "-O3 -std=c++17 --offload-arch=gfx950 -fPIC -fno-gpu-rdc -ffast-math -fno-finite-math-only -DECAD_PRODUCT_BUILD -S --cuda-device-only".split()  # BASEFLAGS of the Makefile
+# the Makefile's flags of the units (CXXFLAGS), for device assembly
+COMMON = "-O3 -std=c++17 --offload-arch=gfx950 -fPIC -fno-gpu-rdc -DECAD_PRODUCT_BUILD -S --cuda-device-only".split()
+FAST = "-ffast-math -fno-finite-math-only".split()
+UNITS = {"flux.hip": FAST, "engine.hip": FAST, "vae.hip": FAST, "operators.hip": "-ffp-contract=fast -Xclang -target-feature -Xclang -packed-fp32-ops".split()}
 KERNELS = ("fgemm4", "fgemm48", "attn_w4a", "attn_w472", "gemm2w4", "gemm3s4", "conv4", "gemm_int8_wide")
 
 
@@ -72,9 +75,9 @@ def main() -> int:
             total += 1
         return 1 if bad else 0
     with tempfile.TemporaryDirectory() as td:
-        for unit in ("flux.hip", "engine.hip", "vae.hip"):
+        for unit, flags in UNITS.items():
             out = Path(td) / (unit + ".s")
-            subprocess.run(["/opt/rocm/bin/hipcc", *FLAGS, str(ROOT / "ecad_amd" / "csrc" / unit), "-o", str(out)], check=True, stderr=subprocess.DEVNULL)
+            subprocess.run(["/opt/rocm/bin/hipcc", *COMMON, *flags, str(ROOT / "ecad_amd" / "csrc" / unit), "-o", str(out)], check=True, stderr=subprocess.DEVNULL)
             bad += audit(out.read_text(), unit)
     return 1 if bad else 0
 

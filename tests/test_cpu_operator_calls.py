@@ -230,3 +230,21 @@ def test_the_library_is_built_without_torch():
     assert "binding.cpp" in beside.stdout
     dynamic = subprocess.run(["readelf", "-d", str(root / "ecad_amd" / "_ops.so")], capture_output=True, text=True, check=True).stdout
     assert "RPATH" not in dynamic and "RUNPATH" not in dynamic
+
+
+def test_the_accumulator_audit_covers_every_unit():
+    """scripts/audit_agpr.py by itself compiles what the Makefile does, with its flags."""
+    root = Path(__file__).resolve().parents[1]
+    sys.path.insert(0, str(root / "scripts"))
+    try:
+        import audit_agpr
+    finally:
+        sys.path.pop(0)
+    run = subprocess.run(["make", "-n", "-B", "-C", str(root / "ecad_amd" / "csrc")], capture_output=True, text=True, check=True).stdout
+    built = {}
+    for line in run.splitlines():
+        if "-save-temps -c ../" in line:
+            built[line.split("-save-temps -c ../")[1].split()[0]] = set(line.split("hipcc ")[1].split(" -save-temps")[0].split())
+    assert set(built) == set(audit_agpr.UNITS)
+    for unit, flags in built.items():
+        assert flags - {"-Wall", "-Wno-unused-function"} == set(audit_agpr.COMMON + audit_agpr.UNITS[unit]) - {"-S", "--cuda-device-only"}, unit
