@@ -2,6 +2,7 @@
 // call into libecad_hip.so.  These launches take 3 to 5 us on the device; the same checks in Python took 8 to 15 us a call (a dozen tensors at half a microsecond each,
 // two allocations at 1.6), here 1 to 2.  Host code only: the operators are the library's, reached through the C ABI of include/ecad_hip.h.
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/TracerMode.h>
@@ -73,10 +74,14 @@ Engine& held(PyObject* o) {
   if (!p) throw python_error();
   return *static_cast<Engine*>(p);
 }
+bool dual_level;  // as the call came in, some thread differentiates forward: only then is there a tangent to look for (read and written with the interpreter's lock)
+
 Engine& engine_of(PyObject* o) {
   refuse_tracing();
-  if (o == Py_None || held(o).closed) throw std::runtime_error("the engine is closed");
-  return held(o);
+  Engine* const e = o == Py_None ? nullptr : &held(o);
+  if (!e || e->closed) throw std::runtime_error("the engine is closed");
+  dual_level = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;
+  return *e;
 }
 const Tensor* maybe(PyObject* o, const char* name) {
   if (o == Py_None) return nullptr;
@@ -119,24 +124,19 @@ enum Dense { WHOLE, LAST };  // contiguous, or the last dimension only
 bool dense(const Tensor& t, Dense how) { return how == WHOLE ? t.is_contiguous() : t.dim() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1; }
 
 // a tangent of forward-mode differentiation (of the tensor, or of what it is a view of); none where that mode is switched off
-bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
+bool has_tangent(const Tensor& t) { return dual_level && t._fw_grad(0).defined(); }
 
+using Keys = c10::DispatchKeySet;
+using Key = c10::DispatchKey;
 // a tensor of another kind that stands for values it does not hold itself (fake, wrapped by a transform, a subclass with a dispatch of its own)
-bool stands_in(const Tensor& t) {
-  static const c10::DispatchKeySet kinds({c10::DispatchKey::Python, c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::Batched});
-  return t.key_set().has_any(kinds);
-}
-
+constexpr Keys STANDS_IN({Key::Python, Key::Functionalize, Key::FuncTorchGradWrapper, Key::FuncTorchBatched, Key::Batched});
 // values that are not what the memory says: the lazily negated ones of x.conj().imag, the zeros without memory of forward-mode differentiation
-bool lazy(const Tensor& t) {
-  static const c10::DispatchKeySet kinds({c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor});
-  return t.key_set().has_any(kinds);
-}
+constexpr Keys LAZY({Key::Negative, Key::ZeroTensor});
 
 // on the engine's device, of that type and shape, with memory of its own; gradients are not recorded by these operators, tangents not carried on
 void check(const Engine& e, const Tensor& t, const char* name, at::ScalarType type, at::IntArrayRef shape, Dense how) {
-  if (t.scalar_type() == type && t.device() == e.device && t.sizes() == shape && dense(t, how) && !(t.requires_grad() && c10::GradMode::is_enabled()) && !has_tangent(t) && !stands_in(t) && !lazy(t)) return;
-  if (stands_in(t)) throw std::runtime_error(std::string(name) + " is a tensor that holds no values itself (traced, transformed, or a subclass with a dispatch of its own)");
+  if (t.scalar_type() == type && t.device() == e.device && t.sizes() == shape && dense(t, how) && !(t.requires_grad() && c10::GradMode::is_enabled()) && !has_tangent(t) && !t.key_set().has_any(STANDS_IN | LAZY)) return;
+  if (t.key_set().has_any(STANDS_IN)) throw std::runtime_error(std::string(name) + " is a tensor that holds no values itself (traced, transformed, or a subclass with a dispatch of its own)");
   if (t.device() != e.device) refuse("%s is on %s, this engine on %s", name, t.device().str().c_str(), e.device.str().c_str());
   if (t.scalar_type() != type) {
     auto of = [](at::ScalarType s) { return s == at::kHalf ? "torch.float16" : s == at::kBFloat16 ? "torch.bfloat16" : s == at::kFloat ? "torch.float32" : s == at::kChar ? "torch.int8" : s == at::kInt ? "torch.int32" : at::toString(s); };
@@ -144,7 +144,7 @@ void check(const Engine& e, const Tensor& t, const char* name, at::ScalarType ty
   }
   if (t.sizes() != shape) refuse("%s must have shape %s, got %s", name, text(shape).c_str(), text(t.sizes()).c_str());
   if (!dense(t, how)) refuse("%s must %s, got strides %s", name, how == WHOLE ? "be contiguous" : "have a dense last dimension", text(t.strides()).c_str());
-  if (lazy(t)) refuse("%s is lazily negated or a zero without memory: its memory does not hold its values (resolve_neg(), or clone it)", name);
+  if (t.key_set().has_any(LAZY)) refuse("%s is lazily negated or a zero without memory: its memory does not hold its values (resolve_neg(), or clone it)", name);
   if (has_tangent(t)) refuse("%s has a forward-mode tangent: this op carries none on (take unpack_dual(...).primal, or switch forward gradients off)", name);
   refuse("%s requires a gradient: this op has none (detach it, or call under torch.no_grad())", name);
 }
