@@ -1,6 +1,7 @@
 // binding.cpp -- the Python side of the small operators (ecad_amd/_ops.so): argument checks of EcadEngine.op_quantize_int8 / op_gemm_int8 / op_gate_norm / op_rope_table / op_rope and the
 // call into libecad_hip.so.  These launches take 3 to 5 us on the device; the same checks in Python took 8 to 15 us a call (a dozen tensors at half a microsecond each,
-// two allocations at 1.6), here 1 to 2.  Host code only: the operators are the library's, reached through the C ABI of include/ecad_hip.h.
+// two allocations at 1.6), here 1 to 2.  Everything that a call may not be given is refused here or in the library: what torch keeps beside a tensor's memory (gradients,
+// tangents, traces, lazy signs) does not get past check().  Host code only: the operators are the library's, reached through the C ABI of include/ecad_hip.h.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>

@@ -72,10 +72,11 @@ template <typename T, bool RAGGED> ECAD_DEV void row_store(T* p, const Pack8& v,
 // loads in flight while one is worked on.  The channel vectors g, 1 + s, t of a sample stay in registers from row to row: read anew for every row they are up to
 // 26 bytes per element out of L2 against the 8 that the rows themselves move.  They are zero beyond the row, and with them everything that is computed there.
 // HOLD false (rows of more than 8192 values on 16 waves, whose lanes have 128 registers): read anew all the same, and from 16384 values on nothing is in flight ahead.
-// Bound by memory: 8 bytes per value (7 with 8-bit rows out), at the 5.15 TB/s of a large copy 14.7 us for 8192 x 1152 (18.1 measured, a launch being 1.9 of them),
-// 104 us for 16384 x 4096 (109), 58.6 us for 32768 x 1152 (57.6: 5.2 TB/s), 52 us for 4096 x 8192 (45: part of it from the last-level cache).  Rows beyond 8192 values:
-// 2048 x 16384 82 us (3.3 TB/s), 2048 x 32768 156 us (3.4): one row per CU at a time, and the channel vectors out of L2 for each.  Few rows: 5 x 1153 4.8 us:
-// a launch, the loads of the row and its vectors, four meetings of the row's waves.
+// Bound by memory: 8 bytes per value (7 with 8-bit rows out), at the 5.15 TB/s of a large copy 14.7 us for 8192 x 1152 (19.0 measured, a launch being 1.9 of them),
+// 104 us for 16384 x 4096 (109), 58.6 us for 32768 x 1152 (56.3: 5.4 TB/s, part of it from the last-level cache), 52 us for 4096 x 8192 (52.4).  Rows beyond 8192 values:
+// 2048 x 16384 79 us (3.4 TB/s), 2048 x 32768 156 us (3.4): one row per CU at a time, and the channel vectors out of L2 for each.  To 8-bit rows 4096 x 1152 15.8 us of 6.4
+// (two rows a wave: ramp and two rows' latency).  Few rows: 5 x 1153 5.5 us: a launch, the loads of the row and its vectors, four meetings of the row's waves.
+// (Times here and in the other headers: medians of a kernel trace, the same data again and again; profiles/operators_kernel_stats.csv.)
 template <typename T, int WAVES, int CH, bool RAGGED, bool HOLD>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void gate_norm_kernel(const GateNormArgs p) {
   constexpr int SLOTS = row_slots(WAVES);
@@ -245,8 +246,8 @@ struct QuantizeArgs {
   int M, K;
 };
 
-// One row per WAVES waves, the whole row in registers between the maximum and the rounding: read once.  Bound by memory, 3 bytes per value: 8192 x 4608 19.5 to 22 us
-// (5.1 to 5.8 TB/s; a copy moves 5.15), 8192 x 1152 7.8 us (3.6 TB/s with its launch), 601 x 4001 4.2 us.
+// One row per WAVES waves, the whole row in registers between the maximum and the rounding: read once.  Bound by memory, 3 bytes per value: 8192 x 4608 19.2 us
+// (5.9 TB/s, part of it from the last-level cache; a copy moves 5.15), 8192 x 1152 7.2 us (3.9 TB/s with its launch), 601 x 4001 4.8 us.
 template <typename T, int WAVES, int CH, bool RAGGED>
 __global__ __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) void quantize_rows_kernel(const QuantizeArgs p) {
   __shared__ unsigned scratch[2][WAVES];

@@ -207,8 +207,9 @@ constexpr int int8_lds_bytes(int bm, int bn, int stages) {
 // BM x BN tile on WM x WN waves, KW such groups along K.  A step is 128 bytes of K per row for every group: pieces of eight rows (1 KiB) travel straight to LDS, 16-byte
 // chunks XOR-swizzled by (row >> 1) & 7 on the source side, so that the fragment reads (16 rows x 16 bytes) meet every bank once.  One barrier per step, STAGES steps in
 // a ring.  KW > 1 is for products of few tiles, whose time is the number of steps: the groups' sums meet in LDS (whole numbers: the same bits).
-// Bound by the latency of a step where tiles are few (601 x 1111 x 4001: 16 steps of two, 12.7 us; 1024 x 1152 x 1152: 7.2 us), by the LDS pieces' issue where they are
-// many (8192 x 4608 x 1152: 64 us on 128 x 128 tiles, 1350 TOP/s; the wide kernels below take those).
+// Bound by the latency of a step where tiles are few (601 x 1111 x 4001: 180 tiles, 16 steps of two, 12.0 us, 13.1 with SiLU; 1024 x 1152 x 1152: 8.0 us), by the LDS pieces'
+// issue where they are many (8192 x 4608 x 1152: 67 us on 128 x 128 tiles, 1290 TOP/s; the wide kernels below take those).  One workgroup walks all of K for its tile: 512 x 1152
+// x 4608 is 144 of them on 256 CUs (11.9 us of 2.3), 64 x 4096 x 8192 64 (18.5 of 6.5).
 template <typename T, int BM, int BN, int WM, int WN, int KW, int STAGES, int EPI>
 __global__ __launch_bounds__(WM * WN * KW * 64, 2) void gemm_int8_kernel(const Int8GemmArgs p) {
   constexpr int NG = WM * WN, NW = NG * KW, FM = BM / WM / 16, FN = BN / WN / 16;
@@ -314,10 +315,11 @@ __global__ __launch_bounds__(WM * WN * KW * 64, 2) void gemm_int8_kernel(const I
 // The same product on one wave per SIMD, 256 x BN tiles on four waves: the K loop over whole stages is one hand-placed asm statement (gemm_int8_asm.h, generated by
 // scripts/gen_gemm_i8.py) that leaves the accumulators in AGPRs.  hipcc knows those only as clobbers of the statement: everything that touches them afterwards is asm
 // too, and the build fails if the compiler uses one before the last is read (scripts/audit_agpr.py).
-// 8192 x 8192 x 4096: 232 us, 2360 TOP/s (a library's 8192^3: 2330).  8192 x 1152 x 4608: 39.4 us (2210 TOP/s), 50 with the gated residual; 8192 x 4608 x 1152: 52 to
-// 57 us (1520 to 1660, as the clock allows), 57 to 62 with GELU; 4096 x 3456 x 1152: 23.5 us (1390).  Bound by the stream of operands into LDS: a piece holds its wave 60 to 180 cycles, and a stage of the 256 x 144
-// tile takes 1 us with 0.5 us of matrix instructions in it (their pipe is busy 36 % of a CU's cycles at K 1152, 40 % at 4608); then by the epilogue, which has the chip to
-// itself in a launch of one round.
+// As the clock allows: 8192 x 8192 x 4096 209 to 241 us (2280 to 2630 TOP/s; a library's 8192^3: 2330); 8192 x 1152 x 4608 41 to 47 us (1850 to 2110), 56 with the gated
+// residual; 8192 x 4608 x 1152 56 to 63 us (1370 to 1560), 61 with GELU; 4096 x 3456 x 1152 23.4 to 25.9 us (1260 to 1390).  Bound by the stream of operands into LDS: a piece
+// holds its wave 60 to 180 cycles, and a stage of the 256 x 144 tile takes 1 us with 0.5 us of matrix instructions in it (their pipe is busy 36 % of a CU's cycles at K 1152, 40 %
+// at 4608); then by what every round of tiles has to itself, one workgroup being on a CU: the ring's fill and the epilogue.  8192 x 4608 x 1152 is 512 tiles of 256 x 288, two
+// rounds of nine stages; by the constants of choose_int8 8 us of a round's 25 are outside its K loop.  8192 x 1152 x 4608 is 256 tiles of 256 x 144, one round.
 template <int BN> struct Int8Wide {
   static constexpr bool tall = BN == 144;                      // waves stacked 4 x 1 (64 x 144 each), else 2 x 2 (128 x BN / 2)
   static constexpr int FM = tall ? 4 : 8, FN = tall ? 9 : BN / 32, stages = tall ? 3 : 2;
@@ -409,7 +411,8 @@ __global__ __launch_bounds__(256) void gemm_int8_wide_kernel(const Int8GemmArgs 
 
 // Few rows (M <= 16 FM): the time is the reading of W.  A workgroup owns 16 columns; its waves take turns along K in steps of 64 bytes per row, operands go
 // straight to registers in the matrix instruction's layout (each W byte is used by one wave only: nothing to share through LDS), several steps in flight; the waves'
-// sums meet in LDS.  8 x 6912 x 1152 (8 MB) 3.9 us, 8 x 4096 x 8192 (33.5 MB) 9.0 us: 3.7 TB/s with the launch and the first loads' latency in it.
+// sums meet in LDS.  8 x 6912 x 1152 (8 MB) 4.5 us, 8 x 4096 x 8192 (33.5 MB) 9.4 us: 3.6 TB/s with the launch and the first loads' latency in it.  Narrow weights are
+// bound by the CUs that have no columns: 1152 are 72 workgroups on 256 CUs, 5.3 MB in 5.7 to 6.5 us at 8 rows and 8.1 to 8.9 at 32.
 template <typename T, int FM, int NW, int EPI>
 __global__ __launch_bounds__(NW * 64) void gemm_int8_rows_kernel(const Int8GemmArgs p) {
   __shared__ int part[NW][FM * 256];

@@ -160,7 +160,9 @@ template <typename T> int gate_norm_t(const OpCtx& ctx, GateNormArgs& a, OpStatu
   const int pieces = (a.D + 7) / 8;
   if (pieces <= 64) return launch_norm<T, 1, 1>(ctx, a, 20, st);
   if (pieces <= 128) return launch_norm<T, 2, 1>(ctx, a, 10, st);
-  if (pieces <= 192) return a.M <= 8 * ctx.num_cus ? launch_norm<T, 3, 1>(ctx, a, 6, st) : launch_norm<T, 1, 3>(ctx, a, 8, st);  // 5 rows 3.9 / 5.6 us, 2048 rows 8.8 / 9.4, 4096 rows 13.9 / 12.5, 32768 rows 75 / 57.5
+  // three waves a row / one: 1152 values 5 rows 4.0 / 5.9 us, 2048 rows 8.1 / 9.3, 4096 rows 13.2 / 12.1, 32768 rows 75 / 55; 1032 values 4.0 / 6.0, 8.3 / 9.5, 13.0 / 12.1,
+  // 64 / 62; 1536 values 4.1 / 6.0, 8.5 / 9.7, 13.5 / 12.7, 100 / 86
+  if (pieces <= 192) return a.M <= 8 * ctx.num_cus ? launch_norm<T, 3, 1>(ctx, a, 6, st) : launch_norm<T, 1, 3>(ctx, a, 8, st);
   if (pieces <= 256) return launch_norm<T, 4, 1>(ctx, a, 5, st);
   if (pieces <= 512) return launch_norm<T, 8, 1>(ctx, a, 2, st);
   if (pieces <= 1024) return launch_norm<T, 8, 2>(ctx, a, 1, st);
@@ -191,16 +193,19 @@ template <typename T, int EPI, int BN> int launch_wide(const OpCtx& ctx, const I
 }
 
 // Which kernel: the one with the smallest estimated time, rounds of the tiles it needs over the chip times (what a round costs outside the K loop + its K stages), in
-// microseconds; a stage costs more the fuller the chip is (operands from L2, and the clock under load).  Fitted to the times below and thirteen other shapes: the pick is
-// the fastest kernel at 19 of 20 (8000 x 500 x 3000: 18 % off).  Measured, us, plain epilogue:
+// microseconds; a stage costs more the fuller the chip is (operands from L2, and the clock under load).  The pick is the fastest kernel at 18 of the 19 shapes of more than
+// 32 rows in profiles/operators_kernel_choice.csv (8000 x 500 x 3000: 21 % off).  Some of them, us, plain epilogue:
 //                        64 x 64   64 x 64, K over two   128 x 128   256 x 144   256 x 256   256 x 288
-//   601 x 1111 x 4001     16.5        13.1                32.9        39.9        60.9        64.0
-//   1024 x 1152 x 1152     7.3        10.7                10.8        13.1        18.9        19.4
-//   2048 x 4608 x 1152    30.4        44.6                24.8        17.6        21.1        23.8
-//   4096 x 3456 x 1152    44.8        67.1                28.1        30.2        23.0        24.7
-//   8192 x 4608 x 1152   111.4       171.5                64.3        62.1        61.1        52.3
-//   8192 x 1152 x 4608    83.5        95.8                69.7        39.4        48.4        52.8
-//   8192 x 8192 x 4096   502         614                 314         287         232         257
+//   512 x 4608 x 1152     12.7        15.6                12.3        14.1        17.9        20.5
+//   512 x 1152 x 4608     16.8        11.9                31.2        29.4        42.6        45.9
+//   601 x 1111 x 4001     16.1        12.0                29.9        32.0        45.3        50.9
+//   1024 x 1152 x 1152     8.0        11.7                11.8        13.4        19.3        19.6
+//   2048 x 4608 x 1152    32.9        46.7                26.1        18.1        21.3        24.3
+//   4096 x 3456 x 1152    48.0        69.8                30.3        31.0        23.4        25.7
+//   8000 x 500 x 3000     30.0        35.8                27.0        32.7        48.6        50.8
+//   8192 x 4608 x 1152   113.9       171.9                67.4        66.7        66.4        63.4
+//   8192 x 1152 x 4608    92.9       102.4                72.9        41.2        51.1        54.9
+//   8192 x 8192 x 4096   542         615                 299         269         209         227
 int choose_int8(const OpCtx& ctx, const Int8GemmArgs& a) {
   struct Tile {
     int id, bm, bn, per_cu, fewest;
@@ -212,7 +217,9 @@ int choose_int8(const OpCtx& ctx, const Int8GemmArgs& a) {
                                {ECAD_I8_K_TILE144, 256, 144, 1, Int8Wide<144>::fewest, 7.0, 0.62, 0.25, 0},
                                {ECAD_I8_K_TILE256, 256, 256, 1, Int8Wide<256>::fewest, 7.0, 0.5, 1.1, 1.1},
                                {ECAD_I8_K_TILE288, 256, 288, 1, Int8Wide<288>::fewest, 8.0, 0.5, 1.35, 1.2}};
-  if (a.M <= 32 && fits(((int64_t)a.N + 15) / 16, 1024)) return ECAD_I8_K_ROWS;  // 32 rows: 6912 x 1152 5.3 us (64 x 64 tiles 5.8), 1152 x 4608 7.9 (11.5), 4096 x 8192 14.0 (18.5); 64 rows: 7.6 (5.8), 12.2 (11.4), 21.0 (18.5)
+  // few-rows kernel / best tile: 32 rows 6912 x 1152 5.8 us / 6.2, 1152 x 4608 8.1 / 11.2, 4096 x 8192 13.3 / 18.2; 64 rows (a form of it that is not kept) 7.6 / 6.2, 12.2 / 11.6,
+  // 21.0 / 18.5
+  if (a.M <= 32 && fits(((int64_t)a.N + 15) / 16, 1024)) return ECAD_I8_K_ROWS;
   const int stages = (a.K + 127) / 128;
   int best = ECAD_I8_K_TILE64;
   double least = 1e300;
@@ -233,7 +240,9 @@ template <typename T, int EPI> int gemm_int8_t(const OpCtx& ctx, const Int8GemmA
     case ECAD_I8_K_ROWS: {
       const dim3 grid((unsigned)(((int64_t)a.N + 15) / 16));
       if (!fits(grid.x, 1024)) return refuse(st, ECAD_E_UNSUPPORTED, "gemm_int8: %d columns are more than one launch of the few-rows kernel takes", a.N);
-      const bool narrow = (int64_t)grid.x < 2 * (int64_t)ctx.num_cus;  // few workgroups: more of K in flight at a time
+      // few workgroups: more of K in flight at a time.  Sixteen waves / eight, 8 rows: 1152 x 4608 5.6 us / 5.7, 4096 x 8192 8.1 / 8.9, 6912 x 1152 4.3 / 4.3; 8208 x 1152 5.0 / 4.6,
+      // 16384 x 1152 7.1 / 6.2
+      const bool narrow = (int64_t)grid.x < 2 * (int64_t)ctx.num_cus;
       if (a.M <= 16 && narrow) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 1, 16, EPI>), grid, dim3(1024), 0, ctx.stream, a);
       else if (a.M <= 16) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 1, 8, EPI>), grid, dim3(512), 0, ctx.stream, a);
       else if (narrow) hipLaunchKernelGGL((gemm_int8_rows_kernel<T, 2, 16, EPI>), grid, dim3(1024), 0, ctx.stream, a);

@@ -23,9 +23,10 @@ struct RopeTableArgs {
 // The angle is counted in quarter turns and reduced in 64 bits: the remainder of p (2 f / pi) from the nearest whole one, |r| <= 1/2, is one fma; only r pi / 2 becomes
 // fp32, so a position of 10^7 is as exact as position 1.  (The frequency itself has 53 bits: the angle
 // is off by 2^-53 of it, which is all of a turn from 2^53 turns on.  Positions beyond come out on the circle, somewhere.)  On |a| <= pi / 4 the Taylor sums below end 2e-9 (sine, a^9) and 2e-10 (cosine, a^10) from the function;
-// their fp32 arithmetic, with the rounding of a, stays within 4.5 2^-24 (64-bit sums would end at 2^-24 of the value, for a table whose rows meet 16-bit heads).
+// their fp32 arithmetic, with the rounding of a, stays within 4.5 2^-24 (1.3 2^-24 at the worst of 6.4 million pairs, 1.7 with YaRN's factor; rounded once: 0.5).  That is
+// a choice: what the roundings lose, carried along in the small terms, gave 0.71 2^-24 and took 131072 x 64 pairs from 15.4 to 16.9 us, for rows that turn 16-bit heads.
 // A thread keeps its pair (frequency and axis are read once) and steps through rows; half a dozen 64-bit operations per pair keep the kernel near its stores (8
-// bytes per pair): 131072 x 64 pairs in 15.8 us (4.3 TB/s; with a division per pair to find the row 22.9), 16384 x 64 in 5.0.
+// bytes per pair): 131072 x 64 pairs in 15.5 us (4.4 TB/s; with a division per pair to find the row 22.9), 16384 x 64 in 5.3.
 __global__ __launch_bounds__(1024) void rope_table_kernel(const RopeTableArgs p) {
   const int r0 = threadIdx.x / (unsigned)p.pairs, j = threadIdx.x - r0 * p.pairs;
   if (r0 >= p.rows_per_block) return;
@@ -69,8 +70,8 @@ constexpr int ROPE_HEADS = 4;  // heads a thread turns with the cosines it has r
 
 // A thread owns one piece of ROPE_HEADS heads of a token: HALF: eight pairs (two pieces half a rotation apart); else four pairs side by side.  Pieces behind the
 // rotation are copied.  Rows of the table are picked per token; an index outside the table leaves its token as it is.
-// Bound by memory, 4 bytes per value and the table once: 2 x 4608 x (16 + 16) x 128 in 26.5 to 27.6 us (5.5 TB/s); 8 tokens of 40 heads x 72 in 4.6 us (launch, index,
-// table row and head one after the other).
+// Bound by memory, 4 bytes per value and the table once: 2 x 4608 x (16 + 16) x 128 in 25.5 us side by side and 25.0 in halves (5.9, 6.0 TB/s: part of it from the last-level
+// cache), (32 + 8) heads in 35.1 and 30.3 (5.4, 6.2); 8 tokens of 40 heads x 72 in 4.7 us (launch, index, table row and head one after the other).
 template <typename T, bool HALF>
 __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs p) {
   const int64_t token0 = (int64_t)blockIdx.x * p.tokens_per_block;

@@ -405,8 +405,9 @@ class EcadEngine:
 
 
     # -- the launches of an 8-bit transformer block ---------------------------------------------
-    # Inference only, like every op here: tensors that require a gradient are refused while gradients are recorded.  Work goes to the current stream of the engine's
-    # device; nothing is allocated but the results.  What does not fit together is a ValueError, outputs that overlap themselves or another argument among it.  The
+    # Inference only, like every op here: tensors that require a gradient are refused while gradients are recorded, those with a forward-mode tangent, lazily negated ones and
+    # calls under a tracer always.  What is written in place has a new version.  Work goes to the current stream of the engine's device, without the interpreter's lock;
+    # several threads may call; nothing is allocated but the results.  What does not fit together is a ValueError, outputs that overlap themselves or another argument among it.  The
     # checks and the call are native (csrc/binding.cpp): these launches are a few microseconds, and so has to be what stands in front of them.
     def _native(self):
         """(functions, this engine) of ecad_amd/_ops.so; a closed engine is None there."""
@@ -466,7 +467,8 @@ class EcadEngine:
         """Cosines and sines of rotary positions (``ecad_op_rope_table``): positions [S] or [S, axes] int32 or fp32 -> [S, sum(axes_dims) / 2, 2] fp32: angles reduced in 64 bits, their
         functions within 4.5 * 2^-24.
         axes_dims: elements that turn with each axis (even; an int for one axis), e.g. (16, 56, 56) for FLUX's (index, row, column).  scaling "linear" (f / factor), "ntk" (theta
-        factor^(d / (d - 2))) or "yarn" (pairs that turn often within ``original_length`` stay, the others are stretched; cosine and sine times 0.1 ln(factor) + 1)."""
+        factor^(d / (d - 2))) or "yarn" (pairs that turn often within ``original_length`` stay, the others are stretched; cosine and sine times 0.1 ln(factor) + 1).
+        ``op_rope`` takes any table of that layout, so other ramps and frequencies are a table of your own."""
         ops, engine = self._ops or self._native()
         number = self.ROPE_SCALINGS.get(scaling)
         if number is None:

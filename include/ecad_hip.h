@@ -285,7 +285,8 @@ int ecad_op_qproj_attention(EcadEngine* e, int call_site, const void* x, const v
  * a sub-layer, and for rotary positions of any head layout.  All of them only launch on `stream` (no allocation, no synchronisation, nothing kept between calls): they
  * may be captured into a graph, and called from several streams.  They run on the engine's device whatever the current device is, and leave that as it was.
  * 16-bit tensors have the engine's dtype; rows may have any width and any stride (in elements) at the alignment of an element; 8-bit rows start on 16 bytes with a
- * stride of a multiple of 16 (so the last 16-byte piece of a row may be read whole; what lies behind the row's values does not matter).
+ * stride of a multiple of 16, in a product of at most 2^23 (so the last 16-byte piece of a row may be read whole; what lies behind the row's values does not matter).
+ * Several threads may call them on one engine at once: each finds its own refusal's message.  An engine may be destroyed when no call on it runs.
  * Zero rows: nothing is done.  Outputs that overlap themselves, each other or an input are refused (columns of one buffer side by side do not overlap), but for the
  * in-place forms that each entry names. */
 
@@ -293,7 +294,8 @@ int ecad_op_qproj_attention(EcadEngine* e, int call_site, const void* x, const v
  * A row with an infinity or a NaN: scale NaN, zeros -- its products are NaN.  1 <= K < 131072.  Weights [N, K] are quantised by the same call, once. */
 int ecad_op_quantize_int8(EcadEngine* e, const void* x, int64_t ldx, int8_t* q, int64_t ldq, float* scale, int M, int K, void* stream);
 
-/* o[M,N] = act(a_scale[m] w_scale[n] (A[M,K] @ W[N,K]^T) + bias[n]), the sum in 32-bit integers; epi as ecad_op_gemm: 0 none, 1 GELU(tanh), 2 SiLU, 3 cache write and
+/* o[M,N] = act(a_scale[m] w_scale[n] (A[M,K] @ W[N,K]^T) + bias[n]), the sum in 32-bit integers, then times a_scale, then times
+ * w_scale in fp32 (sum * a_scale has to be in its range); epi as ecad_op_gemm: 0 none, 1 GELU(tanh), 2 SiLU, 3 cache write and
  * gated residual: out = o rounded (may be NULL), resid_out = resid + (gate_table[n] + gate_mod[m / rows_per_batch][n]) * out (either or both NULL: gate 1 where
  * neither is given; resid_out may be resid).  kernel: ECAD_I8_K_AUTO, or one by name (the same bits; ECAD_E_UNSUPPORTED if it cannot take the shape). */
 enum { ECAD_I8_K_AUTO = 0, ECAD_I8_K_ROWS = 1 /* up to 32 rows: operands straight to registers, K over the waves */, ECAD_I8_K_TILE64 = 2, ECAD_I8_K_TILE128 = 3, ECAD_I8_K_TILE144 = 4 /* 256 x 144 */,
@@ -316,7 +318,8 @@ int ecad_op_gemm_int8(EcadEngine* e, const EcadInt8Gemm* args, void* stream);
 
 /* h' = resid_scale * h + g * post(y);  n = pre(h') * (1 + s) + t.   post / pre: ECAD_NORM_*, x / sqrt(mean x^2 + eps) or (x - mean) / sqrt(var + eps), times weight[D]
  * where not NULL.  g = gate_table[D] + gate_mod[row / rows_per_batch][D] (1 where both are NULL), s and t in the same way from table_scale / mod_scale and
- * table_shift / mod_shift (0 where both are NULL); tables fp32, modulations engine dtype with a stride between samples.
+ * table_shift / mod_shift (0 where both are NULL); tables fp32, modulations engine dtype with a stride between samples, 0 where all samples share one (mod_stride is that of
+ * mod_shift and of mod_scale: a shared one beside one per sample goes into its table).
  * y NULL: h' = h and h_out is not written (no gate, post-norm or residual scale then).  pre ECAD_NORM_NONE: only h_out.  n goes to n_out, or, rounded to the engine
  * dtype first, to 8-bit rows q / q_scale (ecad_op_quantize_int8 of n, bit for bit): exactly one of the two.  h_out may be h, n_out may be y.  1 <= D <= 32768. */
 enum { ECAD_NORM_NONE = 0, ECAD_NORM_RMS = 1, ECAD_NORM_LAYER = 2 };
@@ -345,7 +348,8 @@ int ecad_op_gate_norm(EcadEngine* e, const EcadGateNorm* args, void* stream);
  * other, axes_dims[a] / 2 (host array) on axis a, f = theta^(-2 j / axes_dims[a]).  Scalings for positions beyond the trained ones, by `factor`:
  *   LINEAR  f / factor
  *   NTK     theta * factor^(d / (d - 2)) in place of theta (axes of two elements: theta)
- *   YARN    f w + (f / factor)(1 - w), w = clamp((original_length f / 2 pi - beta_slow) / (beta_fast - beta_slow), 0, 1), and m = 0.1 ln(factor) + 1 (else m = 1) */
+ *   YARN    f w + (f / factor)(1 - w), w = clamp((original_length f / 2 pi - beta_slow) / (beta_fast - beta_slow), 0, 1), and m = 0.1 ln(factor) + 1 (else m = 1)
+ * A ramp over the pair index, other frequencies or another m: ecad_op_rope takes any table of this layout, whoever made it. */
 enum { ECAD_ROPE_NONE = 0, ECAD_ROPE_LINEAR = 1, ECAD_ROPE_NTK = 2, ECAD_ROPE_YARN = 3 };
 int ecad_op_rope_table(EcadEngine* e, const void* positions, int positions_float, const int32_t* axes_dims, int axes, int S, int scaling, double theta, double factor, double original_length,
                        double beta_fast, double beta_slow, float* table, void* stream);
