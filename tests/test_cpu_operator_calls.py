@@ -164,59 +164,75 @@ def test_every_thread_finds_its_own_message():
 
 
 @pytest.fixture
-def slow(tmp_path):
-    """An engine whose launches take 0.3 s, as one does while the device's queue is full; `left` counts those that have returned, and `destroyed` what it was when the engine went."""
-    (tmp_path / "slow.c").write_text("""#include <unistd.h>
-int left, destroyed = -1;
-int launch(void) { usleep(300000); ++left; return 0; }
+def waiting(tmp_path):
+    """An engine whose launches wait (20 s at most) until `go` is set, as one does while the device's queue is full; `entered` and `left` count them, `destroyed` is what `left`
+    was when the engine went."""
+    (tmp_path / "waiting.c").write_text("""#include <stdatomic.h>
+#include <unistd.h>
+atomic_int entered, left, go, destroyed = -1;
+int launch(void) {
+  ++entered;
+  for (int i = 0; i < 20000 && !go; ++i) usleep(1000);
+  ++left;
+  return 0;
+}
 const char* last_error(void* e) { return ""; }
 void destroy(void* e) { destroyed = left; }
 """)
-    subprocess.run(["gcc", "-shared", "-fPIC", str(tmp_path / "slow.c"), "-o", str(tmp_path / "slow.so")], check=True)
-    lib, ops = C.CDLL(str(tmp_path / "slow.so")), L.load_ops()
+    subprocess.run(["gcc", "-shared", "-fPIC", str(tmp_path / "waiting.c"), "-o", str(tmp_path / "waiting.so")], check=True)
+    lib, ops = C.CDLL(str(tmp_path / "waiting.so")), L.load_ops()
     at = lambda name: C.cast(getattr(lib, name), C.c_void_p).value  # noqa: E731
     e = object.__new__(EcadEngine)
     e._h, e.cfg, e._donor = C.c_void_p(1 << 20), L.EcadModelCfg(), None
     e.lib = type("Library", (), {"ecad_destroy": staticmethod(lib.destroy)})
     e._ops = ops, ops.engine((at("launch"),) * 5 + (at("last_error"),), 1 << 20, L.ECAD_DTYPE_F16, -1, lambda index: 0)
-    e.count = lambda name: C.c_int.in_dll(lib, name).value
-    return e
+    e.count = lambda name: C.c_int.in_dll(lib, name)
+    yield e
+    e.count("go").value = 1
 
 
-def test_a_launch_that_waits_stops_no_other_thread(slow):
+def until(condition):
+    while not condition():
+        time.sleep(0.001)
+
+
+def test_a_launch_that_waits_stops_no_other_thread(waiting):
     x = f16(4, 24)
-    caller = threading.Thread(target=lambda: slow.op_quantize_int8(x))
-    longest, t = 0.0, time.perf_counter()
+    caller = threading.Thread(target=lambda: waiting.op_quantize_int8(x))
     caller.start()
-    while caller.is_alive():
-        longest, t = max(longest, time.perf_counter() - t), time.perf_counter()
-        time.sleep(0.005)
-    assert slow.count("left") == 1 and longest < 0.25
+    until(lambda: waiting.count("entered").value)
+    assert waiting.count("left").value == 0  # this thread runs beside the launch
+    waiting.count("go").value = 1
+    caller.join()
+    assert waiting.count("left").value == 1
 
 
-def test_closing_waits_for_the_calls_of_other_threads(slow):
+def test_closing_waits_for_the_calls_of_other_threads(waiting):
     x, seen = f16(4, 24), []
 
     def call():
-        for _ in range(3):
-            try:
-                slow.op_quantize_int8(x)
-            except RuntimeError as e:
-                seen.append(str(e))
-                return
+        waiting.op_quantize_int8(x)
+        try:
+            waiting.op_quantize_int8(x)
+        except RuntimeError as e:
+            seen.append(str(e))
 
     callers = [threading.Thread(target=call) for _ in range(2)]
     for t in callers:
         t.start()
-    time.sleep(0.1)
-    slow.close()
-    assert slow.count("destroyed") == 2
-    for t in callers:
+    until(lambda: waiting.count("entered").value == 2)
+    closer = threading.Thread(target=waiting.close)
+    closer.start()
+    until(lambda: not waiting._h.value)
+    time.sleep(0.1)  # (it is in close() by now)
+    assert closer.is_alive() and waiting.count("destroyed").value == -1
+    waiting.count("go").value = 1
+    for t in (closer, *callers):
         t.join()
-    assert seen == ["the engine is closed"] * 2 and slow.count("left") == 2
+    assert seen == ["the engine is closed"] * 2 and waiting.count("entered").value == 2 and waiting.count("destroyed").value == 2
     with pytest.raises(RuntimeError, match="closed"):
-        slow.op_quantize_int8(x)
-    slow.close()
+        waiting.op_quantize_int8(x)
+    waiting.close()
 
 
 def test_the_library_is_built_without_torch():
