@@ -421,7 +421,7 @@ class EcadEngine:
         return self._ops
 
     def op_quantize_int8(self, x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-        """Rows to 8-bit integers with one scale each (``ecad_op_quantize_int8``): x [M, K] of the engine's dtype at any row stride -> (q [M, K] int8 whose rows start on
+        """Rows to 8-bit integers with one scale each (``ecad_op_quantize_int8``): x [M, K] of the engine's dtype at any row stride from K on -> (q [M, K] int8 whose rows start on
         16 bytes, scale [M] fp32), x ~ q * scale[:, None].  scale = max|row| / 127, q the nearest integer (ties to even) in exact arithmetic.  A row of zeros has
         scale 0; one with an infinity or NaN has scale NaN.  Weights [N, K] (one scale per output channel) go through the same call once.
         ``out``: (q, scale) to write to; q's rows on 16 bytes."""
@@ -464,7 +464,7 @@ class EcadEngine:
     ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 
     def op_rope_table(self, positions, axes_dims, theta=10000.0, scaling="none", factor=1.0, original_length=0, beta_fast=32.0, beta_slow=1.0, out=None) -> torch.Tensor:
-        """Cosines and sines of rotary positions (``ecad_op_rope_table``): positions [S] or [S, axes] int32 or fp32 -> [S, sum(axes_dims) / 2, 2] fp32: angles reduced in 64 bits, their
+        """Cosines and sines of rotary positions (``ecad_op_rope_table``): positions [S] or [S, axes] int32 or fp32, contiguous -> [S, sum(axes_dims) / 2, 2] fp32: angles reduced in 64 bits, their
         functions within 4.5 * 2^-24.
         axes_dims: elements that turn with each axis (even; an int for one axis), e.g. (16, 56, 56) for FLUX's (index, row, column).  scaling "linear" (f / factor), "ntk" (theta
         factor^(d / (d - 2))) or "yarn" (pairs that turn often within ``original_length`` stay, the others are stretched; cosine and sine times 0.1 ln(factor) + 1).

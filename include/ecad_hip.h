@@ -284,8 +284,8 @@ int ecad_op_qproj_attention(EcadEngine* e, int call_site, const void* x, const v
  * Companions of the single-op entry points above for a Linear in 8-bit integers (a scale per token, a scale per output channel), for blocks with norms on both sides of
  * a sub-layer, and for rotary positions of any head layout.  All of them only launch on `stream` (no allocation, no synchronisation, nothing kept between calls): they
  * may be captured into a graph, and called from several streams.  They run on the engine's device whatever the current device is, and leave that as it was.
- * 16-bit tensors have the engine's dtype; rows may have any width and any stride (in elements) at the alignment of an element; 8-bit rows start on 16 bytes with a
- * stride of a multiple of 16, in a product of at most 2^23 (so the last 16-byte piece of a row may be read whole; what lies behind the row's values does not matter).
+ * 16-bit tensors have the engine's dtype; rows may have any width, and any stride (in elements) of at least the width, at the alignment of an element; 8-bit rows start on
+ * 16 bytes with a stride of a multiple of 16, in a product of at most 2^23 (so the last 16-byte piece of a row may be read whole; what lies behind its values does not matter).
  * Several threads may call them on one engine at once: each finds its own refusal's message.  An engine may be destroyed when no call on it runs.
  * Zero rows: nothing is done.  Outputs that overlap themselves, each other or an input are refused (columns of one buffer side by side do not overlap), but for the
  * in-place forms that each entry names. */
@@ -316,8 +316,8 @@ typedef struct EcadInt8Gemm {
 } EcadInt8Gemm;
 int ecad_op_gemm_int8(EcadEngine* e, const EcadInt8Gemm* args, void* stream);
 
-/* h' = resid_scale * h + g * post(y);  n = pre(h') * (1 + s) + t.   post / pre: ECAD_NORM_*, x / sqrt(mean x^2 + eps) or (x - mean) / sqrt(var + eps), times weight[D]
- * where not NULL.  g = gate_table[D] + gate_mod[row / rows_per_batch][D] (1 where both are NULL), s and t in the same way from table_scale / mod_scale and
+/* h' = resid_scale * h + g * post(y);  n = pre(h') * (1 + s) + t.   post / pre: ECAD_NORM_*, x / sqrt(mean x^2 + eps) or (x - mean) / sqrt(var + eps) in fp32 (a
+ * bf16 row beyond 1e19 has no mean square there), times weight[D] where not NULL.  g = gate_table[D] + gate_mod[row / rows_per_batch][D] (1 where both are NULL), s and t in the same way from table_scale / mod_scale and
  * table_shift / mod_shift (0 where both are NULL); tables fp32, modulations engine dtype with a stride between samples, 0 where all samples share one (mod_stride is that of
  * mod_shift and of mod_scale: a shared one beside one per sample goes into its table).
  * y NULL: h' = h and h_out is not written (no gate, post-norm or residual scale then).  pre ECAD_NORM_NONE: only h_out.  n goes to n_out, or, rounded to the engine
