@@ -19,10 +19,9 @@ import tempfile
 from pathlib import Path
 
 ROOT = Path(__file__).resolve().parents[1]
-# the Makefile's flags of the units (CXXFLAGS), for device assembly
-COMMON = "-O3 -std=c++17 --offload-arch=gfx950 -fPIC -fno-gpu-rdc -DECAD_PRODUCT_BUILD -S --cuda-device-only".split()
-FAST = "-ffast-math -fno-finite-math-only".split()
-UNITS = {"flux.hip": FAST, "engine.hip": FAST, "vae.hip": FAST, "operators.hip": "-ffp-contract=fast -Xclang -target-feature -Xclang -packed-fp32-ops".split()}
+FLAGS = "-O3 -std=c++17 --offload-arch=gfx950 -fPIC -fno-gpu-rdc -ffast-math -fno-finite-math-only -DECAD_PRODUCT_BUILD -S --cuda-device-only".split()  # BASEFLAGS of the Makefile
+OPERATOR_FLAGS = [f for f in FLAGS if "-math" not in f] + "-ffp-contract=fast -Xclang -target-feature -Xclang -packed-fp32-ops".split()
+UNITS = {"flux.hip": FLAGS, "engine.hip": FLAGS, "vae.hip": FLAGS, "operators.hip": OPERATOR_FLAGS}
 KERNELS = ("fgemm4", "fgemm48", "attn_w4a", "attn_w472", "gemm2w4", "gemm3s4", "conv4", "gemm_int8_wide")
 
 
@@ -77,7 +76,7 @@ def main() -> int:
     with tempfile.TemporaryDirectory() as td:
         for unit, flags in UNITS.items():
             out = Path(td) / (unit + ".s")
-            subprocess.run(["/opt/rocm/bin/hipcc", *COMMON, *flags, str(ROOT / "ecad_amd" / "csrc" / unit), "-o", str(out)], check=True, stderr=subprocess.DEVNULL)
+            subprocess.run(["/opt/rocm/bin/hipcc", *flags, str(ROOT / "ecad_amd" / "csrc" / unit), "-o", str(out)], check=True, stderr=subprocess.DEVNULL)
             bad += audit(out.read_text(), unit)
     return 1 if bad else 0
 
