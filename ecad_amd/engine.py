@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import os
+import threading
 from typing import Mapping
 
 import numpy as np
@@ -30,6 +31,8 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 
 class EcadEngine:
+    _handles = threading.RLock()  # held where an engine's handles come and go (re-entrant: the collector may close one engine while another one's are made)
+
     def __init__(
         self,
         num_layers=28,
@@ -93,11 +96,13 @@ class EcadEngine:
 
     def close(self):
         if getattr(self, "_h", None) and self._h.value:
-            h, self._h = self._h, C.c_void_p()
-            if self._ops:
-                self._ops[0].close(self._ops[1])  # (calls of other threads have left the library)
-                self._ops = self._ops[0], None
-            self.lib.ecad_destroy(h)
+            with self._handles:
+                h, self._h = self._h, C.c_void_p()
+                ops, self._ops = self._ops, self._ops and (self._ops[0], None)
+            if h.value:
+                if ops:
+                    ops[0].close(ops[1])  # (calls of other threads have left the library)
+                self.lib.ecad_destroy(h)
         self._donor = None
 
     def set_ln_fold(self, on: bool) -> None:
@@ -411,14 +416,15 @@ class EcadEngine:
     # checks and the call are native (csrc/binding.cpp): these launches are a few microseconds, and so has to be what stands in front of them.
     def _native(self):
         """(functions, this engine) of ecad_amd/_ops.so; a closed engine is None there."""
-        if not self._h.value:
-            raise RuntimeError("the engine is closed")
-        if self._ops is None:
-            names = ("ecad_op_quantize_int8", "ecad_op_gemm_int8", "ecad_op_gate_norm", "ecad_op_rope_table", "ecad_op_rope", "ecad_last_error")
-            addresses = tuple(C.cast(getattr(self.lib, n), C.c_void_p).value for n in names)
-            ops = L.load_ops()
-            self._ops = ops, ops.engine(addresses, self._h.value, _TORCH2ECAD[self.dtype], self.device_index, torch._C._cuda_getCurrentRawStream)
-        return self._ops
+        with self._handles:  # one for all threads: close() knows of the calls on this one
+            if not self._h.value:
+                raise RuntimeError("the engine is closed")
+            if self._ops is None:
+                names = ("ecad_op_quantize_int8", "ecad_op_gemm_int8", "ecad_op_gate_norm", "ecad_op_rope_table", "ecad_op_rope", "ecad_last_error")
+                addresses = tuple(C.cast(getattr(self.lib, n), C.c_void_p).value for n in names)
+                ops = L.load_ops()
+                self._ops = ops, ops.engine(addresses, self._h.value, _TORCH2ECAD[self.dtype], self.device_index, torch._C._cuda_getCurrentRawStream)
+            return self._ops
 
     def op_quantize_int8(self, x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """Rows to 8-bit integers with one scale each (``ecad_op_quantize_int8``): x [M, K] of the engine's dtype at any row stride from K on -> (q [M, K] int8 whose rows start on

@@ -235,6 +235,34 @@ def test_closing_waits_for_the_calls_of_other_threads(waiting):
     waiting.close()
 
 
+def test_first_calls_of_several_threads_share_one_handle(waiting, monkeypatch):
+    """close() waits for the calls on the handle it knows: the first calls of two threads must not make one each."""
+    made = []
+
+    class Ops:
+        @staticmethod
+        def engine(*args):
+            time.sleep(0.05)
+            made.append(args)
+            return object()
+
+        @staticmethod
+        def close(engine):
+            pass
+
+    monkeypatch.setattr(L, "load_ops", lambda: Ops)
+    waiting.lib = type("Library", (), {"ecad_destroy": waiting.lib.ecad_destroy, **{n: C.CFUNCTYPE(C.c_int)(lambda: 0) for n in (
+        "ecad_op_quantize_int8", "ecad_op_gemm_int8", "ecad_op_gate_norm", "ecad_op_rope_table", "ecad_op_rope", "ecad_last_error")}})
+    waiting._ops, waiting.dtype, waiting.device_index, handles = None, torch.float16, 0, []
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    threads = [threading.Thread(target=lambda: handles.append(waiting._native())) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(made) == 1 and all(h is handles[0] for h in handles) and len(handles) == 4
+
+
 def test_the_library_is_built_without_torch():
     """The default target where Python has no torch (here: no site packages) is the library alone; where it has, the binding too, without a path to that torch in it."""
     root = Path(__file__).resolve().parents[1]
